@@ -515,6 +515,33 @@ int ugpg_relu_bwd(const float* y, const float* dy, float* dx, int64_t n, void* s
 /* elementwise y = x * mask (dropout with a precomputed scaled mask) */
 int ugpg_mul(const float* x, const float* m, float* y, int64_t n, void* stream);
 
+/* ---- Group normalisation with an activation, channels last ------------------
+ * x, y [B][HW][C], dtype UGPG_DT_F32 or UGPG_DT_BF16 (arithmetic and statistics in fp32);
+ * G groups of C/G consecutive channels; gamma, beta [C] fp32 or NULL (1, 0):
+ *   xh = (x - mean) * rstd,  rstd = 1/sqrt(var + eps) over a sample's group (biased var)
+ *   y = act(xh * gamma + beta)
+ * mean, rstd [B][G] fp32 are written (the backward reads them).  Statistics are centred
+ * (no sum of squares), sums have a fixed order.  The normalisation of a DoubleConv whose
+ * batch is too small for BatchNorm; the reference has BatchNorm only. */
+#define UGPG_ACT_NONE 0
+#define UGPG_ACT_RELU 1
+#define UGPG_ACT_SILU 2
+size_t ugpg_group_norm_workspace(int B, int64_t HW, int C, int G, int backward);
+int ugpg_group_norm_fwd(const void* x, int dtype, int B, int64_t HW, int C, int G,
+                        const float* gamma, const float* beta, float eps, int act, void* y,
+                        float* mean, float* rstd, void* ws, size_t ws_bytes, void* stream);
+/* With dp = dy * act'(xh*gamma + beta):
+ *   dx = rstd * (gamma*dp - mean_g(gamma*dp) - xh*mean_g(gamma*dp*xh))
+ *   dgamma = sum dp*xh;  dbeta = sum dp;  dxsum = sum over pixels and samples of dx (the
+ *   gradient of a bias added to x: the convolution's in front); each [C] or NULL.
+ * (x, dy, dx) types: all fp32, all bf16, bf16 with fp32 dy and dx, or bf16 with fp32 dy.
+ * dx may alias dy where the types agree. */
+int ugpg_group_norm_bwd(const void* dy, int dy_dtype, const void* x, int dtype, int B,
+                        int64_t HW, int C, int G, const float* mean, const float* rstd,
+                        const float* gamma, const float* beta, int act, void* dx, int dx_dtype,
+                        float* dgamma, float* dbeta, float* dxsum, void* ws, size_t ws_bytes,
+                        void* stream);
+
 /* ---- MoNuSeg augmentation (aug_monuseg_dataset.py:113-148,
  * monuseg_dataset.py:137-190): PIL's 8-bit arithmetic reproduced on the GPU. -------- */
 /* One separable pass of PIL's antialiasing resampler (Image.resize BILINEAR): `outer`

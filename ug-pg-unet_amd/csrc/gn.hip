@@ -1,0 +1,954 @@
+// Group normalisation with an activation on channels-last activations [B][P][C] (P pixels):
+//   mean, var over the P * (C/G) values of one sample's group;  xh = (x - mean) * rstd
+//   p = xh * gamma + beta;  y = act(p)                      act: none, ReLU, SiLU
+// and its backward: dp = dy * act'(p);  dbeta = sum dp;  dgamma = sum dp * xh
+//   dx = rstd * (gamma*dp - s1 - xh*s2),  s1, s2 = group means of gamma*dp, gamma*dp*xh
+// Memory-bound (a few operations per value).  Two forms:
+//   one pass ("resident"): a block owns a slab of whole groups of one sample and holds it in
+//     registers between the statistics and the result, so every value is read once;
+//   two passes: a slab too large for a block is cut into chunks of pixels; per-chunk partials
+//     are merged (fp64), then a second pass applies them.
+// Statistics are centred: (mean, M2) of short runs merged by Chan's rule, or the mean first
+// and squares of differences after, never sum(x^2) - n*mean^2.  No atomics: every sum has a
+// fixed order.
+#include "common.h"
+
+namespace ugpg {
+
+// ---------------------------------------------------------------- vector access
+template <int N> struct RawBytes;
+template <> struct RawBytes<2> { typedef uint16_t t; };
+template <> struct RawBytes<4> { typedef uint32_t t; };
+template <> struct RawBytes<8> { typedef uint2 t; };
+template <> struct RawBytes<16> { typedef uint4 t; };
+template <> struct RawBytes<32> { struct t { uint4 a, b; }; };
+
+// V consecutive values of T as loaded (bf16 stays packed: half the registers)
+template <typename T, int V> struct Pack {
+    union {
+        typename RawBytes<sizeof(T) * V>::t raw;
+        uint32_t w[sizeof(T) * V >= 4 ? sizeof(T) * V / 4 : 1];
+        uint16_t h[sizeof(T) * V / 2];
+    };
+    __device__ __forceinline__ Pack() {}
+    __device__ __forceinline__ void load(const T* p) {
+        raw = *reinterpret_cast<const typename RawBytes<sizeof(T) * V>::t*>(p);
+    }
+    __device__ __forceinline__ float get(int e) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[e]);
+        } else if constexpr (V == 1) {
+            return __uint_as_float((uint32_t)h[0] << 16);
+        } else {
+            return __uint_as_float((e & 1) ? (w[e / 2] & 0xffff0000u) : (w[e / 2] << 16));
+        }
+    }
+    __device__ __forceinline__ void set(int e, float v) {
+        if constexpr (sizeof(T) == 4) {
+            w[e] = __float_as_uint(v);
+        } else {
+            union { __bf16 b; uint16_t u; } c;
+            c.b = (__bf16)v;  // round to nearest even: half a bf16 step, once, at the store
+            h[e] = c.u;
+        }
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        *reinterpret_cast<typename RawBytes<sizeof(T) * V>::t*>(p) = raw;
+    }
+};
+
+__device__ __forceinline__ float gn_act(float p, int act) {
+    if (act == UGPG_ACT_RELU) return p < 0.f ? 0.f : p;  // (a NaN stays one)
+    if (act == UGPG_ACT_SILU) return p / (1.f + __expf(-p));
+    return p;
+}
+// dy * act'(p)
+__device__ __forceinline__ float gn_act_bwd(float dy, float p, int act) {
+    if (act == UGPG_ACT_RELU) return p > 0.f ? dy : (p != p ? p : 0.f);
+    if (act == UGPG_ACT_SILU) {
+        const float s = 1.f / (1.f + __expf(-p));
+        return dy * (s * fmaf(p, 1.f - s, 1.f));
+    }
+    return dy;
+}
+
+// ---------------------------------------------------------------- two passes
+// Block (b, chunk, column block): cb vector columns x `rows` pixel rows of threads, each
+// thread keeps its V channels and steps over the chunk's pixels.
+struct GnGeom {
+    int64_t P, ppc;  // pixels of a sample, pixels per chunk
+    int C, G, cpg;
+    int cb, rows, ncol, nchunk;
+};
+struct GnPos {
+    int b, chunk, c, row;  // c: first channel of the thread's vector
+    bool on;
+    int64_t p0, p1;
+};
+template <int V> __device__ __forceinline__ GnPos gn_pos(const GnGeom& g, unsigned id) {
+    GnPos r;
+    const int col = id % g.ncol;
+    const unsigned rest = id / g.ncol;
+    r.chunk = rest % g.nchunk;
+    r.b = rest / g.nchunk;
+    r.row = threadIdx.x / g.cb;
+    r.c = (col * g.cb + threadIdx.x % g.cb) * V;
+    r.on = r.row < g.rows && r.c < g.C;
+    r.p0 = (int64_t)r.chunk * g.ppc;
+    r.p1 = r.p0 + g.ppc < g.P ? r.p0 + g.ppc : g.P;
+    return r;
+}
+
+// per-channel (mean, M2) of a chunk -> part[b][chunk][2][C]
+template <typename T, int V>
+__global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, GnGeom g, float* part) {
+    constexpr int U = 8;
+    __shared__ float s_mean[256 * V], s_m2[256 * V], s_n[256];
+    const GnPos q = gn_pos<V>(g, blockIdx.x);
+    float n = 0.f, mean[V], m2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) mean[e] = m2[e] = 0.f;
+    if (q.on) {
+        const T* xb = x + ((size_t)q.b * g.P) * g.C + q.c;
+        int64_t p = q.p0 + q.row;
+        const int64_t step = g.rows;
+        for (; p + (U - 1) * step < q.p1; p += U * step) {
+            Pack<T, V> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u].load(xb + (size_t)(p + u * step) * g.C);
+            const float rn = 1.f / (n + U);
+            const float wb = U * rn, wq = n * U * rn;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                float s = 0.f, d2 = 0.f;
+#pragma unroll
+                for (int u = 0; u < U; ++u) s += v[u].get(e);
+                const float mb = s * (1.f / U);
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const float d = v[u].get(e) - mb;
+                    d2 = fmaf(d, d, d2);
+                }
+                const float dm = mb - mean[e];
+                mean[e] = fmaf(dm, wb, mean[e]);
+                m2[e] += fmaf(dm * dm, wq, d2);
+            }
+            n += U;
+        }
+        for (; p < q.p1; p += step) {
+            Pack<T, V> v;
+            v.load(xb + (size_t)p * g.C);
+            n += 1.f;
+            const float rn = 1.f / n;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = v.get(e) - mean[e];
+                mean[e] = fmaf(d, rn, mean[e]);
+                m2[e] = fmaf(d, v.get(e) - mean[e], m2[e]);
+            }
+        }
+    }
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        s_mean[e * 256 + t] = mean[e];
+        s_m2[e * 256 + t] = m2[e];
+    }
+    s_n[t] = n;
+    int top = 1;
+    while (top < g.rows) top <<= 1;
+    for (int s = top >> 1; s > 0; s >>= 1) {
+        __syncthreads();
+        if (q.on && q.row < s && q.row + s < g.rows) {
+            const int o = t + s * g.cb;
+            const float nb = s_n[o];
+            if (nb > 0.f) {
+                const float rn = 1.f / (n + nb);
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float dm = s_mean[e * 256 + o] - mean[e];
+                    mean[e] = fmaf(dm, nb * rn, mean[e]);
+                    m2[e] += fmaf(dm * dm, n * nb * rn, s_m2[e * 256 + o]);
+                    s_mean[e * 256 + t] = mean[e];
+                    s_m2[e * 256 + t] = m2[e];
+                }
+                n += nb;
+                s_n[t] = n;
+            }
+        }
+    }
+    if (q.on && q.row == 0) {
+        float* o = part + ((size_t)(q.b * (int64_t)g.nchunk + q.chunk) * 2) * g.C + q.c;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            o[e] = mean[e];
+            o[g.C + e] = m2[e];
+        }
+    }
+}
+
+// one wave per (sample, group): the chunks' partials -> mean, rstd
+__global__ void __launch_bounds__(256) gn_merge_kernel(const float* part, GnGeom g, int B,
+                                                       float eps, float* mean, float* rstd) {
+    const int64_t id = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    const int lane = threadIdx.x & 63;
+    if (id >= (int64_t)B * g.G) return;
+    const int b = id / g.G, gr = id % g.G;
+    const float* pb = part + (size_t)b * g.nchunk * 2 * g.C + gr * g.cpg;
+    const int n = g.nchunk * g.cpg;
+    const double cnt = (double)g.P * g.cpg;
+    double s = 0;
+    for (int i = lane; i < n; i += 64) {
+        const int ch = i / g.cpg, c = i % g.cpg;
+        const int64_t left = g.P - (int64_t)ch * g.ppc;
+        const double np = left < g.ppc ? left : g.ppc;
+        s += np * (double)pb[(size_t)ch * 2 * g.C + c];
+    }
+    const double mu = wave_sum_d(s) / cnt;
+    double q = 0;
+    for (int i = lane; i < n; i += 64) {
+        const int ch = i / g.cpg, c = i % g.cpg;
+        const int64_t left = g.P - (int64_t)ch * g.ppc;
+        const double np = left < g.ppc ? left : g.ppc;
+        const double d = (double)pb[(size_t)ch * 2 * g.C + c] - mu;
+        q += (double)pb[((size_t)ch * 2 + 1) * g.C + c] + np * d * d;
+    }
+    q = wave_sum_d(q);
+    if (lane == 0) {
+        mean[id] = (float)mu;
+        rstd[id] = (float)(1.0 / sqrt(q / cnt + (double)eps));
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(256) gn_apply_kernel(const T* x, GnGeom g, const float* mean,
+                                                       const float* rstd, const float* gamma,
+                                                       const float* beta, int act, T* y) {
+    constexpr int U = 4;
+    const GnPos q = gn_pos<V>(g, blockIdx.x);
+    if (!q.on) return;
+    float mu[V], a[V], h[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const int gi = q.b * g.G + (q.c + e) / g.cpg;
+        mu[e] = mean[gi];
+        a[e] = rstd[gi] * (gamma ? gamma[q.c + e] : 1.f);
+        h[e] = beta ? beta[q.c + e] : 0.f;
+    }
+    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
+    const int64_t step = g.rows;
+    int64_t p = q.p0 + q.row;
+    for (; p + (U - 1) * step < q.p1; p += U * step) {
+        Pack<T, V> v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].load(x + base + (size_t)(p + u * step) * g.C);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                o.set(e, gn_act(fmaf(v[u].get(e) - mu[e], a[e], h[e]), act));
+            o.store(y + base + (size_t)(p + u * step) * g.C);
+        }
+    }
+    for (; p < q.p1; p += step) {
+        Pack<T, V> v, o;
+        v.load(x + base + (size_t)p * g.C);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o.set(e, gn_act(fmaf(v.get(e) - mu[e], a[e], h[e]), act));
+        o.store(y + base + (size_t)p * g.C);
+    }
+}
+
+// per-channel (sum dp, sum dp*xh, sum xh) of a chunk -> part[b][chunk][3][C]
+template <typename T, typename TD, int V>
+__global__ void __launch_bounds__(256) gn_bwd_reduce_kernel(const TD* dy, const T* x, GnGeom g,
+                                                            const float* mean, const float* rstd,
+                                                            const float* gamma, const float* beta,
+                                                            int act, float* part) {
+    constexpr int U = 4;
+    __shared__ float s_a[256 * V], s_b[256 * V], s_x[256 * V];
+    const GnPos q = gn_pos<V>(g, blockIdx.x);
+    float sa[V], sb[V], sx[V], mu[V], rs[V], w[V], h[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) sa[e] = sb[e] = sx[e] = 0.f;
+    if (q.on) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int gi = q.b * g.G + (q.c + e) / g.cpg;
+            mu[e] = mean[gi];
+            rs[e] = rstd[gi];
+            w[e] = gamma ? gamma[q.c + e] : 1.f;
+            h[e] = beta ? beta[q.c + e] : 0.f;
+        }
+        const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
+        const int64_t step = g.rows;
+        int64_t p = q.p0 + q.row;
+        auto add = [&](const Pack<T, V>& v, const Pack<TD, V>& d) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float xh = (v.get(e) - mu[e]) * rs[e];
+                const float dp = gn_act_bwd(d.get(e), fmaf(xh, w[e], h[e]), act);
+                sa[e] += dp;
+                sb[e] = fmaf(dp, xh, sb[e]);
+                sx[e] += xh;
+            }
+        };
+        for (; p + (U - 1) * step < q.p1; p += U * step) {
+            Pack<T, V> v[U];
+            Pack<TD, V> d[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                v[u].load(x + base + (size_t)(p + u * step) * g.C);
+                d[u].load(dy + base + (size_t)(p + u * step) * g.C);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) add(v[u], d[u]);
+        }
+        for (; p < q.p1; p += step) {
+            Pack<T, V> v;
+            Pack<TD, V> d;
+            v.load(x + base + (size_t)p * g.C);
+            d.load(dy + base + (size_t)p * g.C);
+            add(v, d);
+        }
+    }
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        s_a[e * 256 + t] = sa[e];
+        s_b[e * 256 + t] = sb[e];
+        s_x[e * 256 + t] = sx[e];
+    }
+    int top = 1;
+    while (top < g.rows) top <<= 1;
+    for (int s = top >> 1; s > 0; s >>= 1) {
+        __syncthreads();
+        if (q.on && q.row < s && q.row + s < g.rows) {
+            const int o = t + s * g.cb;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                s_a[e * 256 + t] += s_a[e * 256 + o];
+                s_b[e * 256 + t] += s_b[e * 256 + o];
+                s_x[e * 256 + t] += s_x[e * 256 + o];
+            }
+        }
+    }
+    if (q.on && q.row == 0) {
+        float* o = part + ((size_t)(q.b * (int64_t)g.nchunk + q.chunk) * 3) * g.C + q.c;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            o[e] = s_a[e * 256 + t];
+            o[g.C + e] = s_b[e * 256 + t];
+            o[2 * g.C + e] = s_x[e * 256 + t];
+        }
+    }
+}
+
+// block per (sample, group): the chunks' sums per channel -> tot[b][3][C], and the group's
+// s1, s2 -> sums[b][G][2]
+__global__ void __launch_bounds__(256) gn_bwd_merge_kernel(const float* part, GnGeom g,
+                                                           const float* gamma, float* tot,
+                                                           float* sums) {
+    __shared__ double sh[3][256];
+    const int b = blockIdx.x / g.G, gr = blockIdx.x % g.G, t = threadIdx.x;
+    const int ct = g.cpg < 256 ? g.cpg : 256, parts = 256 / ct;
+    const int cl = t % ct, pi = t / ct;
+    const double cnt = (double)g.P * g.cpg;
+    double s1 = 0, s2 = 0;
+    for (int c0 = 0; c0 < g.cpg; c0 += ct) {
+        const int c = gr * g.cpg + c0 + cl;
+        const bool on = pi < parts && c0 + cl < g.cpg;
+        double a = 0, bb = 0, xx = 0;
+        if (on)
+            for (int ch = pi; ch < g.nchunk; ch += parts) {
+                const float* pb = part + ((size_t)(b * (int64_t)g.nchunk + ch) * 3) * g.C + c;
+                a += pb[0];
+                bb += pb[g.C];
+                xx += pb[2 * g.C];
+            }
+        sh[0][t] = a;
+        sh[1][t] = bb;
+        sh[2][t] = xx;
+        __syncthreads();
+        if (on && pi == 0) {
+            for (int k = 1; k < parts; ++k) {
+                a += sh[0][k * ct + cl];
+                bb += sh[1][k * ct + cl];
+                xx += sh[2][k * ct + cl];
+            }
+            float* o = tot + (size_t)b * 3 * g.C + c;
+            o[0] = (float)a;
+            o[g.C] = (float)bb;
+            o[2 * g.C] = (float)xx;
+            const double w = gamma ? (double)gamma[c] : 1.0;
+            s1 += w * a;
+            s2 += w * bb;
+        }
+        __syncthreads();
+    }
+    sh[0][t] = s1;
+    sh[1][t] = s2;
+    __syncthreads();
+    for (int s = 128; s > 0; s >>= 1) {
+        if (t < s) {
+            sh[0][t] += sh[0][t + s];
+            sh[1][t] += sh[1][t + s];
+        }
+        __syncthreads();
+    }
+    if (t == 0) {
+        sums[2 * blockIdx.x] = (float)(sh[0][0] / cnt);
+        sums[2 * blockIdx.x + 1] = (float)(sh[1][0] / cnt);
+    }
+}
+
+// dgamma, dbeta and the sum of dx per channel (the gradient of a bias added to x), from the
+// samples' totals: sum_p dx = rstd * (gamma*A - P*s1 - s2*X) per sample, A = sum dp, X = sum xh
+__device__ void gn_param_grads(int c, int B, int64_t P, int C, int G, int cpg, const float* tot,
+                               const float* sums, const float* rstd, const float* gamma,
+                               float* dgamma, float* dbeta, float* dxsum) {
+    double a = 0, bb = 0, d = 0;
+    const int gr = c / cpg;
+    const double w = gamma ? (double)gamma[c] : 1.0;
+    for (int b = 0; b < B; ++b) {
+        const float* o = tot + (size_t)b * 3 * C + c;
+        a += o[0];
+        bb += o[C];
+        const float* s = sums + 2 * ((size_t)b * G + gr);
+        d += (double)rstd[(size_t)b * G + gr] *
+             (w * o[0] - (double)P * s[0] - (double)s[1] * o[2 * C]);
+    }
+    if (dbeta) dbeta[c] = (float)a;
+    if (dgamma) dgamma[c] = (float)bb;
+    if (dxsum) dxsum[c] = (float)d;
+}
+
+// dx; the blocks past `napply` sum the parameters' gradients over the samples
+template <typename T, typename TD, typename TO, int V>
+__global__ void __launch_bounds__(256) gn_bwd_apply_kernel(
+    const TD* dy, const T* x, GnGeom g, int B, unsigned napply, const float* mean,
+    const float* rstd, const float* gamma, const float* beta, int act, const float* tot,
+    const float* sums, TO* dx, float* dgamma, float* dbeta, float* dxsum) {
+    constexpr int U = 4;
+    if (blockIdx.x >= napply) {
+        const int c = (blockIdx.x - napply) * 256 + threadIdx.x;
+        if (c < g.C)
+            gn_param_grads(c, B, g.P, g.C, g.G, g.cpg, tot, sums, rstd, gamma, dgamma, dbeta, dxsum);
+        return;
+    }
+    const GnPos q = gn_pos<V>(g, blockIdx.x);
+    if (!q.on) return;
+    float mu[V], rs[V], w[V], h[V], s1[V], s2[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const int gi = q.b * g.G + (q.c + e) / g.cpg;
+        mu[e] = mean[gi];
+        rs[e] = rstd[gi];
+        w[e] = gamma ? gamma[q.c + e] : 1.f;
+        h[e] = beta ? beta[q.c + e] : 0.f;
+        s1[e] = sums[2 * gi];
+        s2[e] = sums[2 * gi + 1];
+    }
+    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
+    const int64_t step = g.rows;
+    auto one = [&](const Pack<T, V>& v, const Pack<TD, V>& d, size_t off) {
+        Pack<TO, V> o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const float xh = (v.get(e) - mu[e]) * rs[e];
+            const float dp = gn_act_bwd(d.get(e), fmaf(xh, w[e], h[e]), act);
+            o.set(e, rs[e] * fmaf(-xh, s2[e], fmaf(w[e], dp, -s1[e])));
+        }
+        o.store(dx + off);
+    };
+    int64_t p = q.p0 + q.row;
+    for (; p + (U - 1) * step < q.p1; p += U * step) {
+        Pack<T, V> v[U];
+        Pack<TD, V> d[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u].load(x + base + (size_t)(p + u * step) * g.C);
+            d[u].load(dy + base + (size_t)(p + u * step) * g.C);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) one(v[u], d[u], base + (size_t)(p + u * step) * g.C);
+    }
+    for (; p < q.p1; p += step) {
+        Pack<T, V> v;
+        Pack<TD, V> d;
+        v.load(x + base + (size_t)p * g.C);
+        d.load(dy + base + (size_t)p * g.C);
+        one(v, d, base + (size_t)p * g.C);
+    }
+}
+
+// ---------------------------------------------------------------- one pass
+// Block = (sample, slab of gb whole groups): thread (row, col) holds the V channels `col` of
+// the pixels row, row + rows, ...  (NV of them at most) in registers as loaded.  V divides a
+// group, so a thread's vector lies in one group.
+struct GnSlab {
+    int64_t P;
+    int C, G, cpg, gb, nslab, scv, rows;
+};
+struct GnSlabPos {
+    int b, g0, ng, col, row, c, gl;
+    bool on;
+};
+template <int V> __device__ __forceinline__ GnSlabPos gn_slab_pos(const GnSlab& g) {
+    GnSlabPos r;
+    r.b = blockIdx.x / g.nslab;
+    r.g0 = (blockIdx.x % g.nslab) * g.gb;
+    r.ng = g.G - r.g0 < g.gb ? g.G - r.g0 : g.gb;
+    r.col = threadIdx.x % g.scv;
+    r.row = threadIdx.x / g.scv;
+    r.gl = r.col * V / g.cpg;
+    r.c = r.g0 * g.cpg + r.col * V;
+    r.on = r.row < g.rows && r.gl < r.ng;
+    return r;
+}
+
+// sum of v over the block's threads of the caller's group (one wave per group, fixed order)
+template <int V>
+__device__ __forceinline__ float gn_group_sum(float v, const GnSlab& g, const GnSlabPos& q,
+                                              float* red, float* out) {
+    __syncthreads();
+    red[threadIdx.x] = q.on ? v : 0.f;
+    __syncthreads();
+    const int nw = blockDim.x / 64, w = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const int vpg = g.cpg / V, n = vpg * g.rows;
+    for (int k = w; k < q.ng; k += nw) {
+        float s = 0.f;
+        for (int j = lane; j < n; j += 64) s += red[j / vpg * g.scv + k * vpg + j % vpg];
+        s = wave_sum(s);
+        if (lane == 0) out[k] = s;
+    }
+    __syncthreads();
+    return q.on ? out[q.gl] : 0.f;
+}
+
+constexpr int GN_GB = 64;  // groups of a slab at most
+
+template <typename T, int V, int NV>
+__global__ void __launch_bounds__(1024) gn_fwd_res_kernel(const T* x, GnSlab g, const float* gamma,
+                                                          const float* beta, float eps, int act,
+                                                          T* y, float* mean, float* rstd) {
+    __shared__ float red[1024], out[GN_GB];
+    const GnSlabPos q = gn_slab_pos<V>(g);
+    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
+    Pack<T, V> v[NV];
+    float w[V], h[V];
+    if (q.on) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t p = q.row + (int64_t)i * g.rows;
+            if (p < g.P) v[i].load(x + base + (size_t)p * g.C);
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            w[e] = gamma ? gamma[q.c + e] : 1.f;
+            h[e] = beta ? beta[q.c + e] : 0.f;
+        }
+    }
+    float s = 0.f;
+    if (q.on) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (q.row + (int64_t)i * g.rows < g.P) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) s += v[i].get(e);
+            }
+    }
+    const float rn = 1.f / ((float)g.P * (float)g.cpg);
+    const float mu = gn_group_sum<V>(s, g, q, red, out) * rn;
+    s = 0.f;
+    if (q.on) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (q.row + (int64_t)i * g.rows < g.P) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float d = v[i].get(e) - mu;
+                    s = fmaf(d, d, s);
+                }
+            }
+    }
+    const float var = gn_group_sum<V>(s, g, q, red, out) * rn;
+    const float rs = 1.f / sqrtf(var + eps);
+    if (!q.on) return;
+    if (q.row == 0 && q.col * V % g.cpg == 0) {
+        mean[(size_t)q.b * g.G + q.g0 + q.gl] = mu;
+        rstd[(size_t)q.b * g.G + q.g0 + q.gl] = rs;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) w[e] *= rs;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int64_t p = q.row + (int64_t)i * g.rows;
+        if (p < g.P) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                o.set(e, gn_act(fmaf(v[i].get(e) - mu, w[e], h[e]), act));
+            o.store(y + base + (size_t)p * g.C);
+        }
+    }
+}
+
+// per-channel sums over the block's rows: each thread's v[V] -> tot[scv * V]
+template <int V>
+__device__ __forceinline__ void gn_channel_sums(const float (&v)[V], const GnSlab& g, bool on,
+                                                float* red, float* tot) {
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < V; ++e) red[e * 1024 + threadIdx.x] = on ? v[e] : 0.f;
+    __syncthreads();
+    const int nw = blockDim.x / 64, w = threadIdx.x / 64, lane = threadIdx.x & 63;
+    for (int k = w; k < g.scv * V; k += nw) {
+        const float* r = red + (k % V) * 1024 + k / V;
+        float s = 0.f;
+        for (int j = lane; j < g.rows; j += 64) s += r[j * g.scv];
+        s = wave_sum(s);
+        if (lane == 0) tot[k] = s;
+    }
+}
+
+template <typename T, typename TD, typename TO, int V, int NV>
+__global__ void __launch_bounds__(1024) gn_bwd_res_kernel(
+    const TD* dy, const T* x, GnSlab g, const float* mean, const float* rstd, const float* gamma,
+    const float* beta, int act, TO* dx, float* tot, float* sums) {
+    __shared__ float red[1024 * V], ta[1024], tb[1024], tx[1024], s12[2 * GN_GB];
+    const GnSlabPos q = gn_slab_pos<V>(g);
+    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
+    Pack<T, V> v[NV];
+    Pack<TD, V> d[NV];
+    float w[V], h[V], sa[V], sb[V], sx[V], mu = 0.f, rs = 0.f;
+#pragma unroll
+    for (int e = 0; e < V; ++e) sa[e] = sb[e] = sx[e] = w[e] = h[e] = 0.f;
+    if (q.on) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t p = q.row + (int64_t)i * g.rows;
+            if (p < g.P) {
+                v[i].load(x + base + (size_t)p * g.C);
+                d[i].load(dy + base + (size_t)p * g.C);
+            }
+        }
+        mu = mean[(size_t)q.b * g.G + q.g0 + q.gl];
+        rs = rstd[(size_t)q.b * g.G + q.g0 + q.gl];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            w[e] = gamma ? gamma[q.c + e] : 1.f;
+            h[e] = beta ? beta[q.c + e] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (q.row + (int64_t)i * g.rows < g.P) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    const float xh = (v[i].get(e) - mu) * rs;
+                    const float dp = gn_act_bwd(d[i].get(e), fmaf(xh, w[e], h[e]), act);
+                    sa[e] += dp;
+                    sb[e] = fmaf(dp, xh, sb[e]);
+                    sx[e] += xh;
+                }
+            }
+    }
+    gn_channel_sums<V>(sa, g, q.on, red, ta);
+    gn_channel_sums<V>(sb, g, q.on, red, tb);
+    gn_channel_sums<V>(sx, g, q.on, red, tx);
+    __syncthreads();
+    const int nw = blockDim.x / 64, wv = threadIdx.x / 64, lane = threadIdx.x & 63;
+    const float rn = 1.f / ((float)g.P * (float)g.cpg);
+    for (int k = wv; k < q.ng; k += nw) {
+        float s1 = 0.f, s2 = 0.f;
+        for (int j = lane; j < g.cpg; j += 64) {
+            const int c = k * g.cpg + j;
+            const float gm = gamma ? gamma[q.g0 * g.cpg + c] : 1.f;
+            s1 = fmaf(gm, ta[c], s1);
+            s2 = fmaf(gm, tb[c], s2);
+        }
+        s1 = wave_sum(s1) * rn;
+        s2 = wave_sum(s2) * rn;
+        if (lane == 0) {
+            s12[2 * k] = s1;
+            s12[2 * k + 1] = s2;
+            float* o = sums + 2 * ((size_t)q.b * g.G + q.g0 + k);
+            o[0] = s1;
+            o[1] = s2;
+        }
+    }
+    for (int k = threadIdx.x; k < q.ng * g.cpg; k += blockDim.x) {
+        float* o = tot + (size_t)q.b * 3 * g.C + q.g0 * g.cpg + k;
+        o[0] = ta[k];
+        o[g.C] = tb[k];
+        o[2 * g.C] = tx[k];
+    }
+    __syncthreads();
+    if (!q.on) return;
+    const float s1 = s12[2 * q.gl], s2 = s12[2 * q.gl + 1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int64_t p = q.row + (int64_t)i * g.rows;
+        if (p < g.P) {
+            Pack<TO, V> o;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float xh = (v[i].get(e) - mu) * rs;
+                const float dp = gn_act_bwd(d[i].get(e), fmaf(xh, w[e], h[e]), act);
+                o.set(e, rs * fmaf(-xh, s2, fmaf(w[e], dp, -s1)));
+            }
+            o.store(dx + base + (size_t)p * g.C);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) gn_params_kernel(int B, int64_t P, int C, int G,
+                                                        const float* tot, const float* sums,
+                                                        const float* rstd, const float* gamma,
+                                                        float* dgamma, float* dbeta, float* dxsum) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c < C) gn_param_grads(c, B, P, C, G, C / G, tot, sums, rstd, gamma, dgamma, dbeta, dxsum);
+}
+
+// ---------------------------------------------------------------- host side
+// The one-pass form, where a slab of whole groups fits the registers of a block: at most
+// `nvmax` vectors a thread, 1024 threads.  A pixel's slab is 128 bytes (whole lines) where
+// that leaves 256 blocks, else 64; never less unless the pixel is.  Returns the vectors a
+// thread holds (0: does not fit) and the block size.
+static int gn_slab(int B, int64_t P, int C, int G, int V, int es, int nvmax, GnSlab* o, int* nt) {
+    const int cpg = C / G;
+    if (cpg % V) return 0;
+    for (int target = 128; target >= 64; target -= 64) {
+        int gb = (int)cdiv(target, (int64_t)cpg * es);
+        if (gb > G) gb = G;
+        if (gb > GN_GB) gb = GN_GB;
+        const int64_t scv = (int64_t)gb * cpg / V;
+        if ((int64_t)gb * cpg > 1024) continue;  // (the block's per-channel sums)
+        const int nslab = (int)cdiv(G, gb);
+        if (target == 128 && (int64_t)B * nslab < 256 && cpg * es < 128) continue;
+        for (int n = 256; n <= 1024; n *= 2) {
+            const int rows = n / (int)scv;
+            if (rows == 0) continue;
+            const int64_t nv = cdiv(P, rows);
+            if (nv > (n < 1024 ? 4 : nvmax)) continue;
+            *o = GnSlab{P, C, G, cpg, gb, nslab, (int)scv, rows};
+            *nt = n;
+            return (int)nv;
+        }
+    }
+    return 0;
+}
+
+// widest vector (values) that divides C and that every tensor's address allows
+static int gn_vec(int C, int es_max, const void* a, int ea, const void* b, int eb, const void* c,
+                  int ec) {
+    for (int v = es_max; v > 1; v >>= 1) {
+        if (C % v) continue;
+        auto ok = [v](const void* p, int es) {
+            const int n = v * es < 16 ? v * es : 16;
+            return ((uintptr_t)p % n) == 0;
+        };
+        if (ok(a, ea) && ok(b, eb) && ok(c, ec)) return v;
+    }
+    return 1;
+}
+
+// The vector width of a call: the widest at which the one-pass form fits (its vectors lie in
+// one group), else the widest that C and the addresses allow.
+static int gn_pick(int B, int64_t P, int C, int G, int vmax, int es, int nvmax) {
+    GnSlab o;
+    int nt;
+    for (int v = vmax; v >= 1; v >>= 1)
+        if (gn_slab(B, P, C, G, v, es, nvmax, &o, &nt)) return v;
+    return vmax;
+}
+
+static GnGeom gn_geom(int B, int64_t P, int C, int G, int V) {
+    GnGeom g;
+    g.P = P;
+    g.C = C;
+    g.G = G;
+    g.cpg = C / G;
+    const int cv = C / V;
+    g.ncol = (int)cdiv(cv, 256);
+    g.cb = (int)cdiv(cv, g.ncol);
+    g.rows = 256 / g.cb;
+    // about 2048 blocks (8 per CU), no chunk below 8 pixels a thread, at most 512 chunks
+    int64_t want = cdiv(2048, (int64_t)B * g.ncol);
+    const int64_t most = cdiv(P, (int64_t)g.rows * 8);
+    if (want > most) want = most;
+    if (want > 512) want = 512;
+    if (want < 1) want = 1;
+    g.ppc = cdiv(P, want);
+    g.nchunk = (int)cdiv(P, g.ppc);
+    return g;
+}
+
+static int gn_check(const char* what, const void* x, int B, int64_t P, int C, int G, int act) {
+    if (!x || B <= 0 || P <= 0 || C <= 0 || G <= 0 || C % G || act < UGPG_ACT_NONE ||
+        act > UGPG_ACT_SILU) {
+        set_error("%s: bad arguments (B=%d HW=%lld C=%d groups=%d act=%d)", what, B, (long long)P, C,
+                  G, act);
+        return UGPG_ERR_INVALID;
+    }
+    // (grids: B*G blocks, B * column blocks; offsets are 64-bit)
+    if (C > (1 << 20) || (int64_t)B * G > (1 << 22) || (int64_t)B * cdiv(C, 256) > (1 << 22) ||
+        P > ((int64_t)1 << 40) || (double)B * (double)P * (double)C > 1e15) {
+        set_error("%s: B=%d HW=%lld C=%d is too large", what, B, (long long)P, C);
+        return UGPG_ERR_INVALID;
+    }
+    return UGPG_OK;
+}
+
+// chunk count at the narrowest vector bounds it at every vector width (rows only shrinks)
+static size_t gn_part_floats(int B, int64_t P, int C, int G, int per) {
+    size_t most = 0;
+    for (int v = 8; v >= 1; v >>= 1) {
+        if (C % v) continue;
+        const GnGeom g = gn_geom(B, P, C, G, v);
+        const size_t n = (size_t)B * g.nchunk * per * C;
+        if (n > most) most = n;
+    }
+    return most;
+}
+
+}  // namespace ugpg
+
+using namespace ugpg;
+
+extern "C" size_t ugpg_group_norm_workspace(int B, int64_t HW, int C, int G, int backward) {
+    if (B <= 0 || HW <= 0 || C <= 0 || G <= 0 || C % G) return 0;
+    if (!backward) return gn_part_floats(B, HW, C, G, 2) * 4;
+    return (gn_part_floats(B, HW, C, G, 3) + (size_t)B * 3 * C + (size_t)B * G * 2) * 4;
+}
+
+template <typename T, int V>
+static int gn_fwd_run(const void* x, int B, int64_t P, int C, int G, const float* gamma,
+                      const float* beta, float eps, int act, void* y, float* mean, float* rstd,
+                      void* ws, hipStream_t s) {
+    const T* xt = static_cast<const T*>(x);
+    GnSlab sl;
+    int nt;
+    if (const int nv = gn_slab(B, P, C, G, V, sizeof(T), 16, &sl, &nt)) {
+        const dim3 grid((unsigned)((int64_t)B * sl.nslab));
+#define GN_RES(NV) \
+    hipLaunchKernelGGL((gn_fwd_res_kernel<T, V, NV>), grid, dim3(nt), 0, s, xt, sl, gamma, beta, eps, act, \
+                       static_cast<T*>(y), mean, rstd)
+        if (nv <= 4) GN_RES(4);
+        else if (nv <= 8) GN_RES(8);
+        else GN_RES(16);
+#undef GN_RES
+        return check_launch("group_norm_fwd");
+    }
+    const GnGeom g = gn_geom(B, P, C, G, V);
+    const unsigned nb = (unsigned)((int64_t)B * g.nchunk * g.ncol);
+    float* part = static_cast<float*>(ws);
+    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3(nb), dim3(256), 0, s, xt, g, part);
+    hipLaunchKernelGGL(gn_merge_kernel, dim3((unsigned)cdiv((int64_t)B * G, 4)), dim3(256), 0, s,
+                       part, g, B, eps, mean, rstd);
+    hipLaunchKernelGGL((gn_apply_kernel<T, V>), dim3(nb), dim3(256), 0, s, xt, g, mean, rstd, gamma,
+                       beta, act, static_cast<T*>(y));
+    return check_launch("group_norm_fwd");
+}
+
+extern "C" int ugpg_group_norm_fwd(const void* x, int dtype, int B, int64_t HW, int C, int G,
+                                   const float* gamma, const float* beta, float eps, int act,
+                                   void* y, float* mean, float* rstd, void* ws, size_t ws_bytes,
+                                   void* stream) {
+    if (int rc = gn_check("group_norm_fwd", x, B, HW, C, G, act)) return rc;
+    if (!y || !mean || !rstd || !(eps >= 0.f) || (dtype != UGPG_DT_F32 && dtype != UGPG_DT_BF16)) {
+        set_error("group_norm_fwd: bad arguments (eps=%g dtype=%d)", (double)eps, dtype);
+        return UGPG_ERR_INVALID;
+    }
+    const size_t need = ugpg_group_norm_workspace(B, HW, C, G, 0);
+    if (!ws || ws_bytes < need) {
+        set_error("group_norm_fwd: workspace %zu < %zu", ws_bytes, need);
+        return UGPG_ERR_WORKSPACE;
+    }
+    const int es = dtype == UGPG_DT_F32 ? 4 : 2;
+    const int v = gn_pick(B, HW, C, G, gn_vec(C, 16 / es, x, es, y, es, nullptr, es), es, 16);
+    hipStream_t s = as_stream(stream);
+#define GN_FWD(T, V) gn_fwd_run<T, V>(x, B, HW, C, G, gamma, beta, eps, act, y, mean, rstd, ws, s)
+    if (es == 4) return v == 4 ? GN_FWD(float, 4) : v == 2 ? GN_FWD(float, 2) : GN_FWD(float, 1);
+    return v == 8 ? GN_FWD(__bf16, 8) : v == 4 ? GN_FWD(__bf16, 4) : v == 2 ? GN_FWD(__bf16, 2)
+                                                                         : GN_FWD(__bf16, 1);
+#undef GN_FWD
+}
+
+template <typename T, typename TD, typename TO, int V>
+static int gn_bwd_run(const void* dy, const void* x, int B, int64_t P, int C, int G,
+                      const float* mean, const float* rstd, const float* gamma, const float* beta,
+                      int act, void* dx, float* dgamma, float* dbeta, float* dxsum, void* ws,
+                      hipStream_t s) {
+    const T* xt = static_cast<const T*>(x);
+    const TD* dt = static_cast<const TD*>(dy);
+    float* tot = static_cast<float*>(ws);
+    float* sums = tot + (size_t)B * 3 * C;
+    float* part = sums + (size_t)B * G * 2;
+    const unsigned pblocks = dgamma || dbeta || dxsum ? (unsigned)cdiv(C, 256) : 0;
+    GnSlab sl;
+    int nt;
+    if (const int nv = gn_slab(B, P, C, G, V, sizeof(TD), 8, &sl, &nt)) {
+        const dim3 grid((unsigned)((int64_t)B * sl.nslab));
+#define GN_RES(NV) \
+    hipLaunchKernelGGL((gn_bwd_res_kernel<T, TD, TO, V, NV>), grid, dim3(nt), 0, s, dt, xt, sl, mean, rstd, \
+                       gamma, beta, act, static_cast<TO*>(dx), tot, sums)
+        if (nv <= 4) GN_RES(4);
+        else GN_RES(8);
+#undef GN_RES
+        if (pblocks)
+            hipLaunchKernelGGL(gn_params_kernel, dim3(pblocks), dim3(256), 0, s, B, P, C, G, tot, sums,
+                               rstd, gamma, dgamma, dbeta, dxsum);
+        return check_launch("group_norm_bwd");
+    }
+    const GnGeom g = gn_geom(B, P, C, G, V);
+    const unsigned nb = (unsigned)((int64_t)B * g.nchunk * g.ncol);
+    hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, TD, V>), dim3(nb), dim3(256), 0, s, dt, xt, g, mean,
+                       rstd, gamma, beta, act, part);
+    hipLaunchKernelGGL(gn_bwd_merge_kernel, dim3((unsigned)((int64_t)B * G)), dim3(256), 0, s, part,
+                       g, gamma, tot, sums);
+    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, TD, TO, V>), dim3(nb + pblocks), dim3(256), 0, s, dt, xt,
+                       g, B, nb, mean, rstd, gamma, beta, act, tot, sums, static_cast<TO*>(dx),
+                       dgamma, dbeta, dxsum);
+    return check_launch("group_norm_bwd");
+}
+
+extern "C" int ugpg_group_norm_bwd(const void* dy, int dy_dtype, const void* x, int dtype, int B,
+                                   int64_t HW, int C, int G, const float* mean, const float* rstd,
+                                   const float* gamma, const float* beta, int act, void* dx,
+                                   int dx_dtype, float* dgamma, float* dbeta, float* dxsum, void* ws,
+                                   size_t ws_bytes, void* stream) {
+    if (int rc = gn_check("group_norm_bwd", x, B, HW, C, G, act)) return rc;
+    const int F = UGPG_DT_F32, H = UGPG_DT_BF16;
+    const bool fff = dtype == F && dy_dtype == F && dx_dtype == F;
+    const bool hhh = dtype == H && dy_dtype == H && dx_dtype == H;
+    const bool hfh = dtype == H && dy_dtype == F && dx_dtype == H;
+    const bool hff = dtype == H && dy_dtype == F && dx_dtype == F;
+    if (!dy || !dx || !mean || !rstd || !(fff || hhh || hfh || hff)) {
+        set_error("group_norm_bwd: bad arguments (x, dy, dx types %d %d %d)", dtype, dy_dtype,
+                  dx_dtype);
+        return UGPG_ERR_INVALID;
+    }
+    const size_t need = ugpg_group_norm_workspace(B, HW, C, G, 1);
+    if (!ws || ws_bytes < need) {
+        set_error("group_norm_bwd: workspace %zu < %zu", ws_bytes, need);
+        return UGPG_ERR_WORKSPACE;
+    }
+    const int ex = dtype == F ? 4 : 2, ed = dy_dtype == F ? 4 : 2, eo = dx_dtype == F ? 4 : 2;
+    const int v = gn_pick(B, HW, C, G, gn_vec(C, 16 / ex, x, ex, dy, ed, dx, eo), ed, 8);
+    hipStream_t s = as_stream(stream);
+#define GN_BWD(T, TD, TO, V) \
+    gn_bwd_run<T, TD, TO, V>(dy, x, B, HW, C, G, mean, rstd, gamma, beta, act, dx, dgamma, dbeta, dxsum, ws, s)
+#define GN_BWD_H(TD, TO)                              \
+    (v == 8 ? GN_BWD(__bf16, TD, TO, 8) : v == 4 ? GN_BWD(__bf16, TD, TO, 4) \
+     : v == 2 ? GN_BWD(__bf16, TD, TO, 2) : GN_BWD(__bf16, TD, TO, 1))
+    if (fff)
+        return v == 4 ? GN_BWD(float, float, float, 4)
+               : v == 2 ? GN_BWD(float, float, float, 2) : GN_BWD(float, float, float, 1);
+    if (hhh) return GN_BWD_H(__bf16, __bf16);
+    if (hfh) return GN_BWD_H(float, __bf16);
+    return GN_BWD_H(float, float);
+#undef GN_BWD
+#undef GN_BWD_H
+}

@@ -141,6 +141,10 @@ SIGNATURES = {
     "ugpg_adam_step": (_i, [_p, _p, _p, _p, _i64, _f, _f, _f, _f, _f, _i64, _f, _p]),
     "ugpg_relu_bwd": (_i, [_p, _p, _p, _i64, _p]),
     "ugpg_mul": (_i, [_p, _p, _p, _i64, _p]),
+    "ugpg_group_norm_workspace": (_sz, [_i, _i64, _i, _i, _i]),
+    "ugpg_group_norm_fwd": (_i, [_p, _i, _i, _i64, _i, _i, _p, _p, _f, _i, _p, _p, _p, _p, _sz, _p]),
+    "ugpg_group_norm_bwd": (_i, [_p, _i, _p, _i, _i, _i64, _i, _i, _p, _p, _p, _p, _i, _p, _i, _p,
+                                 _p, _p, _p, _sz, _p]),
     "ugpg_resample_aa_u8": (_i, [_p, _i64, _i, _i, _i, _p, _p, _i, _p, _p]),
     "ugpg_resize_nearest_u8": (_i, [_p, _i64, _i, _i, _i, _p, _p, _p, _i, _i, _p]),
     "ugpg_augment_param_sizes": (_i, [C.POINTER(_i), C.POINTER(_i)]),

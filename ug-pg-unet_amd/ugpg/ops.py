@@ -6,6 +6,7 @@ Activations are NHWC fp32 ``(B, H, W, C)`` tensors.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 
@@ -18,6 +19,12 @@ F32 = torch.float32
 
 def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
+
+
+def on_device(t):
+    """Context: the device of `t` is current (a launch goes to its stream, whatever device
+    the caller left current)."""
+    return torch.cuda.device(t.device) if t.is_cuda else contextlib.nullcontext()
 
 
 def ptr(t):
@@ -453,6 +460,45 @@ def bn_relu_bwd(da, y, mean, invstd, scale, shift, dy, dgamma, dbeta, dconv_bias
     check(lib.ugpg_bn_relu_bwd(ptr(da), *_yargs(y), npix, c, ptr(mean), ptr(invstd), ptr(scale),
                                ptr(shift), *_yargs(dy), ptr(dgamma), ptr(dbeta), ptr(dconv_bias),
                                int(accumulate), ptr(ws), ws.numel(), stream()), "bn_relu_bwd")
+
+
+# ------------------------------------------------------------------ group norm
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2}
+
+
+def _dtype_code(t):
+    if t.dtype == F32:
+        return 0
+    if t.dtype == torch.bfloat16:
+        return 1
+    raise TypeError(f"ugpg: expected float32 or bfloat16, got {t.dtype}")
+
+
+def group_norm_fwd(x, groups, gamma, beta, eps, act):
+    """x (B, ..., C) channels last -> (act(group_norm(x)), mean, rstd), the last two (B, G)."""
+    B, c = x.shape[0], x.shape[-1]
+    hw = x.numel() // (B * c)
+    y = torch.empty_like(x)
+    mean, rstd = empty(B, groups, like=x), empty(B, groups, like=x)
+    ws = workspace(lib.ugpg_group_norm_workspace(B, hw, c, groups, 0), x.device)
+    check(lib.ugpg_group_norm_fwd(ptr(x), _dtype_code(x), B, hw, c, groups, ptr(gamma), ptr(beta),
+                                  float(eps), ACTIVATIONS[act], ptr(y), ptr(mean), ptr(rstd),
+                                  ptr(ws), ws.numel(), stream()), "group_norm_fwd")
+    return y, mean, rstd
+
+
+def group_norm_bwd(dy, x, groups, mean, rstd, gamma, beta, act, dx, dgamma=None, dbeta=None,
+                   dxsum=None):
+    """dx (may be dy) and, where given, dgamma, dbeta and the per-channel sum of dx (the bias
+    gradient of the convolution that wrote x)."""
+    B, c = x.shape[0], x.shape[-1]
+    hw = x.numel() // (B * c)
+    ws = workspace(lib.ugpg_group_norm_workspace(B, hw, c, groups, 1), x.device)
+    check(lib.ugpg_group_norm_bwd(ptr(dy), _dtype_code(dy), ptr(x), _dtype_code(x), B, hw, c, groups,
+                                  ptr(mean), ptr(rstd), ptr(gamma), ptr(beta), ACTIVATIONS[act],
+                                  ptr(dx), _dtype_code(dx), ptr(dgamma), ptr(dbeta), ptr(dxsum),
+                                  ptr(ws), ws.numel(), stream()), "group_norm_bwd")
+    return dx
 
 
 # ------------------------------------------------------------------ pool / resize
