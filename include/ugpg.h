@@ -542,6 +542,55 @@ int ugpg_group_norm_bwd(const void* dy, int dy_dtype, const void* x, int dtype, 
                         float* dgamma, float* dbeta, float* dxsum, void* ws, size_t ws_bytes,
                         void* stream);
 
+/* ---- A teacher's top logits, and distillation from them ----------------------
+ * The previous stage as a teacher (the reference only weights by its uncertainty): a record
+ * of its output, and the loss of the current stage against that record.
+ * Rows: N rows of V logits (inner == 1; row r at logits + r*stride, stride >= V), or the
+ * pixels of N class maps [V][inner] (inner > 1, stride == V*inner).  dtype UGPG_DT_F32 or
+ * UGPG_DT_BF16.  1 <= k <= min(V, 256).  With t a row's logits at temperature T:
+ *   values, indices [N][k][inner]: the k largest, the larger first, equal ones by the lower
+ *     index (a NaN counts as the largest); values have the logits' type
+ *   rest [N][inner]: T * logsumexp(t_v / T) over the others (-inf: none) */
+int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, int64_t inner,
+                    int64_t stride, int k, float temperature, void* values, int64_t* indices,
+                    float* rest, void* stream);
+
+/* q = softmax([values, rest] / T), p = softmax(z / T) with the classes beyond the record's
+ * added up;  KL_r = sum_j q_j (log q_j - log p_j);  row loss = scale * T^2 * w_r * KL_r.
+ * rest == NULL: no mass beyond the record (q over its entries alone).  weight == NULL: 1; a
+ * row of weight 0 gives neither loss nor gradient, whatever it holds.  An entry whose index
+ * lies outside [0, V) is absent (its value is not used); so is one whose index occurred
+ * earlier in the row.  A record without any mass gives neither loss nor gradient.
+ * Class maps: V <= 1024. */
+typedef struct {
+    const void* logits;
+    int dtype;
+    int64_t N;
+    int V;
+    int64_t inner;
+    int64_t stride;
+    const void* values;     /* [N][k][inner], fp32 or bf16 */
+    int values_dtype;
+    const void* indices;    /* [N][k][inner] */
+    int index_bits;         /* 32 or 64 */
+    int k;
+    const float* rest;      /* [N][inner] or NULL */
+    const float* weight;    /* [N][inner] or NULL */
+    double temperature;
+    double scale;
+} ugpg_distill_t;
+size_t ugpg_distill_workspace(const ugpg_distill_t* p);
+/* loss[0] = the rows' sum, row_loss [N][inner] each row's (one at least given); dlogits
+ * (nullable): d loss / d logits, packed ([N][V], or the maps' layout), the logits' type --
+ * written with the sums of the same row, while the row is in the caches */
+int ugpg_distill_fwd(const ugpg_distill_t* p, float* loss, float* row_loss, void* dlogits,
+                     void* ws, size_t ws_bytes, void* stream);
+/* dlogits = gout * d loss / d logits; gout: one value, or one per row (per_row: of the row
+ * losses).  skip_one: dlogits holds ugpg_distill_fwd's gradient already, so nothing is done
+ * where gout is 1 (decided on the device: no synchronisation). */
+int ugpg_distill_bwd(const ugpg_distill_t* p, const float* gout, int per_row, int skip_one,
+                     void* dlogits, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- MoNuSeg augmentation (aug_monuseg_dataset.py:113-148,
  * monuseg_dataset.py:137-190): PIL's 8-bit arithmetic reproduced on the GPU. -------- */
 /* One separable pass of PIL's antialiasing resampler (Image.resize BILINEAR): `outer`

@@ -1,0 +1,1179 @@
+// A teacher's top logits, and the distillation loss that reads them.
+//
+// Record of a teacher's row t over V classes at temperature T: its k largest logits, sorted
+// by value then by the lower index, and `rest` = T * logsumexp(t_v / T over the others): the
+// logit of one class that carries all the others' mass.
+//
+// Loss of a student's row z against a record: both distributions live on k + 1 classes,
+//   q = softmax([t_1 .. t_k, rest] / T),   p = softmax(z / T) with the classes beyond the
+//   kept ones added up,   KL = sum_j q_j (log q_j - log p_j)
+//   loss = scale * T^2 * sum_r w_r KL_r
+//   dz_v = scale * T * w_r * (p_v - q_v)                          v kept
+//        = scale * T * w_r * (p_rest - q_rest) * r_v              else, r_v = p_v / p_rest
+// The kept classes are left out of the rest's sums (by a bitmap), never subtracted from a
+// total: both distributions may have almost all their mass in the kept classes.
+//
+// Bandwidth-bound: a row's logits are read for the sums and again for the gradient, which
+// finds them in the caches; sums over a row are fp32 (runs of 4 or 8 per thread, then trees),
+// the few terms of the k + 1 classes fp64.  No float atomics; orders are fixed.
+#include "common.h"
+#include "vecio.h"
+
+namespace ugpg {
+
+constexpr int DK_MAX = 256;              // entries of a record
+constexpr float NEG_INF = -__builtin_inff();
+constexpr double LOG2E = 1.4426950408889634074;
+
+__device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T> struct RowVec { static constexpr int N = 16 / (int)sizeof(T); };
+
+// The elements [lo, hi) of a row in vectors of N: slot 0 is the part before the first
+// 16-byte boundary, then whole vectors, then the tail.  f(slot, first index, pack, count);
+// a partial pack is filled up with -inf.
+template <typename T> struct RowSpan {
+    static constexpr int N = RowVec<T>::N;
+    const T* z;
+    int lo, hi, head, nv;
+    __device__ __forceinline__ RowSpan(const T* row, int l, int h) : z(row), lo(l), hi(h) {
+        const int mis = (int)(((uintptr_t)(row + l) & 15) / sizeof(T));
+        head = mis ? N - mis : 0;
+        if (head > hi - lo) head = hi - lo;
+        nv = (hi - lo - head) / N;
+    }
+    __device__ __forceinline__ int bits() const { return (nv + 2) * N; }
+    // position of element idx in the bitmap (N bits a slot)
+    __device__ __forceinline__ int bit(int idx) const {
+        const int o = idx - lo;
+        return o < head ? o : o - head + N;
+    }
+    __device__ __forceinline__ Pack<T, N> partial(int i0, int cnt) const {
+        Pack<T, N> v;
+#pragma unroll
+        for (int e = 0; e < N; ++e) v.set(e, e < cnt ? (float)z[i0 + e] : NEG_INF);
+        return v;
+    }
+    template <int U, typename F> __device__ __forceinline__ void scan(int tid, int nt, F f) const {
+        const T* b = z + lo + head;
+        int i = tid;
+        for (; i + (U - 1) * nt < nv; i += U * nt) {
+            Pack<T, N> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u].load(b + (size_t)(i + u * nt) * N);
+#pragma unroll
+            for (int u = 0; u < U; ++u) f(i + u * nt + 1, lo + head + (i + u * nt) * N, v[u], N);
+        }
+        for (; i < nv; i += nt) {
+            Pack<T, N> v;
+            v.load(b + (size_t)i * N);
+            f(i + 1, lo + head + i * N, v, N);
+        }
+        if (tid == 0 && head > 0) f(0, lo, partial(lo, head), head);
+        const int t0 = lo + head + nv * N;
+        if (tid == 64 % nt && t0 < hi) f(nv + 1, t0, partial(t0, hi - t0), hi - t0);
+    }
+};
+
+// running (max, sum of exp2((v - max) * c)); max -inf: nothing yet
+struct MaxSum {
+    float m, s;
+    __device__ __forceinline__ void merge(float m2, float s2, float c) {
+        const float mm = fmaxf(m, m2);
+        if (mm == NEG_INF) {
+            s += s2;  // (0, or a NaN that must stay)
+            return;
+        }
+        s = s * exp2_raw((m - mm) * c) + s2 * exp2_raw((m2 - mm) * c);
+        m = mm;
+    }
+    template <typename P> __device__ __forceinline__ void add(const P& v, int n, float c) {
+        // n values of a pack (compile-time n)
+        float mx = v.get(0);
+        for (int e = 1; e < n; ++e) mx = fmaxf(mx, v.get(e));
+        if (mx > m) {
+            s *= exp2_raw((m - mx) * c);
+            m = mx;
+        }
+        if (m == NEG_INF) {  // nothing, or values that are no numbers: the sum becomes one too
+            for (int e = 0; e < n; ++e) s += v.get(e) == NEG_INF ? 0.f : v.get(e);
+            return;
+        }
+        float t = 0.f;
+        for (int e = 0; e < n; ++e) t += exp2_raw((v.get(e) - m) * c);
+        s += t;
+    }
+    __device__ __forceinline__ void add1(float v, float c) {
+        if (v > m) {
+            s *= exp2_raw((m - v) * c);
+            m = v;
+        }
+        if (v != NEG_INF) s += exp2_raw((v - m) * c);  // (a NaN makes the sum one)
+    }
+    __device__ __forceinline__ void wave(float c) {
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
+            merge(m2, s2, c);
+        }
+    }
+};
+
+// block-wide merge; every thread returns the result (sm: 2 floats per wave)
+__device__ __forceinline__ MaxSum block_maxsum(MaxSum a, float c, float* sm) {
+    a.wave(c);
+    const int w = threadIdx.x / 64, nw = blockDim.x / 64;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) {
+        sm[2 * w] = a.m;
+        sm[2 * w + 1] = a.s;
+    }
+    __syncthreads();
+    MaxSum r{sm[0], sm[1]};
+    for (int i = 1; i < nw; ++i) r.merge(sm[2 * i], sm[2 * i + 1], c);
+    return r;
+}
+
+__device__ __forceinline__ double wave_max_d(double v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// ---------------------------------------------------------------- the loss: arguments
+struct DistillArgs {
+    const void* logits;
+    const void* values;
+    const void* indices;
+    const float* rest;
+    const float* weight;
+    int64_t rows, inner, stride;  // row r = (r / inner, r % inner)
+    int V, k, v16, i64;           // v16: values in bf16; i64: indices in 64 bits
+    double T, coef;               // coef = scale; loss coef*T*T*w*KL, gradient coef*T*w*(p - q)
+    float c;                      // log2(e) / T
+    const float* gout;            // upstream gradient: NULL (1), a scalar, or one per row
+    int gout_rows, skip_one;      // skip_one: nothing to do where the scalar is 1
+    double* row_loss;             // weighted loss per row (or per block, class maps), or NULL
+    float* row_out;               // reduction "none": the loss of each row, or NULL
+    void* dz;                     // gradient, packed rows [rows][V] / maps [N][V][inner], or NULL
+};
+
+__device__ __forceinline__ bool distill_skip(const DistillArgs& a) {
+    return a.skip_one && a.gout[0] == 1.f;
+}
+// entry j of record row (n, p): position in [N][k][inner]
+__device__ __forceinline__ int distill_index(const DistillArgs& a, size_t at) {
+    if (a.i64) {
+        const int64_t i = static_cast<const int64_t*>(a.indices)[at];
+        return i >= 0 && i < a.V ? (int)i : -1;
+    }
+    const int i = static_cast<const int*>(a.indices)[at];
+    return i >= 0 && i < a.V ? i : -1;
+}
+__device__ __forceinline__ float distill_value(const DistillArgs& a, size_t at) {
+    return a.v16 ? (float)static_cast<const __bf16*>(a.values)[at]
+                 : static_cast<const float*>(a.values)[at];
+}
+
+// what a row's k + 1 classes give (computed by one wave over entries in LDS)
+struct RowTerms {
+    double kl;        // NaN / inf as they come out
+    double M, rsq;    // teacher: max, 1 / sum
+    double m, rs;     // student: max, 1 / sum
+    double restdiff;  // (p_rest - q_rest) / s_rest (0 where the student's rest is empty)
+    bool empty;       // the record says nothing: no loss, no gradient
+};
+
+// one wave; idx < 0: absent.  (mr, sr): the student's rest, running max and sum
+__device__ __forceinline__ RowTerms row_terms(const int* idx, const float* t, const float* z, int k,
+                                              float rest, MaxSum r, double T) {
+    const int lane = threadIdx.x & 63;
+    const double iT = 1.0 / T;
+    RowTerms o;
+    double M = rest, m = r.m;
+    for (int j = lane; j < k; j += 64)
+        if (idx[j] >= 0) {
+            M = fmax(M, (double)t[j]);
+            m = fmax(m, (double)z[j]);
+        }
+    o.M = wave_max_d(M);
+    o.m = wave_max_d(m);
+    double sq = 0, ss = 0;
+    for (int j = lane; j < k; j += 64)
+        if (idx[j] >= 0) {
+            sq += exp(((double)t[j] - o.M) * iT);
+            ss += exp(((double)z[j] - o.m) * iT);
+        }
+    sq = wave_sum_d(sq);
+    ss = wave_sum_d(ss);
+    const double er = rest == NEG_INF ? 0.0 : exp(((double)rest - o.M) * iT);
+    const double logr = r.m == NEG_INF ? (double)NEG_INF : ((double)r.m - o.m) * iT + log((double)r.s);
+    sq += er;
+    ss += r.m == NEG_INF ? (double)r.s : exp(logr);  // (an empty rest's sum is 0, or a NaN)
+    o.rsq = 1.0 / sq;
+    o.rs = 1.0 / ss;
+    const double lq = log(sq), ls = log(ss);
+    double kl = 0;
+    for (int j = lane; j < k; j += 64)
+        if (idx[j] >= 0) {
+            const double a = ((double)t[j] - o.M) * iT;
+            const double q = exp(a) * o.rsq;
+            if (!(q == 0.0)) kl += q * ((a - lq) - (((double)z[j] - o.m) * iT - ls));
+        }
+    o.kl = wave_sum_d(kl);
+    const double qr = er * o.rsq;
+    if (!(qr == 0.0)) o.kl += qr * ((((double)rest - o.M) * iT - lq) - (logr - ls));
+    const double pr = r.m == NEG_INF ? 0.0 : exp(logr) * o.rs;
+    o.restdiff = r.m == NEG_INF ? 0.0 : (pr - qr) / (double)r.s;
+    o.empty = o.M == (double)NEG_INF;
+    return o;
+}
+__device__ __forceinline__ float entry_grad(const RowTerms& o, double g, float t, float z, double T) {
+    const double iT = 1.0 / T;
+    return (float)(g * (exp(((double)z - o.m) * iT) * o.rs - exp(((double)t - o.M) * iT) * o.rsq));
+}
+
+// ---------------------------------------------------------------- rows, a block each
+struct RowShared {
+    int idx[DK_MAX];
+    float t[DK_MAX], z[DK_MAX], ms[2 * 16];
+    int dup;
+    float a, mr;
+    double g;
+    RowTerms o;
+};
+
+// the record's entries into LDS, the student's logits at them, and the bitmap of the kept
+// classes within the span; an index given twice counts the first time only
+template <typename T>
+__device__ __forceinline__ void row_entries(const DistillArgs& a, int64_t r, const RowSpan<T>& sp,
+                                            RowShared& s, uint32_t* bits) {
+    const int tid = threadIdx.x, nt = blockDim.x;
+    for (int i = tid; i < (sp.bits() + 31) / 32; i += nt) bits[i] = 0;
+    if (tid == 0) s.dup = 0;
+    for (int j = tid; j < a.k; j += nt) {
+        const size_t at = (size_t)r * a.k + j;
+        const int i = distill_index(a, at);
+        s.idx[j] = i;
+        s.t[j] = distill_value(a, at);
+        s.z[j] = i >= 0 ? (float)sp.z[i] : NEG_INF;
+    }
+    __syncthreads();
+    for (int j = tid; j < a.k; j += nt) {
+        const int i = s.idx[j];
+        if (i >= sp.lo && i < sp.hi) {
+            const int b = sp.bit(i);
+            const uint32_t old = atomicOr(&bits[b >> 5], 1u << (b & 31));
+            if (old >> (b & 31) & 1) s.dup = 1;
+        } else if (i >= 0) {
+            for (int l = 0; l < j; ++l)  // outside the span: no bitmap to ask
+                if (s.idx[l] == i) s.dup = 1;
+        }
+    }
+    __syncthreads();
+    if (s.dup) {  // (no correct record has one)
+        unsigned drop = 0;
+        for (int q = 0, j = tid; j < a.k; j += nt, ++q)
+            for (int l = 0; l < j; ++l) drop |= (unsigned)(s.idx[l] == s.idx[j]) << q;
+        __syncthreads();
+        for (int q = 0, j = tid; j < a.k; j += nt, ++q)
+            if (drop >> q & 1) s.idx[j] = -1;
+        __syncthreads();
+    }
+}
+
+// sums over the span's classes outside the record
+template <typename T>
+__device__ __forceinline__ MaxSum row_rest(const DistillArgs& a, const RowSpan<T>& sp,
+                                           const uint32_t* bits) {
+    constexpr int N = RowVec<T>::N;
+    MaxSum acc{NEG_INF, 0.f};
+    const float c = a.c;
+    sp.template scan<4>(threadIdx.x, blockDim.x, [&](int slot, int i0, const Pack<T, N>& v, int cnt) {
+        const uint32_t w = (bits[slot * N >> 5] >> (slot * N & 31)) & ((1u << N) - 1);
+        if (__builtin_expect(w == 0, 1)) {
+            acc.add(v, N, c);
+        } else {
+            Pack<T, N> u = v;
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (w >> e & 1) u.set(e, NEG_INF);
+            acc.add(u, N, c);
+        }
+    });
+    return acc;
+}
+
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void row_grad(const DistillArgs& a, int64_t r, const RowSpan<T>& sp,
+                                         RowShared& s) {
+    constexpr int N = RowVec<T>::N;
+    T* d = static_cast<T*>(a.dz) + (size_t)r * a.V;
+    const float f = s.a, mr = s.mr, c = a.c;
+    if (f == 0.f || mr == NEG_INF) {  // (f NaN: written as such below)
+        sp.template scan<1>(threadIdx.x, blockDim.x, [&](int, int i0, const Pack<T, N>&, int cnt) {
+            for (int e = 0; e < cnt; ++e) d[i0 + e] = (T)0.f;
+        });
+    } else {
+        sp.template scan<4>(threadIdx.x, blockDim.x, [&](int, int i0, const Pack<T, N>& v, int cnt) {
+            Pack<T, N> o;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o.set(e, f * exp2_raw((v.get(e) - mr) * c));
+            if (ALIGNED && cnt == N) {
+                o.store(d + i0);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (e < cnt) d[i0 + e] = (T)o.get(e);
+            }
+        });
+    }
+    __syncthreads();  // the kept classes over what the scan wrote there
+    if (s.o.empty || s.g == 0.0) return;
+    for (int j = threadIdx.x; j < a.k; j += blockDim.x) {
+        const int i = s.idx[j];
+        if (i >= sp.lo && i < sp.hi) d[i] = (T)entry_grad(s.o, s.g, s.t[j], s.z[j], a.T);
+    }
+}
+
+// wave 0: the row's terms; every thread of the block calls it
+__device__ __forceinline__ void row_finish(const DistillArgs& a, int64_t r, MaxSum rest, bool first,
+                                           RowShared& s) {
+    const float w = a.weight ? a.weight[r] : 1.f;
+    if (threadIdx.x < 64) {
+        const float tr = a.rest ? a.rest[r] : NEG_INF;
+        const RowTerms o = row_terms(s.idx, s.t, s.z, a.k, tr, rest, a.T);
+        if (threadIdx.x == 0) {
+            const bool none = o.empty || w == 0.f;
+            const double l = none ? 0.0 : a.coef * a.T * a.T * (double)w * o.kl;
+            if (first && a.row_loss) a.row_loss[r] = l;
+            if (first && a.row_out) a.row_out[r] = (float)l;
+            const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
+            s.g = none ? 0.0 : a.coef * a.T * (double)w * go;
+            s.a = none ? 0.f : (float)(s.g * o.restdiff);
+            s.mr = rest.m;
+            s.o = o;
+            s.o.empty = none;
+        }
+    }
+    __syncthreads();
+}
+
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(512) distill_row_kernel(DistillArgs a) {
+    extern __shared__ uint32_t bits[];
+    __shared__ RowShared s;
+    if (distill_skip(a)) return;
+    const int64_t r = blockIdx.x;
+    const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, 0, a.V);
+    row_entries<T>(a, r, sp, s, bits);
+    const MaxSum rest = block_maxsum(row_rest<T>(a, sp, bits), a.c, s.ms);
+    row_finish(a, r, rest, true, s);
+    if (a.dz) row_grad<T, ALIGNED>(a, r, sp, s);
+}
+
+// few or very long rows: `split` blocks a row, sums first ...
+template <typename T>
+__global__ void __launch_bounds__(256) distill_part_kernel(DistillArgs a, int split, int chunk,
+                                                           float* part) {
+    extern __shared__ uint32_t bits[];
+    __shared__ RowShared s;
+    if (distill_skip(a)) return;
+    const int64_t r = blockIdx.x / split;
+    const int c = blockIdx.x % split, lo = c * chunk;
+    const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, lo < a.V ? lo : a.V,
+                        lo + chunk < a.V ? lo + chunk : a.V);
+    row_entries<T>(a, r, sp, s, bits);
+    const MaxSum rest = block_maxsum(row_rest<T>(a, sp, bits), a.c, s.ms);
+    if (threadIdx.x == 0) {
+        part[2 * blockIdx.x] = rest.m;
+        part[2 * blockIdx.x + 1] = rest.s;
+    }
+}
+// ... then the row's terms (every block of a row, the same way) and its share of the gradient
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) distill_join_kernel(DistillArgs a, int split, int chunk,
+                                                           int gsplit, int gchunk,
+                                                           const float* part) {
+    extern __shared__ uint32_t bits[];
+    __shared__ RowShared s;
+    if (distill_skip(a)) return;
+    const int64_t r = blockIdx.x / gsplit;
+    const int c = blockIdx.x % gsplit, lo = c * gchunk;
+    const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, lo < a.V ? lo : a.V,
+                        lo + gchunk < a.V ? lo + gchunk : a.V);
+    row_entries<T>(a, r, sp, s, bits);
+    MaxSum rest{NEG_INF, 0.f};
+    for (int i = threadIdx.x; i < split; i += blockDim.x)
+        rest.merge(part[2 * (r * split + i)], part[2 * (r * split + i) + 1], a.c);
+    rest = block_maxsum(rest, a.c, s.ms);
+    row_finish(a, r, rest, c == 0, s);
+    if (a.dz) row_grad<T, ALIGNED>(a, r, sp, s);
+}
+
+// ---------------------------------------------------------------- short rows, a wave each
+constexpr int DW_MAX = 512;  // classes
+struct WaveShared {
+    int idx[DK_MAX];
+    float t[DK_MAX], z[DK_MAX];
+    uint32_t bits[DW_MAX / 32];
+};
+
+// LDS written and read by one wave: its operations stay in order, the compiler must too
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// NV values a lane; returns the row's weighted loss (every lane)
+template <typename T, int NV>
+__device__ __forceinline__ double distill_wave_row(const DistillArgs& a, int64_t r, WaveShared& s) {
+    const int lane = threadIdx.x & 63;
+    const T* z = static_cast<const T*>(a.logits) + r * a.stride;
+    float v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) v[i] = lane + 64 * i < a.V ? (float)z[lane + 64 * i] : NEG_INF;
+    if (lane < DW_MAX / 32) s.bits[lane] = 0;
+    wave_sync();
+    bool dup = false;
+    for (int j = lane; j < a.k; j += 64) {
+        const size_t at = (size_t)r * a.k + j;
+        const int i = distill_index(a, at);
+        s.idx[j] = i;
+        s.t[j] = distill_value(a, at);
+        s.z[j] = i >= 0 ? (float)z[i] : NEG_INF;
+        if (i >= 0) dup |= atomicOr(&s.bits[i >> 5], 1u << (i & 31)) >> (i & 31) & 1;
+    }
+    wave_sync();
+    if (__any(dup)) {
+        unsigned drop = 0;
+        for (int q = 0, j = lane; j < a.k; j += 64, ++q)
+            for (int l = 0; l < j; ++l) drop |= (unsigned)(s.idx[l] == s.idx[j]) << q;
+        wave_sync();
+        for (int q = 0, j = lane; j < a.k; j += 64, ++q)
+            if (drop >> q & 1) s.idx[j] = -1;
+        wave_sync();
+    }
+    const float w = a.weight ? a.weight[r] : 1.f;
+    MaxSum rest{NEG_INF, 0.f};
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int x = lane + 64 * i;
+        if (x < a.V && !(s.bits[x >> 5] >> (x & 31) & 1)) rest.add1(v[i], a.c);
+    }
+    rest.wave(a.c);
+    const float tr = a.rest ? a.rest[r] : NEG_INF;
+    const RowTerms o = row_terms(s.idx, s.t, s.z, a.k, tr, rest, a.T);
+    const bool none = o.empty || w == 0.f;
+    const double l = none ? 0.0 : a.coef * a.T * a.T * (double)w * o.kl;
+    if (a.dz) {
+        T* d = static_cast<T*>(a.dz) + (size_t)r * a.V;
+        const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
+        const double g = none ? 0.0 : a.coef * a.T * (double)w * go;
+        const float f = none || rest.m == NEG_INF ? 0.f : (float)(g * o.restdiff);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int x = lane + 64 * i;
+            if (x < a.V && !(s.bits[x >> 5] >> (x & 31) & 1))
+                d[x] = (T)(f == 0.f ? 0.f : f * exp2_raw((v[i] - rest.m) * a.c));
+        }
+        for (int j = lane; j < a.k; j += 64)
+            if (s.idx[j] >= 0)
+                d[s.idx[j]] = (T)(none ? 0.f : entry_grad(o, g, s.t[j], s.z[j], a.T));
+    }
+    wave_sync();  // the next row reuses the LDS
+    return l;
+}
+
+// one block for everything: also sums the rows (loss out)
+template <typename T, int NV>
+__global__ void __launch_bounds__(1024) distill_wave_one_kernel(DistillArgs a, float* loss) {
+    __shared__ WaveShared s[16];
+    __shared__ double sum[16];
+    if (distill_skip(a)) return;
+    const int w = threadIdx.x / 64, nw = blockDim.x / 64;
+    double acc = 0;
+    for (int64_t r = w; r < a.rows; r += nw) {
+        const double l = distill_wave_row<T, NV>(a, r, s[w]);
+        if (a.row_out && (threadIdx.x & 63) == 0) a.row_out[r] = (float)l;
+        acc += l;
+    }
+    if ((threadIdx.x & 63) == 0) sum[w] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0 && loss) {
+        for (int i = 1; i < nw; ++i) acc += sum[i];
+        loss[0] = (float)acc;
+    }
+}
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) distill_wave_kernel(DistillArgs a) {
+    __shared__ WaveShared s[4];
+    if (distill_skip(a)) return;
+    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    if (r >= a.rows) return;
+    const double l = distill_wave_row<T, NV>(a, r, s[threadIdx.x / 64]);
+    if ((threadIdx.x & 63) == 0) {
+        if (a.row_loss) a.row_loss[r] = l;
+        if (a.row_out) a.row_out[r] = (float)l;
+    }
+}
+
+// ---------------------------------------------------------------- class maps, a thread each
+constexpr int DM_MAX = 1024;  // classes
+template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(DistillArgs a) {
+    extern __shared__ uint32_t bits[];  // [ceil(V / 32)][256]
+    __shared__ double red[4];
+    if (distill_skip(a)) return;
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    double l = 0;
+    if (r < a.rows) {
+        const int64_t n = r / a.inner, p = r % a.inner;
+        const T* z = static_cast<const T*>(a.logits) + (size_t)n * a.V * a.inner + p;
+        const size_t rec = (size_t)n * a.k * a.inner + p;
+        uint32_t* mine = bits + threadIdx.x;
+        const int nw = (a.V + 31) / 32;
+        for (int i = 0; i < nw; ++i) mine[256 * i] = 0;
+        const float w = a.weight ? a.weight[r] : 1.f;
+        const float rest = a.rest ? a.rest[r] : NEG_INF;
+        const float fT = (float)a.T;
+        const float iT = 1.f / fT;
+        // kept classes: marks (an index seen before is absent), maxima
+        float M = rest, m = NEG_INF;
+        for (int j = 0; j < a.k; ++j) {
+            const int i = distill_index(a, rec + (size_t)j * a.inner);
+            if (i < 0 || (mine[256 * (i >> 5)] >> (i & 31) & 1)) continue;
+            mine[256 * (i >> 5)] |= 1u << (i & 31);
+            M = fmaxf(M, distill_value(a, rec + (size_t)j * a.inner));
+            m = fmaxf(m, (float)z[(size_t)i * a.inner]);
+        }
+        MaxSum rs{NEG_INF, 0.f};
+        for (int i0 = 0; i0 < a.V; i0 += 32) {
+            const uint32_t b = mine[256 * (i0 >> 5)];
+            const int top = a.V - i0 < 32 ? a.V - i0 : 32;
+            for (int e = 0; e < top; ++e) {
+                const float v = (float)z[(size_t)(i0 + e) * a.inner];
+                if (!(b >> e & 1)) rs.add1(v, a.c);
+            }
+        }
+        m = fmaxf(m, rs.m);
+        // the k + 1 terms; the marks are cleared as entries are met, so a second pass over the
+        // entries again takes each index once
+        auto entries = [&](bool set, auto f) {
+            for (int j = 0; j < a.k; ++j) {
+                const size_t at = rec + (size_t)j * a.inner;
+                const int i = distill_index(a, at);
+                if (i < 0) continue;
+                const uint32_t b = 1u << (i & 31);
+                uint32_t& word = mine[256 * (i >> 5)];
+                if (((word & b) != 0) == set) continue;
+                word ^= b;
+                f(i, distill_value(a, at), (float)z[(size_t)i * a.inner]);
+            }
+        };
+        double sq = 0, ss = 0;
+        entries(false, [&](int, float t, float zi) {
+            sq += expf((t - M) * iT);
+            ss += expf((zi - m) * iT);
+        });
+        const float er = rest == NEG_INF ? 0.f : expf((rest - M) * iT);
+        const double iTd = 1.0 / a.T;
+        const bool has = rs.m != NEG_INF;
+        const double logr = has ? ((double)rs.m - (double)m) * iTd + log((double)rs.s) : (double)NEG_INF;
+        const float er_s = has ? rs.s * expf((rs.m - m) * iT) : rs.s;
+        sq += er;
+        ss += er_s;
+        const double lq = log(sq), ls = log(ss), rsq = 1.0 / sq, rss = 1.0 / ss;
+        const bool none = M == NEG_INF || w == 0.f;
+        const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
+        const double g = none ? 0.0 : a.coef * a.T * (double)w * go;
+        T* d = static_cast<T*>(a.dz) + (a.dz ? (size_t)n * a.V * a.inner + p : 0);
+        double kl = 0;
+        entries(true, [&](int i, float t, float zi) {
+            const double q = (double)expf((t - M) * iT) * rsq;
+            if (!(q == 0.0))
+                kl += q * ((((double)t - (double)M) * iTd - lq) - (((double)zi - (double)m) * iTd - ls));
+            if (a.dz) d[(size_t)i * a.inner] = (T)(none ? 0.f : (float)(g * ((double)expf((zi - m) * iT) * rss - q)));
+        });
+        const double qr = (double)er * rsq;
+        if (!(qr == 0.0)) kl += qr * ((((double)rest - (double)M) * iTd - lq) - (logr - ls));
+        l = none ? 0.0 : a.coef * a.T * a.T * (double)w * kl;
+        if (a.row_out) a.row_out[r] = (float)l;
+        if (a.dz) {
+            const float f = none || !has ? 0.f : (float)(g * (((double)er_s * rss - qr) / (double)rs.s));
+            for (int i0 = 0; i0 < a.V; i0 += 32) {
+                const uint32_t b = mine[256 * (i0 >> 5)];
+                const int top = a.V - i0 < 32 ? a.V - i0 : 32;
+                for (int e = 0; e < top; ++e) {
+                    const float v = (float)z[(size_t)(i0 + e) * a.inner];
+                    if (!(b >> e & 1))
+                        d[(size_t)(i0 + e) * a.inner] = (T)(f == 0.f ? 0.f : f * exp2_raw((v - rs.m) * a.c));
+                }
+            }
+        }
+    }
+    l = wave_sum_d(l);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = l;
+    __syncthreads();
+    if (threadIdx.x == 0 && a.row_loss) a.row_loss[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+__global__ void __launch_bounds__(1024) distill_sum_kernel(const double* part, int64_t n, float* loss) {
+    __shared__ double s[16];
+    double acc = 0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) acc += part[i];
+    acc = wave_sum_d(acc);
+    if ((threadIdx.x & 63) == 0) s[threadIdx.x / 64] = acc;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 1; i < 16; ++i) acc += s[i];
+        loss[0] = (float)acc;
+    }
+}
+
+// ---------------------------------------------------------------- a teacher's top logits
+// Order of a row: the larger value first, then the lower index; a NaN counts as the largest.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    const uint32_t b = __float_as_uint(v + 0.f);  // (-0 is 0)
+    return v != v ? 0xffffffffu : b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+// larger is earlier
+__device__ __forceinline__ uint64_t order_pair(uint32_t key, int idx) {
+    return (uint64_t)key << 32 | (uint32_t)~idx;
+}
+
+struct TopArgs {
+    const void* logits;
+    int64_t rows, inner, stride;
+    int V, k;
+    float T, c;  // temperature, log2(e) / T
+    void* values;
+    int64_t* indices;
+    float* rest;
+};
+
+__device__ __forceinline__ float rest_logit(MaxSum r, float T) {
+    // (+inf among the others: their sum of exp is not a number, their logit is +inf)
+    if (r.m == __builtin_inff()) return r.m;
+    return r.m == NEG_INF ? NEG_INF + r.s : (float)((double)r.m + (double)T * log((double)r.s));
+}
+
+constexpr int TK_CAP = 2048;   // candidates a block can hold
+constexpr int TK_RANK = 512;   // candidates up to here are ranked by counting
+struct TopShared {
+    uint64_t cand[TK_CAP];
+    float mx[512];
+    float ms[32];
+    uint32_t hist[256];
+    int n, eq[9];
+    uint32_t tau;
+};
+
+// Exact selection by key digits, for rows the threshold does not thin out (many equal values,
+// masked rows, NaN): the k-th key by four histograms, then the larger ones and the first of
+// the equal ones in index order.  Leaves the k candidates in s.cand; returns the rest's sums.
+template <typename T>
+__device__ MaxSum top_exact(const TopArgs& a, const RowSpan<T>& sp, TopShared& s) {
+    constexpr int N = RowVec<T>::N;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, w = tid / 64, nw = nt / 64;
+    uint32_t prefix = 0;
+    int need = a.k;  // entries still to take among the keys that match the prefix
+    for (int d = 24; d >= 0; d -= 8) {
+        for (int i = tid; i < 256; i += nt) s.hist[i] = 0;
+        __syncthreads();
+        const uint32_t high = d == 24 ? 0u : 0xffffffffu << (d + 8);
+        sp.template scan<1>(tid, nt, [&](int, int, const Pack<T, N>& v, int cnt) {
+            for (int e = 0; e < cnt; ++e) {
+                const uint32_t key = order_key(v.get(e));
+                const bool in = ((key ^ prefix) & high) == 0;
+                const uint32_t dig = key >> d & 255;
+                // equal digits across the wave (a row of one value): one addition
+                const uint32_t first = __builtin_amdgcn_readfirstlane(dig);
+                const uint64_t act = __ballot(1), same = __ballot(in && dig == first);
+                if (same == act) {
+                    if ((int)(__ffsll((unsigned long long)act) - 1) == lane) atomicAdd(&s.hist[first], (uint32_t)__popcll(act));
+                } else if (in) {
+                    atomicAdd(&s.hist[dig], 1u);
+                }
+            }
+        });
+        __syncthreads();
+        // digit of the k-th key: the largest b with (count of digits >= b) >= need
+        if (tid == 0) {
+            int left = need, b = 255;
+            for (; b > 0 && left > (int)s.hist[b]; --b) left -= s.hist[b];
+            s.eq[0] = left;
+            s.tau = prefix | (uint32_t)b << d;
+        }
+        __syncthreads();
+        need = s.eq[0];
+        prefix = s.tau;
+        __syncthreads();
+    }
+    // prefix: the k-th key; `need` of the values equal to it belong to the record
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    MaxSum acc{NEG_INF, 0.f};
+    int taken = 0;
+    const int lo = sp.lo, hi = sp.hi;
+    for (int base = lo; base < hi; base += nt) {
+        const int i = base + tid;
+        const uint32_t key = i < hi ? order_key((float)sp.z[i]) : 0u;
+        const bool eq = i < hi && key == prefix;
+        bool take = i < hi && key > prefix;
+        if (taken < need) {  // (uniform)
+            const uint64_t m = __ballot(eq);
+            if (lane == 0) s.eq[1 + w] = __popcll(m);
+            __syncthreads();
+            int before = taken, all = taken;
+            for (int q = 0; q < nw; ++q) {
+                if (q < w) before += s.eq[1 + q];
+                all += s.eq[1 + q];
+            }
+            const int pos = before + __popcll(m & ((1ull << lane) - 1));
+            take |= eq && pos < need;
+            taken = all;
+            __syncthreads();
+        }
+        if (take) {
+            const int at = atomicAdd(&s.n, 1);  // (the order of s.cand does not matter)
+            s.cand[at] = order_pair(key, i);
+        } else if (i < hi) {
+            acc.add1((float)sp.z[i], a.c);
+        }
+    }
+    __syncthreads();
+    return acc;
+}
+
+template <typename T> __global__ void __launch_bounds__(512) top_row_kernel(TopArgs a) {
+    constexpr int N = RowVec<T>::N;
+    __shared__ TopShared s;
+    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63;
+    const int64_t r = blockIdx.x;
+    const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, 0, a.V);
+    const float c = a.c;
+    // a lower bound of the k-th largest value: the k-th largest of the threads' maxima, to
+    // the upper 16 bits of its key; -inf where everything fits the buffer
+    float tau = NEG_INF;
+    if (a.V > TK_RANK) {
+        float mx = NEG_INF;
+        sp.template scan<4>(tid, nt, [&](int, int, const Pack<T, N>& v, int) {
+            float m = v.get(0);
+#pragma unroll
+            for (int e = 1; e < N; ++e) m = fmaxf(m, v.get(e));
+            mx = fmaxf(mx, m);
+        });
+        s.mx[tid] = mx;
+        __syncthreads();
+        if (tid < 64) {
+            uint32_t key[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int x = lane + 64 * i;
+                key[i] = x < nt ? order_key(s.mx[x]) >> 16 : 0u;
+            }
+            uint32_t t = 0;
+            for (int b = 15; b >= 0; --b) {
+                const uint32_t up = t | 1u << b;
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) n += __popcll(__ballot(key[i] >= up));
+                if (n >= a.k) t = up;
+            }
+            if (lane == 0) s.tau = t << 16;
+        }
+        __syncthreads();
+        const uint32_t t = s.tau;
+        // (keys below that of -inf belong to no value; a NaN's cannot be a bound)
+        tau = t <= 0x007fffffu ? NEG_INF : t >= 0xff800000u ? __builtin_inff() : key_value(t);
+    }
+    if (tid == 0) s.n = 0;
+    __syncthreads();
+    MaxSum acc{NEG_INF, 0.f};
+    sp.template scan<4>(tid, nt, [&](int, int i0, const Pack<T, N>& v, int cnt) {
+        float m = v.get(0);
+#pragma unroll
+        for (int e = 1; e < N; ++e) m = fmaxf(m, v.get(e));
+        if (m < tau) {
+            if (m > acc.m) {
+                acc.s *= exp2_raw((acc.m - m) * c);
+                acc.m = m;
+            }
+            float t = 0.f;
+            if (acc.m != NEG_INF)
+                for (int e = 0; e < N; ++e) t += exp2_raw((v.get(e) - acc.m) * c);
+            else
+                for (int e = 0; e < N; ++e) t += v.get(e) == NEG_INF ? 0.f : v.get(e);
+            acc.s += t;
+        } else {
+            for (int e = 0; e < cnt; ++e) {
+                const float x = v.get(e);
+                if (x < tau) {
+                    acc.add1(x, c);
+                } else {
+                    const int at = atomicAdd(&s.n, 1);
+                    if (at < TK_CAP) s.cand[at] = order_pair(order_key(x), i0 + e);
+                }
+            }
+        }
+    });
+    __syncthreads();
+    int n = s.n;
+    MaxSum rest = block_maxsum(acc, c, s.ms);
+    if (n > TK_CAP || rest.s != rest.s) {
+        __syncthreads();
+        rest = block_maxsum(top_exact<T>(a, sp, s), c, s.ms);
+        n = a.k;
+    }
+    // rank the candidates; the first k are the record, the others join the rest
+    if (n > TK_RANK) {
+        int m = 1024;
+        while (m < n) m <<= 1;
+        for (int i = n + tid; i < m; i += nt) s.cand[i] = 0;
+        for (int len = 2; len <= m; len <<= 1)
+            for (int st = len >> 1; st > 0; st >>= 1) {
+                __syncthreads();
+                for (int i = tid; i < m / 2; i += nt) {
+                    const int x = (i / st) * 2 * st + i % st, y = x + st;
+                    const uint64_t p = s.cand[x], q = s.cand[y];
+                    if ((p < q) == ((x & len) == 0)) {
+                        s.cand[x] = q;
+                        s.cand[y] = p;
+                    }
+                }
+            }
+        __syncthreads();
+    }
+    const int per = n > TK_RANK ? 1 : (n + nt - 1) / nt;
+    uint64_t mine[4];
+    int rank[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const int i = tid + q * nt;
+        rank[q] = -1;
+        if (n <= TK_RANK && q < per && i < n) {
+            mine[q] = s.cand[i];
+            int b = 0;
+            for (int j = 0; j < n; ++j) b += s.cand[j] > mine[q];
+            rank[q] = b;
+        }
+    }
+    __syncthreads();
+    if (n <= TK_RANK) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (rank[q] >= 0) s.cand[rank[q]] = mine[q];
+        __syncthreads();
+    }
+    T* val = static_cast<T*>(a.values) + (size_t)r * a.k;
+    int64_t* idx = a.indices + (size_t)r * a.k;
+    for (int i = tid; i < a.k; i += nt) {
+        val[i] = (T)key_value((uint32_t)(s.cand[i] >> 32));
+        idx[i] = (int64_t)(uint32_t)~(uint32_t)s.cand[i];
+    }
+    MaxSum more{NEG_INF, 0.f};
+    for (int i = a.k + tid; i < n; i += nt) more.add1(key_value((uint32_t)(s.cand[i] >> 32)), c);
+    more = block_maxsum(more, c, s.ms);
+    rest.merge(more.m, more.s, c);
+    if (tid == 0) a.rest[r] = rest_logit(rest, a.T);
+}
+
+// at most 64 classes: a wave a row, a class a lane, ranked by counting
+template <typename T> __global__ void __launch_bounds__(256) top_wave_kernel(TopArgs a) {
+    const int lane = threadIdx.x & 63;
+    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    if (r >= a.rows) return;
+    const float v = lane < a.V ? (float)static_cast<const T*>(a.logits)[r * a.stride + lane] : NEG_INF;
+    const uint32_t key = lane < a.V ? order_key(v) : 0u;
+    int rank = 0;
+    for (int j = 0; j < a.V; ++j) {
+        const uint32_t kj = __builtin_amdgcn_readlane(key, j);
+        rank += kj > key || (kj == key && j < lane);
+    }
+    const bool kept = lane < a.V && rank < a.k;
+    MaxSum rest{NEG_INF, 0.f};
+    if (!kept && lane < a.V) rest.add1(v, a.c);
+    rest.wave(a.c);
+    if (kept) {
+        static_cast<T*>(a.values)[(size_t)r * a.k + rank] = (T)key_value(key);
+        a.indices[(size_t)r * a.k + rank] = lane;
+    }
+    if (lane == 0) a.rest[r] = rest_logit(rest, a.T);
+}
+
+// class maps: a thread a pixel, k rounds of "the next in order"; VR > 0: the pixel's classes
+// stay in registers
+template <typename T, int VR> __global__ void __launch_bounds__(256) top_map_kernel(TopArgs a) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= a.rows) return;
+    const int64_t n = r / a.inner, p = r % a.inner;
+    const T* z = static_cast<const T*>(a.logits) + (size_t)n * a.V * a.inner + p;
+    T* val = static_cast<T*>(a.values) + (size_t)n * a.k * a.inner + p;
+    int64_t* idx = a.indices + (size_t)n * a.k * a.inner + p;
+    uint32_t key[VR > 0 ? VR : 1];
+    if constexpr (VR > 0) {
+#pragma unroll
+        for (int i = 0; i < VR; ++i) key[i] = i < a.V ? order_key((float)z[(size_t)i * a.inner]) : 0u;
+    }
+    uint64_t last = ~0ull;
+    MaxSum rest{NEG_INF, 0.f};
+    for (int j = 0; j <= a.k; ++j) {
+        uint64_t best = 0;
+        auto see = [&](uint32_t kv, int i) {
+            const uint64_t o = order_pair(kv, i);
+            if (j == 0 || o < last) {
+                if (j < a.k) best = o > best ? o : best;
+                else rest.add1(key_value(kv), a.c);
+            }
+        };
+        if constexpr (VR > 0) {
+#pragma unroll
+            for (int i = 0; i < VR; ++i)
+                if (i < a.V) see(key[i], i);
+        } else {
+            for (int i = 0; i < a.V; ++i) see(order_key((float)z[(size_t)i * a.inner]), i);
+        }
+        if (j < a.k) {
+            last = best;
+            val[(size_t)j * a.inner] = (T)key_value((uint32_t)(best >> 32));
+            idx[(size_t)j * a.inner] = (int64_t)(uint32_t)~(uint32_t)best;
+        }
+    }
+    a.rest[r] = rest_logit(rest, a.T);
+}
+
+// ---------------------------------------------------------------- host side
+// shared by both operators: N rows of V (inner == 1, row stride >= V) or N maps of V x inner
+static int rows_check(const char* what, const void* logits, int dtype, int64_t N, int V, int64_t inner,
+                      int64_t stride, int k, double T) {
+    if (!logits || (dtype != UGPG_DT_F32 && dtype != UGPG_DT_BF16) || N <= 0 || V <= 0 || inner <= 0 ||
+        k < 1 || k > V || !(T > 0.0) || !(T < 1e30)) {
+        set_error("%s: bad arguments (dtype=%d N=%lld V=%d inner=%lld k=%d T=%g)", what, dtype,
+                  (long long)N, V, (long long)inner, k, T);
+        return UGPG_ERR_INVALID;
+    }
+    if (k > DK_MAX) {
+        set_error("%s: k=%d entries, at most %d", what, k, DK_MAX);
+        return UGPG_ERR_INVALID;
+    }
+    if (inner == 1 ? stride < V && N > 1 : stride != (int64_t)V * inner) {
+        set_error("%s: row stride %lld does not fit V=%d inner=%lld", what, (long long)stride, V,
+                  (long long)inner);
+        return UGPG_ERR_INVALID;
+    }
+    // (grids of at most 2^32 threads; V leaves room for a span's padding in 32 bits)
+    if (V > (1 << 30) || (inner == 1 ? N > (1 << 22) : N > (int64_t)0x7fffffff / inner)) {
+        set_error("%s: N=%lld V=%d inner=%lld is too large", what, (long long)N, V, (long long)inner);
+        return UGPG_ERR_INVALID;
+    }
+    if ((uintptr_t)logits % (dtype == UGPG_DT_F32 ? 4 : 2)) {
+        set_error("%s: logits are not aligned to their type", what);
+        return UGPG_ERR_INVALID;
+    }
+    return UGPG_OK;
+}
+
+// A row's blocks: one where the rows alone fill the card (256 CUs) and its bitmap fits
+// (2^18 classes, 32 KB), else enough that about 512 run, of at least 4096 classes each.
+struct Split {
+    int n, chunk;
+};
+static Split row_split(int64_t rows, int V) {
+    int64_t n = rows >= 256 ? 1 : cdiv(512, rows);
+    const int64_t most = V / 4096 > 1 ? V / 4096 : 1, least = cdiv(V, 1 << 18);
+    if (n > most) n = most;
+    if (n < least) n = least;
+    Split s;
+    s.chunk = (int)(cdiv(cdiv(V, n), 64) * 64);
+    s.n = (int)cdiv(V, s.chunk);
+    return s;
+}
+
+}  // namespace ugpg
+
+using namespace ugpg;
+
+extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, int64_t inner,
+                               int64_t stride, int k, float temperature, void* values,
+                               int64_t* indices, float* rest, void* stream) {
+    if (int rc = rows_check("top_logits", logits, dtype, N, V, inner, stride, k, temperature)) return rc;
+    if (!values || !indices || !rest) {
+        set_error("top_logits: values, indices and rest must be given");
+        return UGPG_ERR_INVALID;
+    }
+    TopArgs a{logits, N * inner, inner, stride, V, k, temperature, (float)(LOG2E / temperature), values, indices, rest};
+    hipStream_t s = as_stream(stream);
+    const bool f32 = dtype == UGPG_DT_F32;
+#define TOP_GO(KF, KH, grid, nt)                                              \
+    do {                                                                      \
+        if (f32) hipLaunchKernelGGL(KF, dim3((unsigned)(grid)), dim3(nt), 0, s, a); \
+        else hipLaunchKernelGGL(KH, dim3((unsigned)(grid)), dim3(nt), 0, s, a);     \
+    } while (0)
+    if (inner > 1) {
+        const int64_t g = cdiv(a.rows, 256);
+        if (V <= 8) TOP_GO((top_map_kernel<float, 8>), (top_map_kernel<__bf16, 8>), g, 256);
+        else if (V <= 16) TOP_GO((top_map_kernel<float, 16>), (top_map_kernel<__bf16, 16>), g, 256);
+        else if (V <= 32) TOP_GO((top_map_kernel<float, 32>), (top_map_kernel<__bf16, 32>), g, 256);
+        else TOP_GO((top_map_kernel<float, 0>), (top_map_kernel<__bf16, 0>), g, 256);
+    } else if (V <= 64) {
+        TOP_GO((top_wave_kernel<float>), (top_wave_kernel<__bf16>), cdiv(N, 4), 256);
+    } else {
+        // twice as many maxima as entries keep the candidates near k
+        const int nt = k <= 64 && V <= 4096 ? 128 : k <= 128 && V <= 16384 ? 256 : 512;
+        TOP_GO((top_row_kernel<float>), (top_row_kernel<__bf16>), N, nt);
+    }
+#undef TOP_GO
+    return check_launch("top_logits");
+}
+
+static int distill_check(const char* what, const ugpg_distill_t* p) {
+    if (!p) {
+        set_error("%s: no descriptor", what);
+        return UGPG_ERR_INVALID;
+    }
+    if (int rc = rows_check(what, p->logits, p->dtype, p->N, p->V, p->inner, p->stride, p->k, p->temperature))
+        return rc;
+    if (!p->values || !p->indices || (p->values_dtype != UGPG_DT_F32 && p->values_dtype != UGPG_DT_BF16) ||
+        (p->index_bits != 32 && p->index_bits != 64) || !(p->scale == p->scale)) {
+        set_error("%s: bad record (values type %d, %d-bit indices) or scale %g", what, p->values_dtype,
+                  p->index_bits, p->scale);
+        return UGPG_ERR_INVALID;
+    }
+    if (p->inner > 1 && p->V > DM_MAX) {
+        set_error("%s: class maps of %d classes, at most %d", what, p->V, DM_MAX);
+        return UGPG_ERR_INVALID;
+    }
+    return UGPG_OK;
+}
+
+extern "C" size_t ugpg_distill_workspace(const ugpg_distill_t* p) {
+    if (distill_check("distill_workspace", p)) return 0;
+    if (p->inner > 1) return (size_t)cdiv(p->N * p->inner, 256) * 8;
+    size_t n = (size_t)p->N * 8;
+    if (p->V > DW_MAX) {
+        const Split sp = row_split(p->N, p->V);
+        if (sp.n > 1) n += (size_t)p->N * sp.n * 8;
+    }
+    return n;
+}
+
+template <typename T>
+static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, void* ws, hipStream_t s) {
+    const int es = sizeof(T);
+    const int64_t rows = a.rows;
+    int64_t nsum = rows;
+    a.row_loss = loss ? static_cast<double*>(ws) : nullptr;
+    if (p->inner > 1) {
+        nsum = cdiv(rows, 256);
+        hipLaunchKernelGGL((distill_map_kernel<T>), dim3((unsigned)nsum), dim3(256),
+                           (unsigned)(cdiv(a.V, 32) * 1024), s, a);
+    } else if (a.V <= DW_MAX) {
+        // up to 64 rows: one block of 16 waves, which also sums them
+        const bool one = rows <= 64;
+        const int nv = (int)cdiv(a.V, 64);
+#define DISTILL_WAVE(NV)                                                                          \
+    do {                                                                                          \
+        if (one)                                                                                  \
+            hipLaunchKernelGGL((distill_wave_one_kernel<T, NV>), dim3(1), dim3(1024), 0, s, a, loss); \
+        else                                                                                      \
+            hipLaunchKernelGGL((distill_wave_kernel<T, NV>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a); \
+    } while (0)
+        if (nv <= 1) DISTILL_WAVE(1);
+        else if (nv <= 4) DISTILL_WAVE(4);
+        else DISTILL_WAVE(8);
+#undef DISTILL_WAVE
+        if (one) return check_launch("distill");
+    } else {
+        // 16-byte stores where the gradient's rows lie as the logits' do
+        const bool al = !a.dz || (((uintptr_t)a.dz ^ (uintptr_t)a.logits) % 16 == 0 &&
+                                  (a.stride - a.V) * es % 16 == 0);
+        const Split sp = row_split(rows, a.V);
+        auto lds = [&](int span) { return (unsigned)(((span + 3 * RowVec<T>::N + 31) / 32) * 4); };
+        if (sp.n == 1) {
+            const int nt = a.V <= 8192 ? 256 : 512;
+            if (al)
+                hipLaunchKernelGGL((distill_row_kernel<T, true>), dim3((unsigned)rows), dim3(nt), lds(a.V), s, a);
+            else
+                hipLaunchKernelGGL((distill_row_kernel<T, false>), dim3((unsigned)rows), dim3(nt), lds(a.V), s, a);
+        } else {
+            float* part = reinterpret_cast<float*>(static_cast<double*>(ws) + rows);
+            const unsigned g = (unsigned)(rows * sp.n);
+            hipLaunchKernelGGL((distill_part_kernel<T>), dim3(g), dim3(256), lds(sp.chunk), s, a, sp.n, sp.chunk, part);
+            // without a gradient one block a row joins them, over no classes of its own
+            const int gn = a.dz ? sp.n : 1, gc = a.dz ? sp.chunk : 0;
+            const unsigned gg = (unsigned)(rows * gn);
+            if (al)
+                hipLaunchKernelGGL((distill_join_kernel<T, true>), dim3(gg), dim3(256), lds(gc), s, a, sp.n, sp.chunk, gn, gc, part);
+            else
+                hipLaunchKernelGGL((distill_join_kernel<T, false>), dim3(gg), dim3(256), lds(gc), s, a, sp.n, sp.chunk, gn, gc, part);
+        }
+    }
+    if (loss)
+        hipLaunchKernelGGL(distill_sum_kernel, dim3(1), dim3(1024), 0, s, a.row_loss, nsum, loss);
+    return check_launch("distill");
+}
+
+static DistillArgs distill_args(const ugpg_distill_t* p) {
+    DistillArgs a{};
+    a.logits = p->logits;
+    a.values = p->values;
+    a.indices = p->indices;
+    a.rest = p->rest;
+    a.weight = p->weight;
+    a.rows = p->N * p->inner;
+    a.inner = p->inner;
+    a.stride = p->stride;
+    a.V = p->V;
+    a.k = p->k;
+    a.v16 = p->values_dtype == UGPG_DT_BF16;
+    a.i64 = p->index_bits == 64;
+    a.T = p->temperature;
+    a.coef = p->scale;
+    a.c = (float)(LOG2E / p->temperature);
+    return a;
+}
+
+static int distill_ws_check(const char* what, const ugpg_distill_t* p, const void* ws, size_t n) {
+    const size_t need = ugpg_distill_workspace(p);
+    if (!ws || n < need) {
+        set_error("%s: workspace %zu < %zu", what, n, need);
+        return UGPG_ERR_WORKSPACE;
+    }
+    return UGPG_OK;
+}
+
+extern "C" int ugpg_distill_fwd(const ugpg_distill_t* p, float* loss, float* row_loss, void* dlogits,
+                                void* ws, size_t ws_bytes, void* stream) {
+    if (int rc = distill_check("distill_fwd", p)) return rc;
+    if (!loss && !row_loss) {
+        set_error("distill_fwd: neither loss nor row_loss given");
+        return UGPG_ERR_INVALID;
+    }
+    if (int rc = distill_ws_check("distill_fwd", p, ws, ws_bytes)) return rc;
+    DistillArgs a = distill_args(p);
+    a.row_out = row_loss;
+    a.dz = dlogits;
+    return p->dtype == UGPG_DT_F32 ? distill_run<float>(p, a, loss, ws, as_stream(stream))
+                                   : distill_run<__bf16>(p, a, loss, ws, as_stream(stream));
+}
+
+extern "C" int ugpg_distill_bwd(const ugpg_distill_t* p, const float* gout, int per_row, int skip_one,
+                                void* dlogits, void* ws, size_t ws_bytes, void* stream) {
+    if (int rc = distill_check("distill_bwd", p)) return rc;
+    if (!gout || !dlogits || (per_row && skip_one)) {
+        set_error("distill_bwd: bad arguments (per_row=%d skip_one=%d)", per_row, skip_one);
+        return UGPG_ERR_INVALID;
+    }
+    if (int rc = distill_ws_check("distill_bwd", p, ws, ws_bytes)) return rc;
+    DistillArgs a = distill_args(p);
+    a.gout = gout;
+    a.gout_rows = per_row != 0;
+    a.skip_one = skip_one != 0;
+    a.dz = dlogits;
+    return p->dtype == UGPG_DT_F32 ? distill_run<float>(p, a, nullptr, ws, as_stream(stream))
+                                   : distill_run<__bf16>(p, a, nullptr, ws, as_stream(stream));
+}

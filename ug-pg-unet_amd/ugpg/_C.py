@@ -61,6 +61,14 @@ class WgradDesc(C.Structure):
                 ("dy_bn", C.POINTER(BnLazy))]
 
 
+class DistillDesc(C.Structure):
+    """ugpg_distill_t."""
+    _fields_ = [("logits", _p), ("dtype", _i), ("N", _i64), ("V", _i), ("inner", _i64),
+                ("stride", _i64), ("values", _p), ("values_dtype", _i), ("indices", _p),
+                ("index_bits", _i), ("k", _i), ("rest", _p), ("weight", _p),
+                ("temperature", C.c_double), ("scale", C.c_double)]
+
+
 # name -> (restype, argtypes); must match include/ugpg.h exactly
 SIGNATURES = {
     "ugpg_version": (C.c_char_p, []),
@@ -145,6 +153,10 @@ SIGNATURES = {
     "ugpg_group_norm_fwd": (_i, [_p, _i, _i, _i64, _i, _i, _p, _p, _f, _i, _p, _p, _p, _p, _sz, _p]),
     "ugpg_group_norm_bwd": (_i, [_p, _i, _p, _i, _i, _i64, _i, _i, _p, _p, _p, _p, _i, _p, _i, _p,
                                  _p, _p, _p, _sz, _p]),
+    "ugpg_top_logits": (_i, [_p, _i, _i64, _i, _i64, _i64, _i, _f, _p, _p, _p, _p]),
+    "ugpg_distill_workspace": (_sz, [C.POINTER(DistillDesc)]),
+    "ugpg_distill_fwd": (_i, [C.POINTER(DistillDesc), _p, _p, _p, _p, _sz, _p]),
+    "ugpg_distill_bwd": (_i, [C.POINTER(DistillDesc), _p, _i, _i, _p, _p, _sz, _p]),
     "ugpg_resample_aa_u8": (_i, [_p, _i64, _i, _i, _i, _p, _p, _i, _p, _p]),
     "ugpg_resize_nearest_u8": (_i, [_p, _i64, _i, _i, _i, _p, _p, _p, _i, _i, _p]),
     "ugpg_augment_param_sizes": (_i, [C.POINTER(_i), C.POINTER(_i)]),

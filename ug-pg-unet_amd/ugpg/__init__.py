@@ -13,6 +13,8 @@ from .unet_parts import DoubleConv, Down, InConv, OutConv, Up  # noqa: F401
 from .unet import (PGUNet1, PGUNet2, PGUNet3, PGUNet4, ProgressiveUNet,  # noqa: F401
                    STAGE_RESOLUTIONS, transfer_state)
 from .loss import UncertaintyGuidedLoss  # noqa: F401
+from .distill import (DistillationLoss, TopLogits, distillation_loss,  # noqa: F401
+                      teacher_top_logits)
 from .norm import GroupNormAct, group_norm_act  # noqa: F401
 from .optim import RMSprop  # noqa: F401
 from .trainer import UncertaintyGuidedProgressiveTrainer  # noqa: F401

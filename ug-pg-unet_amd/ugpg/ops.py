@@ -12,7 +12,8 @@ import os
 
 import torch
 
-from ._C import Bnb, BnLazy, BwdRoute, ConvDesc, PackItem, Src, WgradDesc, check, lib
+from ._C import (Bnb, BnLazy, BwdRoute, ConvDesc, DistillDesc, PackItem, Src, WgradDesc, check,
+                 lib)
 
 F32 = torch.float32
 
@@ -850,6 +851,76 @@ def ce_ug_bwd(x, y, wts, class_weights, gout):
     check(lib.ugpg_ce_ug_bwd(ptr(x), ptr(y), ptr(wts), ptr(class_weights), B, K, ptr(gout),
                              ptr(dx), stream()), "ce_ug_bwd")
     return dx
+
+
+# ------------------------------------------------------------------ distillation
+TOP_MAX = 256        # entries of a teacher's record
+MAP_CLASSES = 1024   # classes of the maps distillation reads
+
+
+def _class_layout(logits):
+    """(logits, N, V, inner, row stride) of (N, V) rows -- any row stride, unit column stride
+    -- or (N, V, *spatial) class maps; other strides are copied."""
+    N, V = logits.shape[:2]
+    inner = logits.numel() // (N * V)
+    if inner > 1:
+        return logits.contiguous(), N, V, inner, V * inner
+    rows = logits.reshape(N, V)
+    if (V > 1 and rows.stride(1) != 1) or (N > 1 and rows.stride(0) < V):
+        rows = rows.contiguous()
+    return rows, N, V, 1, max(rows.stride(0), V)
+
+
+def _dev_ptr(t):
+    if not t.is_cuda:
+        raise RuntimeError("ugpg: tensor is not on a ROCm/HIP device (no CPU fallback)")
+    return t.data_ptr()
+
+
+def top_logits(logits, k, temperature):
+    """-> (values, indices, rest) of ugpg_top_logits, shaped (N, k, *spatial) and (N, *spatial)."""
+    x, N, V, inner, stride = _class_layout(logits)
+    sp = logits.shape[2:]
+    values = torch.empty(N, k, *sp, dtype=x.dtype, device=x.device)
+    indices = torch.empty(N, k, *sp, dtype=torch.int64, device=x.device)
+    rest = torch.empty(N, *sp, dtype=F32, device=x.device)
+    check(lib.ugpg_top_logits(_dev_ptr(x), _dtype_code(x), N, V, inner, stride, int(k),
+                              float(temperature), ptr(values), ptr(indices), ptr(rest), stream()),
+          "top_logits")
+    return values, indices, rest
+
+
+def _distill_desc(logits, values, indices, rest, weight, temperature, scale):
+    x, N, V, inner, stride = _class_layout(logits)
+    d = DistillDesc(_dev_ptr(x), _dtype_code(x), N, V, inner, stride, ptr(values), _dtype_code(values),
+                    ptr(indices), 32 if indices.dtype == torch.int32 else 64, values.shape[1], ptr(rest),
+                    ptr(weight), float(temperature), float(scale))
+    nbytes = lib.ugpg_distill_workspace(C.byref(d))
+    if nbytes == 0:
+        check(-1, "distill_workspace")
+    return d, x, workspace(nbytes, x.device)
+
+
+def distill_fwd(logits, values, indices, rest, weight, temperature, scale, per_row=False, grad=False):
+    """-> (loss, dlogits or None): loss a scalar, or (per_row) one value a row."""
+    d, x, ws = _distill_desc(logits, values, indices, rest, weight, temperature, scale)
+    loss = torch.empty((logits.shape[0], *logits.shape[2:]) if per_row else (), dtype=F32, device=x.device)
+    dz = torch.empty(logits.shape, dtype=x.dtype, device=x.device) if grad else None
+    check(lib.ugpg_distill_fwd(C.byref(d), None if per_row else ptr(loss), ptr(loss) if per_row else None,
+                               ptr(dz), ptr(ws), ws.numel(), stream()), "distill_fwd")
+    return loss, dz
+
+
+def distill_bwd(logits, values, indices, rest, weight, temperature, scale, gout, dz=None):
+    """dlogits for the upstream gradient gout (a scalar, or one value a row).  dz: the
+    gradient distill_fwd wrote, kept where gout is 1 and written anew where it is not."""
+    d, x, ws = _distill_desc(logits, values, indices, rest, weight, temperature, scale)
+    skip = dz is not None
+    if dz is None:
+        dz = torch.empty(logits.shape, dtype=x.dtype, device=x.device)
+    check(lib.ugpg_distill_bwd(C.byref(d), _f32(gout), int(gout.dim() > 0), int(skip), ptr(dz), ptr(ws),
+                               ws.numel(), stream()), "distill_bwd")
+    return dz
 
 
 def adam_step(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0):
