@@ -526,21 +526,31 @@ int ugpg_mul(const float* x, const float* m, float* y, int64_t n, void* stream);
 #define UGPG_ACT_NONE 0
 #define UGPG_ACT_RELU 1
 #define UGPG_ACT_SILU 2
-size_t ugpg_group_norm_workspace(int B, int64_t HW, int C, int G, int backward);
-int ugpg_group_norm_fwd(const void* x, int dtype, int B, int64_t HW, int C, int G,
-                        const float* gamma, const float* beta, float eps, int act, void* y,
-                        float* mean, float* rstd, void* ws, size_t ws_bytes, void* stream);
+typedef struct {
+    const void* x;
+    int dtype;
+    int B;
+    int64_t HW;
+    int C, G;
+    const float* gamma;     /* or NULL */
+    const float* beta;      /* or NULL */
+    float eps;
+    int act;
+    float* mean;            /* [B][G]: written by the forward, read by the backward */
+    float* rstd;
+} ugpg_group_norm_t;
+/* bytes of workspace (from the sizes alone) */
+size_t ugpg_group_norm_workspace(const ugpg_group_norm_t* p, int backward);
+int ugpg_group_norm_fwd(const ugpg_group_norm_t* p, void* y, void* ws, size_t ws_bytes, void* stream);
 /* With dp = dy * act'(xh*gamma + beta):
  *   dx = rstd * (gamma*dp - mean_g(gamma*dp) - xh*mean_g(gamma*dp*xh))
  *   dgamma = sum dp*xh;  dbeta = sum dp;  dxsum = sum over pixels and samples of dx (the
  *   gradient of a bias added to x: the convolution's in front); each [C] or NULL.
  * (x, dy, dx) types: all fp32, all bf16, bf16 with fp32 dy and dx, or bf16 with fp32 dy.
  * dx may alias dy where the types agree. */
-int ugpg_group_norm_bwd(const void* dy, int dy_dtype, const void* x, int dtype, int B,
-                        int64_t HW, int C, int G, const float* mean, const float* rstd,
-                        const float* gamma, const float* beta, int act, void* dx, int dx_dtype,
-                        float* dgamma, float* dbeta, float* dxsum, void* ws, size_t ws_bytes,
-                        void* stream);
+int ugpg_group_norm_bwd(const ugpg_group_norm_t* p, const void* dy, int dy_dtype, void* dx,
+                        int dx_dtype, float* dgamma, float* dbeta, float* dxsum, void* ws,
+                        size_t ws_bytes, void* stream);
 
 /* ---- A teacher's top logits, and distillation from them ----------------------
  * The previous stage as a teacher (the reference only weights by its uncertainty): a record
@@ -579,7 +589,8 @@ typedef struct {
     double temperature;
     double scale;
 } ugpg_distill_t;
-size_t ugpg_distill_workspace(const ugpg_distill_t* p);
+/* bytes of workspace of the forward / the backward (the latter may be 0) */
+size_t ugpg_distill_workspace(const ugpg_distill_t* p, int backward);
 /* loss[0] = the rows' sum, row_loss [N][inner] each row's (one at least given); dlogits
  * (nullable): d loss / d logits, packed ([N][V], or the maps' layout), the logits' type --
  * written with the sums of the same row, while the row is in the caches */

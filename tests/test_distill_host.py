@@ -76,17 +76,19 @@ def test_c_entries_refuse_before_any_launch():
                dict(index_bits=16), dict(k=0), dict(temperature=-1.0), dict(scale=float("nan")), dict(stride=3),
                dict(inner=2, V=1025, stride=2050, k=3)):
         d = desc(**kw)
-        assert lib.ugpg_distill_workspace(C.byref(d)) == 0
+        assert lib.ugpg_distill_workspace(C.byref(d), 0) == 0
         assert lib.ugpg_distill_fwd(C.byref(d), p, None, None, p, 1 << 30, None) == -1, kw
         assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, p, p, 1 << 30, None) == -1, kw
         assert b"distill_bwd" in lib.ugpg_last_error()
     for kw in (dict(), dict(N=3, V=100000, stride=100000), dict(inner=100, stride=900)):
         d = desc(**kw)
-        need = lib.ugpg_distill_workspace(C.byref(d))
-        assert need > 0
+        need, nb = (lib.ugpg_distill_workspace(C.byref(d), b) for b in (0, 1))
+        assert need > 0 and (nb > 0) == (d.V > 512)
         assert lib.ugpg_distill_fwd(C.byref(d), p, None, None, p, need - 1, None) == -3
         assert lib.ugpg_distill_fwd(C.byref(d), p, None, None, None, need, None) == -3
-        assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, p, p, need - 1, None) == -3
+        if nb:
+            assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, p, p, nb - 1, None) == -3
+            assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, p, None, nb, None) == -3
     d = desc()
     assert lib.ugpg_distill_fwd(C.byref(d), None, None, None, p, 1 << 20, None) == -1
     assert lib.ugpg_distill_bwd(C.byref(d), None, 0, 0, p, p, 1 << 20, None) == -1

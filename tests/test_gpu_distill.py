@@ -387,8 +387,8 @@ def test_writes_stay_inside(dev, shape, k):
     from ugpg import _C, ops
     for dtype in (F32, BF16):
         z, v, i, r, w = record(shape, k, dev, dtype, 2.0)
-        d, x, ws = ops._distill_desc(z, v, i, r, w, 2.0, 1.0)
-        need = _C.lib.ugpg_distill_workspace(C.byref(d))
+        call = ops.DistillCall(z, v, i, r, w, 2.0, 1.0)
+        d, need = call.desc, call.nbytes
         work = guarded((need,), dev, torch.uint8)
         loss, rows = guarded((1,), dev), guarded((z.numel() // shape[1],), dev)
         dz = guarded(shape, dev, dtype)
@@ -396,7 +396,7 @@ def test_writes_stay_inside(dev, shape, k):
                                          work.t.data_ptr(), need, ops.stream()), "distill_fwd")
         for n, t in (("ws", work), ("loss", loss), ("rows", rows), ("dlogits", dz)):
             t.check(n)
-        want, grad = ops.distill_fwd(z, v, i, r, w, 2.0, 1.0, grad=True)
+        want, grad = call.forward(grad=True)
         assert torch.equal(want.view(1), loss.t) and torch.equal(grad, dz.t)
         # a partial record's buffers too
         vals, idx, rest = guarded(v.shape, dev, dtype), guarded((2 * i.numel(),), dev, torch.int32), guarded(r.shape, dev)
@@ -471,6 +471,28 @@ def test_offsets_past_32_bits(dev):
     rows, dz, size, unit = ref_loss(z[N - 2:].detach(), top.values, top.indices, full.rest[N - 2:], None, 2.0, 1.0)
     assert ((loss[N - 2:].double() - rows).abs() <= REL * unit + 2.0 ** -23 * rows.abs()).all()
     check_grad(g[N - 2:], dz, size)
+
+
+def test_differentiable_once(dev):
+    """Second derivatives are refused, not silently zero; create_graph alone is fine."""
+    import ugpg
+    z, v, i, r, w = record((30, 7), 3, dev, F32, 2.0)
+    zr = z.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(ugpg.distillation_loss(zr, (v, i, r), 2.0), (zr,), create_graph=True)
+    (h,) = torch.autograd.grad(ugpg.distillation_loss(zr, (v, i, r), 2.0), (zr,))
+    assert torch.equal(g.detach(), h)
+    with pytest.raises(RuntimeError, match="once"):
+        g.sum().backward()
+
+
+def test_record_written_after_the_forward_is_noticed(dev):
+    import ugpg
+    z, v, i, r, w = record((30, 7), 3, dev, F32, 2.0)
+    zr = z.clone().requires_grad_(True)
+    loss = ugpg.distillation_loss(zr, (v, i, r), 2.0, weight=w)
+    v.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        (2 * loss).backward()
 
 
 def test_loss_object(dev):

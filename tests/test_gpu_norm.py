@@ -210,11 +210,12 @@ def test_same_bits_every_time_and_inside_bounds(dev):
         x, w, b, dy = make(shape, G, dev, torch.float32, "relu", seed=6)
         first = None
         for _ in range(3):
-            y, mean, rstd = ops.group_norm_fwd(x, G, w, b, 1e-5, "relu")
+            call = ops.GroupNormCall(x, G, w, b, 1e-5, "relu")
+            y, mean, rstd = call.forward(), call.mean, call.rstd
             dx = guarded(shape, dev)
             C = shape[-1]
             dw, db, dxs = (guarded((C,), dev) for _ in range(3))
-            ops.group_norm_bwd(dy, x, G, mean, rstd, w, b, "relu", dx.t, dw.t, db.t, dxs.t)
+            ops.group_norm_bwd(call, dy, dx.t, dw.t, db.t, dxs.t)
             for n, t in (("dx", dx), ("dw", dw), ("db", db), ("dxsum", dxs)):
                 t.check(n)
             now = [y, mean, rstd, dx.t, dw.t, db.t, dxs.t]
@@ -234,13 +235,14 @@ def test_mixed_types_of_the_bf16_arithmetic(dev, shape, G, out):
     x, w, b, _ = make(shape, G, dev, torch.bfloat16, "relu", seed=8)
     g = torch.Generator(device=dev).manual_seed(1)
     dy = torch.randn(shape, generator=g, device=dev)
-    _, mean, rstd = ops.group_norm_fwd(x, G, w, b, 1e-5, "relu")
+    call = ops.GroupNormCall(x, G, w, b, 1e-5, "relu")
+    call.forward()
     dx = torch.empty(shape, dtype=out, device=dev)
-    ops.group_norm_bwd(dy, x, G, mean, rstd, w, b, "relu", dx)
+    ops.group_norm_bwd(call, dy, dx)
     _, edx, _, _, r = ref(x, G, w, b, 1e-5, "relu", dy)
     near(dx, edx, 512.0 * r.max().item(), "dx", HALF16 if out == torch.bfloat16 else 0.0)
     if out == torch.float32:  # in place over the upstream gradient
-        ops.group_norm_bwd(dy, x, G, mean, rstd, w, b, "relu", dy)
+        ops.group_norm_bwd(call, dy, dy)
         assert torch.equal(dy, dx)
 
 
@@ -289,6 +291,19 @@ def test_other_stream_and_captured_graph(dev):
             fresh = [t.detach().clone().requires_grad_(True) for t in args]
             ex = step(*fresh, dy)
             assert all(torch.equal(a, c) for a, c in zip(outs, ex)), k
+
+
+def test_differentiable_once(dev):
+    """Second derivatives are refused, not silently left out; create_graph alone is fine."""
+    import ugpg
+    x, w, b, dy = make((2, 6, 5, 24), 4, dev, torch.float32, "silu")
+    leaf = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(ugpg.group_norm_act(leaf[0], 4, *leaf[1:], activation="silu"), leaf, dy)
+    got = torch.autograd.grad(ugpg.group_norm_act(leaf[0], 4, *leaf[1:], activation="silu"), leaf, dy,
+                              create_graph=True)
+    assert all(torch.equal(a, c.detach()) for a, c in zip(want, got))
+    with pytest.raises(RuntimeError, match="only once"):
+        (got[0].sum() + leaf[0].sum()).backward()
 
 
 def test_offsets_past_32_bits(dev):

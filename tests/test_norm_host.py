@@ -38,27 +38,35 @@ def test_module_refuses_bad_arguments():
 
 
 def test_c_entries_refuse_before_any_launch():
+    import ctypes as C
     from ugpg import _C
     lib, p = _C.lib, 0x1000  # never dereferenced on the host
-    need = lib.ugpg_group_norm_workspace(2, 64, 32, 4, 0)
-    assert need > 0 and lib.ugpg_group_norm_workspace(2, 64, 32, 5, 0) == 0
 
-    def fwd(x=p, dt=0, B=2, hw=64, C=32, G=4, eps=1e-5, act=1, y=p, mean=p, ws=p, n=need):
-        return lib.ugpg_group_norm_fwd(x, dt, B, hw, C, G, None, None, eps, act, y, mean, p, ws, n, None)
-    for kw in (dict(x=None), dict(dt=2), dict(B=0), dict(hw=0), dict(C=30), dict(G=0), dict(eps=-1.0),
-               dict(eps=float("nan")), dict(act=3), dict(act=-1), dict(y=None), dict(mean=None),
-               dict(C=1 << 21, G=1), dict(B=1 << 22, G=8), dict(hw=1 << 41)):
-        assert fwd(**kw) == -1, kw
+    def desc(**kw):
+        f = dict(x=p, dtype=0, B=2, HW=64, C=32, G=4, gamma=None, beta=None, eps=1e-5, act=1, mean=p, rstd=p)
+        f.update(kw)
+        return C.byref(_C.GroupNormDesc(*f.values()))
+    sizes = (dict(dtype=2), dict(B=0), dict(HW=0), dict(C=30), dict(G=0), dict(G=5), dict(eps=-1.0),
+             dict(eps=float("nan")), dict(act=3), dict(act=-1), dict(C=1 << 21, G=1), dict(B=1 << 22, G=8),
+             dict(HW=1 << 41))
+    big = 1 << 40
+    for kw in (*sizes, dict(x=None), dict(mean=None), dict(rstd=None)):
+        assert lib.ugpg_group_norm_fwd(desc(**kw), p, p, big, None) == -1, kw
         assert b"group_norm_fwd" in lib.ugpg_last_error()
-    assert fwd(n=need - 1) == -3 and fwd(ws=None) == -3
-
-    nb = lib.ugpg_group_norm_workspace(2, 64, 32, 4, 1)
-
-    def bwd(dy=p, dyt=0, x=p, dt=0, dx=p, dxt=0, mean=p, G=4, n=nb):
-        return lib.ugpg_group_norm_bwd(dy, dyt, x, dt, 2, 64, 32, G, mean, p, None, None, 1, dx, dxt,
-                                       None, None, None, p, n, None)
-    for kw in (dict(dy=None), dict(x=None), dict(dx=None), dict(mean=None), dict(G=5),
-               dict(dyt=1), dict(dxt=1), dict(dt=1, dyt=1), dict(dt=2)):
-        assert bwd(**kw) == -1, kw
+        assert lib.ugpg_group_norm_bwd(desc(**kw), p, kw.get("dtype", 0), p, kw.get("dtype", 0), None, None,
+                                       None, p, big, None) == -1, kw
         assert b"group_norm_bwd" in lib.ugpg_last_error()
+    for kw in sizes:
+        assert lib.ugpg_group_norm_workspace(desc(**kw), 0) == 0
+        assert lib.ugpg_group_norm_workspace(desc(**kw), 1) == 0
+    need, nb = (lib.ugpg_group_norm_workspace(desc(), k) for k in (0, 1))
+    assert 0 < need <= nb
+    assert lib.ugpg_group_norm_fwd(None, p, p, big, None) == -1
+    assert lib.ugpg_group_norm_fwd(desc(), None, p, big, None) == -1
+    assert lib.ugpg_group_norm_fwd(desc(), p, p, need - 1, None) == -3
+    assert lib.ugpg_group_norm_fwd(desc(), p, None, need, None) == -3
+    bwd = lambda d=0, dy=p, dyt=0, dx=p, dxt=0, n=nb: lib.ugpg_group_norm_bwd(
+        desc(dtype=d), dy, dyt, dx, dxt, None, None, None, p, n, None)
     assert bwd(n=nb - 1) == -3
+    for kw in (dict(dy=None), dict(dx=None), dict(dyt=1), dict(dxt=1), dict(d=1, dyt=1)):
+        assert bwd(**kw) == -1, kw

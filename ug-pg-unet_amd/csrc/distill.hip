@@ -1050,10 +1050,10 @@ static int distill_check(const char* what, const ugpg_distill_t* p) {
     return UGPG_OK;
 }
 
-extern "C" size_t ugpg_distill_workspace(const ugpg_distill_t* p) {
+extern "C" size_t ugpg_distill_workspace(const ugpg_distill_t* p, int backward) {
     if (distill_check("distill_workspace", p)) return 0;
-    if (p->inner > 1) return (size_t)cdiv(p->N * p->inner, 256) * 8;
-    size_t n = (size_t)p->N * 8;
+    if (p->inner > 1) return backward ? 0 : (size_t)cdiv(p->N * p->inner, 256) * 8;
+    size_t n = backward ? 0 : (size_t)p->N * 8;  // the rows' losses, then the parts of split rows
     if (p->V > DW_MAX) {
         const Split sp = row_split(p->N, p->V);
         if (sp.n > 1) n += (size_t)p->N * sp.n * 8;
@@ -1062,7 +1062,8 @@ extern "C" size_t ugpg_distill_workspace(const ugpg_distill_t* p) {
 }
 
 template <typename T>
-static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, void* ws, hipStream_t s) {
+static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, bool backward, void* ws,
+                       hipStream_t s) {
     const int es = sizeof(T);
     const int64_t rows = a.rows;
     int64_t nsum = rows;
@@ -1100,7 +1101,7 @@ static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, void
             else
                 hipLaunchKernelGGL((distill_row_kernel<T, false>), dim3((unsigned)rows), dim3(nt), lds(a.V), s, a);
         } else {
-            float* part = reinterpret_cast<float*>(static_cast<double*>(ws) + rows);
+            float* part = reinterpret_cast<float*>(static_cast<double*>(ws) + (backward ? 0 : rows));
             const unsigned g = (unsigned)(rows * sp.n);
             hipLaunchKernelGGL((distill_part_kernel<T>), dim3(g), dim3(256), lds(sp.chunk), s, a, sp.n, sp.chunk, part);
             // without a gradient one block a row joins them, over no classes of its own
@@ -1137,9 +1138,10 @@ static DistillArgs distill_args(const ugpg_distill_t* p) {
     return a;
 }
 
-static int distill_ws_check(const char* what, const ugpg_distill_t* p, const void* ws, size_t n) {
-    const size_t need = ugpg_distill_workspace(p);
-    if (!ws || n < need) {
+static int distill_ws_check(const char* what, const ugpg_distill_t* p, int backward, const void* ws,
+                            size_t n) {
+    const size_t need = ugpg_distill_workspace(p, backward);
+    if (need && (!ws || n < need)) {
         set_error("%s: workspace %zu < %zu", what, n, need);
         return UGPG_ERR_WORKSPACE;
     }
@@ -1153,12 +1155,12 @@ extern "C" int ugpg_distill_fwd(const ugpg_distill_t* p, float* loss, float* row
         set_error("distill_fwd: neither loss nor row_loss given");
         return UGPG_ERR_INVALID;
     }
-    if (int rc = distill_ws_check("distill_fwd", p, ws, ws_bytes)) return rc;
+    if (int rc = distill_ws_check("distill_fwd", p, 0, ws, ws_bytes)) return rc;
     DistillArgs a = distill_args(p);
     a.row_out = row_loss;
     a.dz = dlogits;
-    return p->dtype == UGPG_DT_F32 ? distill_run<float>(p, a, loss, ws, as_stream(stream))
-                                   : distill_run<__bf16>(p, a, loss, ws, as_stream(stream));
+    return p->dtype == UGPG_DT_F32 ? distill_run<float>(p, a, loss, false, ws, as_stream(stream))
+                                   : distill_run<__bf16>(p, a, loss, false, ws, as_stream(stream));
 }
 
 extern "C" int ugpg_distill_bwd(const ugpg_distill_t* p, const float* gout, int per_row, int skip_one,
@@ -1168,12 +1170,12 @@ extern "C" int ugpg_distill_bwd(const ugpg_distill_t* p, const float* gout, int 
         set_error("distill_bwd: bad arguments (per_row=%d skip_one=%d)", per_row, skip_one);
         return UGPG_ERR_INVALID;
     }
-    if (int rc = distill_ws_check("distill_bwd", p, ws, ws_bytes)) return rc;
+    if (int rc = distill_ws_check("distill_bwd", p, 1, ws, ws_bytes)) return rc;
     DistillArgs a = distill_args(p);
     a.gout = gout;
     a.gout_rows = per_row != 0;
     a.skip_one = skip_one != 0;
     a.dz = dlogits;
-    return p->dtype == UGPG_DT_F32 ? distill_run<float>(p, a, nullptr, ws, as_stream(stream))
-                                   : distill_run<__bf16>(p, a, nullptr, ws, as_stream(stream));
+    return p->dtype == UGPG_DT_F32 ? distill_run<float>(p, a, nullptr, true, ws, as_stream(stream))
+                                   : distill_run<__bf16>(p, a, nullptr, true, ws, as_stream(stream));
 }

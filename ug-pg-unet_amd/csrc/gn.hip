@@ -744,17 +744,27 @@ static GnGeom gn_geom(int B, int64_t P, int C, int G, int V) {
     return g;
 }
 
-static int gn_check(const char* what, const void* x, int B, int64_t P, int C, int G, int act) {
-    if (!x || B <= 0 || P <= 0 || C <= 0 || G <= 0 || C % G || act < UGPG_ACT_NONE ||
-        act > UGPG_ACT_SILU) {
-        set_error("%s: bad arguments (B=%d HW=%lld C=%d groups=%d act=%d)", what, B, (long long)P, C,
-                  G, act);
+static int gn_check(const char* what, const ugpg_group_norm_t* p, bool tensors) {
+    if (!p) {
+        set_error("%s: no descriptor", what);
+        return UGPG_ERR_INVALID;
+    }
+    if (p->B <= 0 || p->HW <= 0 || p->C <= 0 || p->G <= 0 || p->C % p->G ||
+        (p->dtype != UGPG_DT_F32 && p->dtype != UGPG_DT_BF16) || p->act < UGPG_ACT_NONE ||
+        p->act > UGPG_ACT_SILU || !(p->eps >= 0.f)) {
+        set_error("%s: bad arguments (dtype=%d B=%d HW=%lld C=%d groups=%d eps=%g act=%d)", what,
+                  p->dtype, p->B, (long long)p->HW, p->C, p->G, (double)p->eps, p->act);
+        return UGPG_ERR_INVALID;
+    }
+    if (tensors && (!p->x || !p->mean || !p->rstd)) {
+        set_error("%s: x, mean and rstd must be given", what);
         return UGPG_ERR_INVALID;
     }
     // (grids: B*G blocks, B * column blocks; offsets are 64-bit)
-    if (C > (1 << 20) || (int64_t)B * G > (1 << 22) || (int64_t)B * cdiv(C, 256) > (1 << 22) ||
-        P > ((int64_t)1 << 40) || (double)B * (double)P * (double)C > 1e15) {
-        set_error("%s: B=%d HW=%lld C=%d is too large", what, B, (long long)P, C);
+    if (p->C > (1 << 20) || (int64_t)p->B * p->G > (1 << 22) ||
+        (int64_t)p->B * cdiv(p->C, 256) > (1 << 22) || p->HW > ((int64_t)1 << 40) ||
+        (double)p->B * (double)p->HW * (double)p->C > 1e15) {
+        set_error("%s: B=%d HW=%lld C=%d is too large", what, p->B, (long long)p->HW, p->C);
         return UGPG_ERR_INVALID;
     }
     return UGPG_OK;
@@ -776,16 +786,21 @@ static size_t gn_part_floats(int B, int64_t P, int C, int G, int per) {
 
 using namespace ugpg;
 
-extern "C" size_t ugpg_group_norm_workspace(int B, int64_t HW, int C, int G, int backward) {
-    if (B <= 0 || HW <= 0 || C <= 0 || G <= 0 || C % G) return 0;
-    if (!backward) return gn_part_floats(B, HW, C, G, 2) * 4;
-    return (gn_part_floats(B, HW, C, G, 3) + (size_t)B * 3 * C + (size_t)B * G * 2) * 4;
+extern "C" size_t ugpg_group_norm_workspace(const ugpg_group_norm_t* p, int backward) {
+    if (gn_check("group_norm_workspace", p, false)) return 0;
+    if (!backward) return gn_part_floats(p->B, p->HW, p->C, p->G, 2) * 4;
+    return (gn_part_floats(p->B, p->HW, p->C, p->G, 3) + (size_t)p->B * 3 * p->C +
+            (size_t)p->B * p->G * 2) * 4;
 }
 
 template <typename T, int V>
-static int gn_fwd_run(const void* x, int B, int64_t P, int C, int G, const float* gamma,
-                      const float* beta, float eps, int act, void* y, float* mean, float* rstd,
-                      void* ws, hipStream_t s) {
+static int gn_fwd_run(const ugpg_group_norm_t* d, void* y, void* ws, hipStream_t s) {
+    const void* x = d->x;
+    const int B = d->B, C = d->C, G = d->G, act = d->act;
+    const int64_t P = d->HW;
+    const float *gamma = d->gamma, *beta = d->beta;
+    const float eps = d->eps;
+    float *mean = d->mean, *rstd = d->rstd;
     const T* xt = static_cast<const T*>(x);
     GnSlab sl;
     int nt;
@@ -811,24 +826,29 @@ static int gn_fwd_run(const void* x, int B, int64_t P, int C, int G, const float
     return check_launch("group_norm_fwd");
 }
 
-extern "C" int ugpg_group_norm_fwd(const void* x, int dtype, int B, int64_t HW, int C, int G,
-                                   const float* gamma, const float* beta, float eps, int act,
-                                   void* y, float* mean, float* rstd, void* ws, size_t ws_bytes,
-                                   void* stream) {
-    if (int rc = gn_check("group_norm_fwd", x, B, HW, C, G, act)) return rc;
-    if (!y || !mean || !rstd || !(eps >= 0.f) || (dtype != UGPG_DT_F32 && dtype != UGPG_DT_BF16)) {
-        set_error("group_norm_fwd: bad arguments (eps=%g dtype=%d)", (double)eps, dtype);
-        return UGPG_ERR_INVALID;
-    }
-    const size_t need = ugpg_group_norm_workspace(B, HW, C, G, 0);
-    if (!ws || ws_bytes < need) {
-        set_error("group_norm_fwd: workspace %zu < %zu", ws_bytes, need);
+static int gn_ws_check(const char* what, const ugpg_group_norm_t* p, int backward, const void* ws,
+                       size_t n) {
+    const size_t need = ugpg_group_norm_workspace(p, backward);
+    if (!ws || n < need) {
+        set_error("%s: workspace %zu < %zu", what, n, need);
         return UGPG_ERR_WORKSPACE;
     }
-    const int es = dtype == UGPG_DT_F32 ? 4 : 2;
-    const int v = gn_pick(B, HW, C, G, gn_vec(C, 16 / es, x, es, y, es, nullptr, es), es, 16);
+    return UGPG_OK;
+}
+
+extern "C" int ugpg_group_norm_fwd(const ugpg_group_norm_t* p, void* y, void* ws, size_t ws_bytes,
+                                   void* stream) {
+    if (int rc = gn_check("group_norm_fwd", p, true)) return rc;
+    if (!y) {
+        set_error("group_norm_fwd: no output");
+        return UGPG_ERR_INVALID;
+    }
+    if (int rc = gn_ws_check("group_norm_fwd", p, 0, ws, ws_bytes)) return rc;
+    const int es = p->dtype == UGPG_DT_F32 ? 4 : 2;
+    const int v = gn_pick(p->B, p->HW, p->C, p->G, gn_vec(p->C, 16 / es, p->x, es, y, es, nullptr, es),
+                          es, 16);
     hipStream_t s = as_stream(stream);
-#define GN_FWD(T, V) gn_fwd_run<T, V>(x, B, HW, C, G, gamma, beta, eps, act, y, mean, rstd, ws, s)
+#define GN_FWD(T, V) gn_fwd_run<T, V>(p, y, ws, s)
     if (es == 4) return v == 4 ? GN_FWD(float, 4) : v == 2 ? GN_FWD(float, 2) : GN_FWD(float, 1);
     return v == 8 ? GN_FWD(__bf16, 8) : v == 4 ? GN_FWD(__bf16, 4) : v == 2 ? GN_FWD(__bf16, 2)
                                                                          : GN_FWD(__bf16, 1);
@@ -836,10 +856,12 @@ extern "C" int ugpg_group_norm_fwd(const void* x, int dtype, int B, int64_t HW, 
 }
 
 template <typename T, typename TD, typename TO, int V>
-static int gn_bwd_run(const void* dy, const void* x, int B, int64_t P, int C, int G,
-                      const float* mean, const float* rstd, const float* gamma, const float* beta,
-                      int act, void* dx, float* dgamma, float* dbeta, float* dxsum, void* ws,
-                      hipStream_t s) {
+static int gn_bwd_run(const ugpg_group_norm_t* p, const void* dy, void* dx, float* dgamma,
+                      float* dbeta, float* dxsum, void* ws, hipStream_t s) {
+    const void* x = p->x;
+    const int B = p->B, C = p->C, G = p->G, act = p->act;
+    const int64_t P = p->HW;
+    const float *gamma = p->gamma, *beta = p->beta, *mean = p->mean, *rstd = p->rstd;
     const T* xt = static_cast<const T*>(x);
     const TD* dt = static_cast<const TD*>(dy);
     float* tot = static_cast<float*>(ws);
@@ -873,32 +895,25 @@ static int gn_bwd_run(const void* dy, const void* x, int B, int64_t P, int C, in
     return check_launch("group_norm_bwd");
 }
 
-extern "C" int ugpg_group_norm_bwd(const void* dy, int dy_dtype, const void* x, int dtype, int B,
-                                   int64_t HW, int C, int G, const float* mean, const float* rstd,
-                                   const float* gamma, const float* beta, int act, void* dx,
+extern "C" int ugpg_group_norm_bwd(const ugpg_group_norm_t* p, const void* dy, int dy_dtype, void* dx,
                                    int dx_dtype, float* dgamma, float* dbeta, float* dxsum, void* ws,
                                    size_t ws_bytes, void* stream) {
-    if (int rc = gn_check("group_norm_bwd", x, B, HW, C, G, act)) return rc;
-    const int F = UGPG_DT_F32, H = UGPG_DT_BF16;
+    if (int rc = gn_check("group_norm_bwd", p, true)) return rc;
+    const int F = UGPG_DT_F32, H = UGPG_DT_BF16, dtype = p->dtype;
     const bool fff = dtype == F && dy_dtype == F && dx_dtype == F;
     const bool hhh = dtype == H && dy_dtype == H && dx_dtype == H;
     const bool hfh = dtype == H && dy_dtype == F && dx_dtype == H;
     const bool hff = dtype == H && dy_dtype == F && dx_dtype == F;
-    if (!dy || !dx || !mean || !rstd || !(fff || hhh || hfh || hff)) {
+    if (!dy || !dx || !(fff || hhh || hfh || hff)) {
         set_error("group_norm_bwd: bad arguments (x, dy, dx types %d %d %d)", dtype, dy_dtype,
                   dx_dtype);
         return UGPG_ERR_INVALID;
     }
-    const size_t need = ugpg_group_norm_workspace(B, HW, C, G, 1);
-    if (!ws || ws_bytes < need) {
-        set_error("group_norm_bwd: workspace %zu < %zu", ws_bytes, need);
-        return UGPG_ERR_WORKSPACE;
-    }
+    if (int rc = gn_ws_check("group_norm_bwd", p, 1, ws, ws_bytes)) return rc;
     const int ex = dtype == F ? 4 : 2, ed = dy_dtype == F ? 4 : 2, eo = dx_dtype == F ? 4 : 2;
-    const int v = gn_pick(B, HW, C, G, gn_vec(C, 16 / ex, x, ex, dy, ed, dx, eo), ed, 8);
+    const int v = gn_pick(p->B, p->HW, p->C, p->G, gn_vec(p->C, 16 / ex, p->x, ex, dy, ed, dx, eo), ed, 8);
     hipStream_t s = as_stream(stream);
-#define GN_BWD(T, TD, TO, V) \
-    gn_bwd_run<T, TD, TO, V>(dy, x, B, HW, C, G, mean, rstd, gamma, beta, act, dx, dgamma, dbeta, dxsum, ws, s)
+#define GN_BWD(T, TD, TO, V) gn_bwd_run<T, TD, TO, V>(p, dy, dx, dgamma, dbeta, dxsum, ws, s)
 #define GN_BWD_H(TD, TO)                              \
     (v == 8 ? GN_BWD(__bf16, TD, TO, 8) : v == 4 ? GN_BWD(__bf16, TD, TO, 4) \
      : v == 2 ? GN_BWD(__bf16, TD, TO, 2) : GN_BWD(__bf16, TD, TO, 1))

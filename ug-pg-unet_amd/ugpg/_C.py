@@ -61,6 +61,12 @@ class WgradDesc(C.Structure):
                 ("dy_bn", C.POINTER(BnLazy))]
 
 
+class GroupNormDesc(C.Structure):
+    """ugpg_group_norm_t."""
+    _fields_ = [("x", _p), ("dtype", _i), ("B", _i), ("HW", _i64), ("C", _i), ("G", _i),
+                ("gamma", _p), ("beta", _p), ("eps", _f), ("act", _i), ("mean", _p), ("rstd", _p)]
+
+
 class DistillDesc(C.Structure):
     """ugpg_distill_t."""
     _fields_ = [("logits", _p), ("dtype", _i), ("N", _i64), ("V", _i), ("inner", _i64),
@@ -149,12 +155,11 @@ SIGNATURES = {
     "ugpg_adam_step": (_i, [_p, _p, _p, _p, _i64, _f, _f, _f, _f, _f, _i64, _f, _p]),
     "ugpg_relu_bwd": (_i, [_p, _p, _p, _i64, _p]),
     "ugpg_mul": (_i, [_p, _p, _p, _i64, _p]),
-    "ugpg_group_norm_workspace": (_sz, [_i, _i64, _i, _i, _i]),
-    "ugpg_group_norm_fwd": (_i, [_p, _i, _i, _i64, _i, _i, _p, _p, _f, _i, _p, _p, _p, _p, _sz, _p]),
-    "ugpg_group_norm_bwd": (_i, [_p, _i, _p, _i, _i, _i64, _i, _i, _p, _p, _p, _p, _i, _p, _i, _p,
-                                 _p, _p, _p, _sz, _p]),
+    "ugpg_group_norm_workspace": (_sz, [C.POINTER(GroupNormDesc), _i]),
+    "ugpg_group_norm_fwd": (_i, [C.POINTER(GroupNormDesc), _p, _p, _sz, _p]),
+    "ugpg_group_norm_bwd": (_i, [C.POINTER(GroupNormDesc), _p, _i, _p, _i, _p, _p, _p, _p, _sz, _p]),
     "ugpg_top_logits": (_i, [_p, _i, _i64, _i, _i64, _i64, _i, _f, _p, _p, _p, _p]),
-    "ugpg_distill_workspace": (_sz, [C.POINTER(DistillDesc)]),
+    "ugpg_distill_workspace": (_sz, [C.POINTER(DistillDesc), _i]),
     "ugpg_distill_fwd": (_i, [C.POINTER(DistillDesc), _p, _p, _p, _p, _sz, _p]),
     "ugpg_distill_bwd": (_i, [C.POINTER(DistillDesc), _p, _i, _i, _p, _p, _sz, _p]),
     "ugpg_resample_aa_u8": (_i, [_p, _i64, _i, _i, _i, _p, _p, _i, _p, _p]),
@@ -215,7 +220,10 @@ class _Lib:
         return self._lib
 
     def __getattr__(self, name):
-        return getattr(self.load(), name)
+        fn = getattr(self.load(), name)
+        if name in SIGNATURES:  # found on the instance from now on, without this call
+            self.__dict__[name] = fn
+        return fn
 
 
 lib = _Lib()

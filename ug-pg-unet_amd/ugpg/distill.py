@@ -12,7 +12,6 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
@@ -64,21 +63,25 @@ class _DistillFn(torch.autograd.Function):
     def forward(ctx, logits, values, indices, rest, weight, temperature, scale, per_row, grad):
         # With a gradient to come, a scalar loss writes it here, for an upstream gradient of 1,
         # while each row is in the caches: one reading of the logits instead of two.
-        args = (logits, values, indices, rest, weight, temperature, scale)
         with ops.on_device(logits):
-            loss, dz = ops.distill_fwd(*args, per_row=per_row, grad=grad and not per_row)
-        ctx.save_for_backward(*args[:5])
-        ctx.temperature, ctx.scale, ctx.dz = temperature, scale, dz
+            call = ops.DistillCall(logits, values, indices, rest, weight, temperature, scale)
+            loss, dz = call.forward(per_row, grad and not per_row)
+        if grad:
+            ctx.save_for_backward(logits, values, indices, rest, weight)
+            ctx.call, ctx.dz = call, dz
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gout):
         dz, ctx.dz = ctx.dz, None  # handed out once; a second backward writes its own
-        with ops.on_device(gout):
-            dz = ops.distill_bwd(*ctx.saved_tensors, ctx.temperature, ctx.scale,
-                                 gout.contiguous().float(), dz)
-        return (dz, *[None] * 8)
+        ctx.saved_tensors  # (raises if one was written in place since)
+        twice = torch.is_grad_enabled()  # create_graph
+        if gout.dtype != torch.float32 or not gout.is_contiguous():
+            gout = gout.detach().float().contiguous()
+        dz = ctx.call.backward(gout, dz)
+        if twice:
+            (dz,) = ops.differentiable_once("distillation_loss", (dz,))
+        return dz, None, None, None, None, None, None, None, None
 
 
 def distillation_loss(logits, top, temperature=1.0, weight=None, reduction="mean", scale=1.0):

@@ -9,32 +9,34 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from . import ops
 
 
 class _GroupNormActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act):
+    def forward(ctx, x, weight, bias, groups, eps, act, grad):
         with ops.on_device(x):
-            y, mean, rstd = ops.group_norm_fwd(x, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.groups, ctx.act = groups, act
+            call = ops.GroupNormCall(x, groups, weight, bias, eps, act)
+            y = call.forward()
+        if grad:
+            ctx.save_for_backward(x, weight, bias)
+            ctx.call = call
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
+        ctx.saved_tensors  # (raises if one was written in place since)
         need = ctx.needs_input_grad
-        with ops.on_device(x):
-            dx = torch.empty_like(x)
-            dw = torch.empty_like(weight) if need[1] else None
-            db = torch.empty_like(bias) if need[2] else None
-            ops.group_norm_bwd(dy.contiguous(), x, ctx.groups, mean, rstd, weight, bias, ctx.act, dx,
-                               dw, db)
-        return (dx if need[0] else None), dw, db, None, None, None
+        twice = torch.is_grad_enabled()  # create_graph
+        if dy.dtype != ctx.call.x.dtype or not dy.is_contiguous():
+            dy = dy.detach().to(ctx.call.x.dtype).contiguous()
+        dx, dw, db = ctx.call.backward(dy, need[1], need[2])
+        if not need[0]:
+            dx = None
+        if twice:
+            dx, dw, db = ops.differentiable_once("group_norm_act", (dx, dw, db))
+        return dx, dw, db, None, None, None, None
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="relu"):
@@ -68,9 +70,12 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
         raise RuntimeError("ugpg: tensor is not on a ROCm/HIP device (no CPU fallback)")
     if x.numel() == 0:
         raise ValueError(f"group_norm_act: empty input {tuple(x.shape)}")
-    weight = None if weight is None else weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
-    return _GroupNormActFn.apply(x.contiguous(), weight, bias, num_groups, float(eps), activation)
+    grad = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (x, weight, bias))
+    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
+    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
+    x = x if x.is_contiguous() else x.contiguous()
+    return _GroupNormActFn.apply(x, weight, bias, num_groups, float(eps), activation, grad)
 
 
 class GroupNormAct(nn.GroupNorm):
