@@ -122,6 +122,8 @@ def fill(kind, shape, dev, dtype, seed=1):
         z = torch.where(pos % 37 == 5, z, -math.inf)
     elif kind == "lowest":
         z = torch.where(pos % 37 == 5, z, low)
+    elif kind == "huge":  # products with log2(e)/T leave float32
+        z = torch.where(pos % 5 == 2, 3e38, torch.where(pos % 5 == 3, -3e38, z))
     elif kind == "nothing":
         z = torch.full(shape, -math.inf, device=dev)
     elif kind == "inf":
@@ -137,7 +139,7 @@ def fill(kind, shape, dev, dtype, seed=1):
     return z.to(dtype)
 
 
-KINDS = ["random", "equal", "ascending", "ties", "zeros", "masked", "lowest", "nothing", "inf", "nan",
+KINDS = ["random", "equal", "ascending", "ties", "zeros", "masked", "lowest", "huge", "nothing", "inf", "nan",
          "one_nan", "one_thread", "confident"]
 
 
@@ -146,7 +148,7 @@ KINDS = ["random", "equal", "ascending", "ties", "zeros", "masked", "lowest", "n
 def test_top_logits(dev, dtype, kind):
     import ugpg
     for shape, k in TOP_SHAPES:
-        for T in (1.0, 2.0) if kind == "random" else (1.5,):
+        for T in (0.5, 1.0, 2.0) if kind in ("random", "lowest", "huge") else (1.5,):
             z = fill(kind, shape, dev, dtype)
             top = ugpg.teacher_top_logits(z, k, T)
             v, i, r = ref_top(z, k, T)
@@ -314,6 +316,16 @@ def test_masked_students(dev, shape, k):
         loss = ugpg.distillation_loss(zr, (v, i, r), 0.5, reduction="sum")
         check_loss(loss, rows, unit)
         loss.backward()
+        check_grad(zr.grad, dz, size)
+    # everything outside the record at the type's lowest value, or beyond what T divides
+    for bad in (torch.finfo(F32).min, 3e38):
+        zb = torch.where(out, bad, z)
+        rows, dz, size, unit = ref_loss(zb, v, i, None, None, 0.5, 1.0)
+        zr = zb.clone().requires_grad_(True)
+        loss = ugpg.distillation_loss(zr, (v, i, None), 0.5, reduction="sum")
+        loss.backward()
+        if bad < 0:
+            check_loss(loss, rows, unit)
         check_grad(zr.grad, dz, size)
     # all others masked: with no rest in the record that is fine, with one it is infinite
     zb = torch.where(out, -math.inf, z)

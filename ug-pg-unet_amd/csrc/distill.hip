@@ -69,13 +69,37 @@ template <typename T> struct RowSpan {
             v.load(b + (size_t)i * N);
             f(i + 1, lo + head + i * N, v, N);
         }
+        ends(tid, nt, f);
+    }
+    // the same from the row's end: what an earlier scan read last is the likeliest in the caches
+    template <int U, typename F> __device__ __forceinline__ void scan_back(int tid, int nt, F f) const {
+        const T* b = z + lo + head;
+        int i = (nv - tid - 1) / nt * nt + tid;  // the thread's last vector
+        if (tid < nv) {
+            for (; i - (U - 1) * nt >= 0; i -= U * nt) {
+                Pack<T, N> v[U];
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u].load(b + (size_t)(i - u * nt) * N);
+#pragma unroll
+                for (int u = 0; u < U; ++u) f(i - u * nt + 1, lo + head + (i - u * nt) * N, v[u], N);
+            }
+            for (; i >= 0; i -= nt) {
+                Pack<T, N> v;
+                v.load(b + (size_t)i * N);
+                f(i + 1, lo + head + i * N, v, N);
+            }
+        }
+        ends(tid, nt, f);
+    }
+    // the parts that are no whole vector
+    template <typename F> __device__ __forceinline__ void ends(int tid, int nt, F f) const {
         if (tid == 0 && head > 0) f(0, lo, partial(lo, head), head);
         const int t0 = lo + head + nv * N;
         if (tid == 64 % nt && t0 < hi) f(nv + 1, t0, partial(t0, hi - t0), hi - t0);
     }
 };
 
-// running (max, sum of exp2((v - max) * c)); max -inf: nothing yet
+// (max, sum of exp2((v - max) * c)); max -inf: nothing yet
 struct MaxSum {
     float m, s;
     __device__ __forceinline__ void merge(float m2, float s2, float c) {
@@ -87,35 +111,49 @@ struct MaxSum {
         s = s * exp2_raw((m - mm) * c) + s2 * exp2_raw((m2 - mm) * c);
         m = mm;
     }
-    template <typename P> __device__ __forceinline__ void add(const P& v, int n, float c) {
-        // n values of a pack (compile-time n)
-        float mx = v.get(0);
-        for (int e = 1; e < n; ++e) mx = fmaxf(mx, v.get(e));
-        if (mx > m) {
-            s *= exp2_raw((m - mx) * c);
-            m = mx;
-        }
-        if (m == NEG_INF) {  // nothing, or values that are no numbers: the sum becomes one too
-            for (int e = 0; e < n; ++e) s += v.get(e) == NEG_INF ? 0.f : v.get(e);
-            return;
-        }
-        float t = 0.f;
-        for (int e = 0; e < n; ++e) t += exp2_raw((v.get(e) - m) * c);
-        s += t;
-    }
-    __device__ __forceinline__ void add1(float v, float c) {
-        if (v > m) {
-            s *= exp2_raw((m - v) * c);
-            m = v;
-        }
-        if (v != NEG_INF) s += exp2_raw((v - m) * c);  // (a NaN makes the sum one)
-    }
+    // the maximum first: one exponential a lane, not one a step
     __device__ __forceinline__ void wave(float c) {
+        float mm = m;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            const float m2 = __shfl_xor(m, o, 64), s2 = __shfl_xor(s, o, 64);
-            merge(m2, s2, c);
+        for (int o = 32; o > 0; o >>= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));
+        s = wave_sum(m == mm ? s : s * exp2_raw((m - mm) * c));  // (all -inf: s is 0, or a NaN)
+        m = mm;
+    }
+};
+// A product v * c below this is far from overflow, and exp2(v * c - mc) is one fma and one
+// exp2; values near the type's ends take the difference first.
+constexpr float EXP_SAFE = 1e38f;
+// A thread's running form: s = the sum of exp2(v * c - mc), mc = fl(m * c).  The rounding of
+// mc is a factor common to all terms; done() takes it out again.
+struct RunSum {
+    float m = NEG_INF, mc = NEG_INF, s = 0.f;
+    __device__ __forceinline__ void raise(float v, float c) {
+        if (v > m) {
+            const float vc = v * c;
+            const bool safe = fabsf(mc) < EXP_SAFE && fabsf(vc) < EXP_SAFE;
+            s *= exp2_raw(safe ? mc - vc : (m - v) * c);
+            m = v;
+            mc = vc;
         }
+    }
+    // n values (compile-time n, a power of two), mx their maximum
+    __device__ __forceinline__ void add(const float* v, int n, float mx, float c) {
+        raise(mx, c);
+        float t[8];
+        if (fabsf(mc) < EXP_SAFE) {
+            for (int e = 0; e < n; ++e) t[e] = exp2_raw(fmaf(v[e], c, -mc));
+        } else if (m == NEG_INF) {  // nothing, or values that are no numbers: nor is the sum then
+            for (int e = 0; e < n; ++e) t[e] = v[e] == NEG_INF ? 0.f : v[e];
+        } else {
+            for (int e = 0; e < n; ++e) t[e] = exp2_raw((v[e] - m) * c);
+        }
+        for (int h = n / 2; h > 0; h >>= 1)
+            for (int e = 0; e < h; ++e) t[e] += t[e + h];
+        s += t[0];
+    }
+    __device__ __forceinline__ void add1(float v, float c) { add(&v, 1, v, c); }
+    __device__ __forceinline__ MaxSum done(float c) const {
+        return MaxSum{m, fabsf(mc) < EXP_SAFE ? s * exp2_raw(-fmaf(m, c, -mc)) : s};
     }
 };
 
@@ -129,14 +167,16 @@ __device__ __forceinline__ MaxSum block_maxsum(MaxSum a, float c, float* sm) {
         sm[2 * w + 1] = a.s;
     }
     __syncthreads();
-    MaxSum r{sm[0], sm[1]};
-    for (int i = 1; i < nw; ++i) r.merge(sm[2 * i], sm[2 * i + 1], c);
+    MaxSum r{sm[0], 0.f};
+    for (int i = 1; i < nw; ++i) r.m = fmaxf(r.m, sm[2 * i]);
+    for (int i = 0; i < nw; ++i)
+        r.s += sm[2 * i] == r.m ? sm[2 * i + 1] : sm[2 * i + 1] * exp2_raw((sm[2 * i] - r.m) * c);
     return r;
 }
 
-__device__ __forceinline__ double wave_max_d(double v) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
 
@@ -177,60 +217,70 @@ __device__ __forceinline__ float distill_value(const DistillArgs& a, size_t at) 
 
 // what a row's k + 1 classes give (computed by one wave over entries in LDS)
 struct RowTerms {
-    double kl;        // NaN / inf as they come out
-    double M, rsq;    // teacher: max, 1 / sum
-    double m, rs;     // student: max, 1 / sum
-    double restdiff;  // (p_rest - q_rest) / s_rest (0 where the student's rest is empty)
-    bool empty;       // the record says nothing: no loss, no gradient
+    double kl;       // NaN / inf as they come out
+    double M, m, iT; // the teacher's and the student's maximum, 1 / T
+    float rsq, rs;   // 1 / sums
+    float restdiff;  // (p_rest - q_rest) / s_rest (0 where the student's rest is empty)
+    bool empty;      // the record says nothing: no loss, no gradient
+    // exp((t - M) / T): the quotient in fp64, rounded once
+    __device__ __forceinline__ float q(float t) const { return expf((float)(((double)t - M) * iT)); }
+    __device__ __forceinline__ float p(float z) const { return expf((float)(((double)z - m) * iT)); }
+    __device__ __forceinline__ float grad(double g, float t, float z) const {
+        return (float)(g * ((double)(p(z) * rs) - (double)(q(t) * rsq)));
+    }
 };
 
-// one wave; idx < 0: absent.  (mr, sr): the student's rest, running max and sum
+// One wave; idx < 0: absent.  r: the student's rest.  The exponentials are fp32 (their errors,
+// 2^-22 of each probability, do not favour one side), what the loss is the difference of --
+// logarithms of probabilities -- fp64.
 __device__ __forceinline__ RowTerms row_terms(const int* idx, const float* t, const float* z, int k,
                                               float rest, MaxSum r, double T) {
     const int lane = threadIdx.x & 63;
     const double iT = 1.0 / T;
     RowTerms o;
-    double M = rest, m = r.m;
+    float M = rest, m = r.m;
     for (int j = lane; j < k; j += 64)
         if (idx[j] >= 0) {
-            M = fmax(M, (double)t[j]);
-            m = fmax(m, (double)z[j]);
+            M = fmaxf(M, t[j]);
+            m = fmaxf(m, z[j]);
         }
-    o.M = wave_max_d(M);
-    o.m = wave_max_d(m);
-    double sq = 0, ss = 0;
+    M = wave_max(M);
+    m = wave_max(m);
+    o.M = M;
+    o.m = m;
+    o.iT = iT;
+    float sq = 0.f, ss = 0.f;
     for (int j = lane; j < k; j += 64)
         if (idx[j] >= 0) {
-            sq += exp(((double)t[j] - o.M) * iT);
-            ss += exp(((double)z[j] - o.m) * iT);
+            sq += o.q(t[j]);
+            ss += o.p(z[j]);
         }
-    sq = wave_sum_d(sq);
-    ss = wave_sum_d(ss);
-    const double er = rest == NEG_INF ? 0.0 : exp(((double)rest - o.M) * iT);
-    const double logr = r.m == NEG_INF ? (double)NEG_INF : ((double)r.m - o.m) * iT + log((double)r.s);
+    sq = wave_sum(sq);
+    ss = wave_sum(ss);
+    const float er = rest == NEG_INF ? 0.f : o.q(rest);
+    const float sr = r.m == NEG_INF ? r.s : r.s * o.p(r.m);  // (an empty rest's sum is 0, or a NaN)
     sq += er;
-    ss += r.m == NEG_INF ? (double)r.s : exp(logr);  // (an empty rest's sum is 0, or a NaN)
-    o.rsq = 1.0 / sq;
-    o.rs = 1.0 / ss;
-    const double lq = log(sq), ls = log(ss);
+    ss += sr;
+    o.rsq = 1.f / sq;
+    o.rs = 1.f / ss;
+    // log q_j - log p_j = (t_j - M)/T - (z_j - m)/T - shift
+    const double lq = log((double)sq), ls = log((double)ss);
     double kl = 0;
     for (int j = lane; j < k; j += 64)
         if (idx[j] >= 0) {
-            const double a = ((double)t[j] - o.M) * iT;
-            const double q = exp(a) * o.rsq;
-            if (!(q == 0.0)) kl += q * ((a - lq) - (((double)z[j] - o.m) * iT - ls));
+            const float q = o.q(t[j]) * o.rsq;
+            if (!(q == 0.f))
+                kl += (double)q * ((((double)t[j] - o.M) * iT - lq) - (((double)z[j] - o.m) * iT - ls));
         }
     o.kl = wave_sum_d(kl);
-    const double qr = er * o.rsq;
-    if (!(qr == 0.0)) o.kl += qr * ((((double)rest - o.M) * iT - lq) - (logr - ls));
-    const double pr = r.m == NEG_INF ? 0.0 : exp(logr) * o.rs;
-    o.restdiff = r.m == NEG_INF ? 0.0 : (pr - qr) / (double)r.s;
-    o.empty = o.M == (double)NEG_INF;
+    const float qr = er * o.rsq;
+    if (!(qr == 0.f)) {
+        const double logr = r.m == NEG_INF ? (double)NEG_INF : ((double)r.m - o.m) * iT + log((double)r.s);
+        o.kl += (double)qr * ((((double)rest - o.M) * iT - lq) - (logr - ls));
+    }
+    o.restdiff = r.m == NEG_INF ? 0.f : (sr * o.rs - qr) / r.s;
+    o.empty = M == NEG_INF;
     return o;
-}
-__device__ __forceinline__ float entry_grad(const RowTerms& o, double g, float t, float z, double T) {
-    const double iT = 1.0 / T;
-    return (float)(g * (exp(((double)z - o.m) * iT) * o.rs - exp(((double)t - o.M) * iT) * o.rsq));
 }
 
 // ---------------------------------------------------------------- rows, a block each
@@ -287,21 +337,23 @@ template <typename T>
 __device__ __forceinline__ MaxSum row_rest(const DistillArgs& a, const RowSpan<T>& sp,
                                            const uint32_t* bits) {
     constexpr int N = RowVec<T>::N;
-    MaxSum acc{NEG_INF, 0.f};
+    RunSum acc;
     const float c = a.c;
     sp.template scan<4>(threadIdx.x, blockDim.x, [&](int slot, int i0, const Pack<T, N>& v, int cnt) {
         const uint32_t w = (bits[slot * N >> 5] >> (slot * N & 31)) & ((1u << N) - 1);
-        if (__builtin_expect(w == 0, 1)) {
-            acc.add(v, N, c);
-        } else {
-            Pack<T, N> u = v;
+        float x[N];
 #pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (w >> e & 1) u.set(e, NEG_INF);
-            acc.add(u, N, c);
+        for (int e = 0; e < N; ++e) x[e] = v.get(e);
+        if (__builtin_expect(w != 0, 0)) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = w >> e & 1 ? NEG_INF : x[e];
         }
+        float mx = x[0];
+#pragma unroll
+        for (int e = 1; e < N; ++e) mx = fmaxf(mx, x[e]);
+        acc.add(x, N, mx, c);
     });
-    return acc;
+    return acc.done(c);
 }
 
 template <typename T, bool ALIGNED>
@@ -310,29 +362,41 @@ __device__ __forceinline__ void row_grad(const DistillArgs& a, int64_t r, const 
     constexpr int N = RowVec<T>::N;
     T* d = static_cast<T*>(a.dz) + (size_t)r * a.V;
     const float f = s.a, mr = s.mr, c = a.c;
+    auto put = [&](int i0, const Pack<T, N>& o, int cnt) {
+        if (ALIGNED && cnt == N) {
+            o.store(d + i0);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (e < cnt) d[i0 + e] = (T)o.get(e);
+        }
+    };
     if (f == 0.f || mr == NEG_INF) {  // (f NaN: written as such below)
-        sp.template scan<1>(threadIdx.x, blockDim.x, [&](int, int i0, const Pack<T, N>&, int cnt) {
-            for (int e = 0; e < cnt; ++e) d[i0 + e] = (T)0.f;
+        Pack<T, N> o;
+#pragma unroll
+        for (int e = 0; e < N; ++e) o.set(e, 0.f);
+        sp.template scan<1>(threadIdx.x, blockDim.x, [&](int, int i0, const Pack<T, N>&, int cnt) { put(i0, o, cnt); });
+    } else if (const float mc = mr * c; fabsf(mc) < EXP_SAFE) {
+        const float fc = f * exp2_raw(-fmaf(mr, c, -mc));  // (as RunSum::done)
+        sp.template scan_back<4>(threadIdx.x, blockDim.x, [&](int, int i0, const Pack<T, N>& v, int cnt) {
+            Pack<T, N> o;
+#pragma unroll
+            for (int e = 0; e < N; ++e) o.set(e, fc * exp2_raw(fmaf(v.get(e), c, -mc)));
+            put(i0, o, cnt);
         });
     } else {
-        sp.template scan<4>(threadIdx.x, blockDim.x, [&](int, int i0, const Pack<T, N>& v, int cnt) {
+        sp.template scan<1>(threadIdx.x, blockDim.x, [&](int, int i0, const Pack<T, N>& v, int cnt) {
             Pack<T, N> o;
 #pragma unroll
             for (int e = 0; e < N; ++e) o.set(e, f * exp2_raw((v.get(e) - mr) * c));
-            if (ALIGNED && cnt == N) {
-                o.store(d + i0);
-            } else {
-#pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (e < cnt) d[i0 + e] = (T)o.get(e);
-            }
+            put(i0, o, cnt);
         });
     }
     __syncthreads();  // the kept classes over what the scan wrote there
     if (s.o.empty || s.g == 0.0) return;
     for (int j = threadIdx.x; j < a.k; j += blockDim.x) {
         const int i = s.idx[j];
-        if (i >= sp.lo && i < sp.hi) d[i] = (T)entry_grad(s.o, s.g, s.t[j], s.z[j], a.T);
+        if (i >= sp.lo && i < sp.hi) d[i] = (T)s.o.grad(s.g, s.t[j], s.z[j]);
     }
 }
 
@@ -350,7 +414,7 @@ __device__ __forceinline__ void row_finish(const DistillArgs& a, int64_t r, MaxS
             if (first && a.row_out) a.row_out[r] = (float)l;
             const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
             s.g = none ? 0.0 : a.coef * a.T * (double)w * go;
-            s.a = none ? 0.f : (float)(s.g * o.restdiff);
+            s.a = none ? 0.f : (float)(s.g * (double)o.restdiff);
             s.mr = rest.m;
             s.o = o;
             s.o.empty = none;
@@ -359,15 +423,15 @@ __device__ __forceinline__ void row_finish(const DistillArgs& a, int64_t r, MaxS
     __syncthreads();
 }
 
-template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(512) distill_row_kernel(DistillArgs a) {
+template <typename T, bool ALIGNED, int NT>
+__global__ void __launch_bounds__(NT) distill_row_kernel(DistillArgs a) {
     extern __shared__ uint32_t bits[];
     __shared__ RowShared s;
     if (distill_skip(a)) return;
     const int64_t r = blockIdx.x;
     const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, 0, a.V);
     row_entries<T>(a, r, sp, s, bits);
-    const MaxSum rest = block_maxsum(row_rest<T>(a, sp, bits), a.c, s.ms);
+    const MaxSum rest = block_maxsum(row_rest(a, sp, bits), a.c, s.ms);
     row_finish(a, r, rest, true, s);
     if (a.dz) row_grad<T, ALIGNED>(a, r, sp, s);
 }
@@ -384,7 +448,7 @@ __global__ void __launch_bounds__(256) distill_part_kernel(DistillArgs a, int sp
     const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, lo < a.V ? lo : a.V,
                         lo + chunk < a.V ? lo + chunk : a.V);
     row_entries<T>(a, r, sp, s, bits);
-    const MaxSum rest = block_maxsum(row_rest<T>(a, sp, bits), a.c, s.ms);
+    const MaxSum rest = block_maxsum(row_rest(a, sp, bits), a.c, s.ms);
     if (threadIdx.x == 0) {
         part[2 * blockIdx.x] = rest.m;
         part[2 * blockIdx.x + 1] = rest.s;
@@ -456,12 +520,13 @@ __device__ __forceinline__ double distill_wave_row(const DistillArgs& a, int64_t
         wave_sync();
     }
     const float w = a.weight ? a.weight[r] : 1.f;
-    MaxSum rest{NEG_INF, 0.f};
+    RunSum acc;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int x = lane + 64 * i;
-        if (x < a.V && !(s.bits[x >> 5] >> (x & 31) & 1)) rest.add1(v[i], a.c);
+        if (x < a.V && !(s.bits[x >> 5] >> (x & 31) & 1)) acc.add1(v[i], a.c);
     }
+    MaxSum rest = acc.done(a.c);
     rest.wave(a.c);
     const float tr = a.rest ? a.rest[r] : NEG_INF;
     const RowTerms o = row_terms(s.idx, s.t, s.z, a.k, tr, rest, a.T);
@@ -471,7 +536,7 @@ __device__ __forceinline__ double distill_wave_row(const DistillArgs& a, int64_t
         T* d = static_cast<T*>(a.dz) + (size_t)r * a.V;
         const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
         const double g = none ? 0.0 : a.coef * a.T * (double)w * go;
-        const float f = none || rest.m == NEG_INF ? 0.f : (float)(g * o.restdiff);
+        const float f = none || rest.m == NEG_INF ? 0.f : (float)(g * (double)o.restdiff);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int x = lane + 64 * i;
@@ -480,7 +545,7 @@ __device__ __forceinline__ double distill_wave_row(const DistillArgs& a, int64_t
         }
         for (int j = lane; j < a.k; j += 64)
             if (s.idx[j] >= 0)
-                d[s.idx[j]] = (T)(none ? 0.f : entry_grad(o, g, s.t[j], s.z[j], a.T));
+                d[s.idx[j]] = (T)(none ? 0.f : o.grad(g, s.t[j], s.z[j]));
     }
     wave_sync();  // the next row reuses the LDS
     return l;
@@ -547,15 +612,17 @@ template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(
             M = fmaxf(M, distill_value(a, rec + (size_t)j * a.inner));
             m = fmaxf(m, (float)z[(size_t)i * a.inner]);
         }
-        MaxSum rs{NEG_INF, 0.f};
+        RunSum acc;
         for (int i0 = 0; i0 < a.V; i0 += 32) {
             const uint32_t b = mine[256 * (i0 >> 5)];
             const int top = a.V - i0 < 32 ? a.V - i0 : 32;
             for (int e = 0; e < top; ++e) {
                 const float v = (float)z[(size_t)(i0 + e) * a.inner];
-                if (!(b >> e & 1)) rs.add1(v, a.c);
+                if (!(b >> e & 1)) acc.add1(v, a.c);
             }
         }
+        const MaxSum rs = acc.done(a.c);
+        const bool has = rs.m != NEG_INF;
         m = fmaxf(m, rs.m);
         // the k + 1 terms; the marks are cleared as entries are met, so a second pass over the
         // entries again takes each index once
@@ -578,7 +645,6 @@ template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(
         });
         const float er = rest == NEG_INF ? 0.f : expf((rest - M) * iT);
         const double iTd = 1.0 / a.T;
-        const bool has = rs.m != NEG_INF;
         const double logr = has ? ((double)rs.m - (double)m) * iTd + log((double)rs.s) : (double)NEG_INF;
         const float er_s = has ? rs.s * expf((rs.m - m) * iT) : rs.s;
         sq += er;
@@ -661,22 +727,24 @@ __device__ __forceinline__ float rest_logit(MaxSum r, float T) {
     return r.m == NEG_INF ? NEG_INF + r.s : (float)((double)r.m + (double)T * log((double)r.s));
 }
 
-constexpr int TK_CAP = 2048;   // candidates a block can hold
-constexpr int TK_RANK = 512;   // candidates up to here are ranked by counting
-struct TopShared {
-    uint64_t cand[TK_CAP];
-    float mx[512];
-    float ms[32];
+constexpr int TK_NEAR = 512;  // values at or above the last bound that are ranked at most
+// CAP: vectors set aside at most
+template <int CAP> struct TopShared {
+    uint4 raw[CAP];
+    uint32_t key[CAP], idx[CAP];  // the maximum's key; first index
+    uint8_t cnt[CAP];             // values of the vector
+    uint64_t near[TK_NEAR], sum[8];
+    float mx[512], ms[32];
     uint32_t hist[256];
-    int n, eq[9];
+    int n, nn, eq[9];
     uint32_t tau;
 };
 
 // Exact selection by key digits, for rows the threshold does not thin out (many equal values,
 // masked rows, NaN): the k-th key by four histograms, then the larger ones and the first of
-// the equal ones in index order.  Leaves the k candidates in s.cand; returns the rest's sums.
-template <typename T>
-__device__ MaxSum top_exact(const TopArgs& a, const RowSpan<T>& sp, TopShared& s) {
+// the equal ones in index order.  Leaves the k entries in s.near; returns the rest's sums.
+template <typename T, typename S>
+__device__ MaxSum top_exact(const TopArgs& a, const RowSpan<T>& sp, S& s) {
     constexpr int N = RowVec<T>::N;
     const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63, w = tid / 64, nw = nt / 64;
     uint32_t prefix = 0;
@@ -714,9 +782,9 @@ __device__ MaxSum top_exact(const TopArgs& a, const RowSpan<T>& sp, TopShared& s
         __syncthreads();
     }
     // prefix: the k-th key; `need` of the values equal to it belong to the record
-    if (tid == 0) s.n = 0;
+    if (tid == 0) s.nn = 0;
     __syncthreads();
-    MaxSum acc{NEG_INF, 0.f};
+    RunSum acc;
     int taken = 0;
     const int lo = sp.lo, hi = sp.hi;
     for (int base = lo; base < hi; base += nt) {
@@ -739,146 +807,236 @@ __device__ MaxSum top_exact(const TopArgs& a, const RowSpan<T>& sp, TopShared& s
             __syncthreads();
         }
         if (take) {
-            const int at = atomicAdd(&s.n, 1);  // (the order of s.cand does not matter)
-            s.cand[at] = order_pair(key, i);
+            const int at = atomicAdd(&s.nn, 1);  // (their order does not matter)
+            s.near[at] = order_pair(key, i);
         } else if (i < hi) {
             acc.add1((float)sp.z[i], a.c);
         }
     }
     __syncthreads();
-    return acc;
+    return acc.done(a.c);
 }
 
-template <typename T> __global__ void __launch_bounds__(512) top_row_kernel(TopArgs a) {
-    constexpr int N = RowVec<T>::N;
-    __shared__ TopShared s;
-    const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 63;
+// one wave: the upper 16 bits of the k-th largest of n <= 64 * R keys (key(i): the i-th), bit
+// by bit, counting with ballots (shuffles would cost several times the comparisons)
+template <int R, typename F> __device__ __forceinline__ uint32_t kth_prefix_of(int n, int k, F key) {
+    const int lane = threadIdx.x & 63;
+    uint32_t v[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) v[i] = lane + 64 * i < n ? key(lane + 64 * i) >> 16 : 0u;
+    uint32_t t = 0;
+    for (int b = 15; b >= 0; --b) {
+        const uint32_t up = t | 1u << b;
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) c += __popcll(__ballot(v[i] >= up));
+        if (c >= k) t = up;
+    }
+    return t;
+}
+template <typename F> __device__ __forceinline__ uint32_t kth_prefix(int n, int k, F key) {
+    if (n <= 256) return kth_prefix_of<4>(n, k, key);
+    if (n <= 512) return kth_prefix_of<8>(n, k, key);
+    if (n <= 1024) return kth_prefix_of<16>(n, k, key);
+    return kth_prefix_of<32>(n, k, key);
+}
+// that prefix as a value that bounds the k-th from below
+__device__ __forceinline__ float prefix_value(uint32_t t) {
+    t <<= 16;
+    // (keys below that of -inf belong to no value; a NaN's cannot be a bound)
+    return t <= 0x007fffffu ? NEG_INF : t >= 0xff800000u ? __builtin_inff() : key_value(t);
+}
+
+// A row is read once, in segments: the first quarter, up to the half, the rest.  A vector
+// whose maximum reaches a lower bound tau of the k-th largest value is set aside as loaded; the
+// others go into the rest's sums at once.  tau comes from the threads' maxima over the first
+// quarter (which is read a second time, from the caches) and rises to the k-th maximum of
+// what is set aside before each further segment, which so adds about k vectors.  At the end
+// the values of the vectors set aside are told apart: those near the k-th are ranked by
+// counting, the others join the rest.  What bounds it is the instructions: setting single
+// values aside took 196 us for 2048 x 131072 bf16 (22 vector instructions a value), and so did
+// two readings of whole rows; rows held in registers 299 (a block a CU).
+template <typename T, int NT, int CAP> __global__ void __launch_bounds__(NT, 8) top_row_kernel(TopArgs a) {
+    constexpr int N = RowVec<T>::N, U = 4;
+    __shared__ TopShared<CAP> s;
+    constexpr int nt = NT;
+    const int tid = threadIdx.x, lane = tid & 63;
     const int64_t r = blockIdx.x;
     const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, 0, a.V);
+    const T* const body = sp.z + sp.head;
     const float c = a.c;
-    // a lower bound of the k-th largest value: the k-th largest of the threads' maxima, to
-    // the upper 16 bits of its key; -inf where everything fits the buffer
     float tau = NEG_INF;
-    if (a.V > TK_RANK) {
-        float mx = NEG_INF;
-        sp.template scan<4>(tid, nt, [&](int, int, const Pack<T, N>& v, int) {
-            float m = v.get(0);
-#pragma unroll
-            for (int e = 1; e < N; ++e) m = fmaxf(m, v.get(e));
-            mx = fmaxf(mx, m);
-        });
-        s.mx[tid] = mx;
-        __syncthreads();
-        if (tid < 64) {
-            uint32_t key[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int x = lane + 64 * i;
-                key[i] = x < nt ? order_key(s.mx[x]) >> 16 : 0u;
-            }
-            uint32_t t = 0;
-            for (int b = 15; b >= 0; --b) {
-                const uint32_t up = t | 1u << b;
-                int n = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) n += __popcll(__ballot(key[i] >= up));
-                if (n >= a.k) t = up;
-            }
-            if (lane == 0) s.tau = t << 16;
-        }
-        __syncthreads();
-        const uint32_t t = s.tau;
-        // (keys below that of -inf belong to no value; a NaN's cannot be a bound)
-        tau = t <= 0x007fffffu ? NEG_INF : t >= 0xff800000u ? __builtin_inff() : key_value(t);
-    }
-    if (tid == 0) s.n = 0;
-    __syncthreads();
-    MaxSum acc{NEG_INF, 0.f};
-    sp.template scan<4>(tid, nt, [&](int, int i0, const Pack<T, N>& v, int cnt) {
+    RunSum acc;
+    auto top_of = [](const Pack<T, N>& v) {
         float m = v.get(0);
 #pragma unroll
         for (int e = 1; e < N; ++e) m = fmaxf(m, v.get(e));
-        if (m < tau) {
-            if (m > acc.m) {
-                acc.s *= exp2_raw((acc.m - m) * c);
-                acc.m = m;
+        return m;
+    };
+    auto eat = [&](int i0, const Pack<T, N>& v, int cnt) {
+        float x[N], mx = top_of(v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = v.get(e);
+        if (__builtin_expect(!(mx < tau), 0)) {
+            const int at = atomicAdd(&s.n, 1);
+            if (at < CAP) {
+                s.raw[at] = v.raw;
+                s.key[at] = order_key(mx);
+                s.idx[at] = i0;
+                s.cnt[at] = (uint8_t)cnt;
             }
-            float t = 0.f;
-            if (acc.m != NEG_INF)
-                for (int e = 0; e < N; ++e) t += exp2_raw((v.get(e) - acc.m) * c);
-            else
-                for (int e = 0; e < N; ++e) t += v.get(e) == NEG_INF ? 0.f : v.get(e);
-            acc.s += t;
-        } else {
-            for (int e = 0; e < cnt; ++e) {
-                const float x = v.get(e);
-                if (x < tau) {
-                    acc.add1(x, c);
-                } else {
-                    const int at = atomicAdd(&s.n, 1);
-                    if (at < TK_CAP) s.cand[at] = order_pair(order_key(x), i0 + e);
-                }
+            mx = NEG_INF;
+#pragma unroll
+            for (int e = 0; e < N; ++e) x[e] = NEG_INF;
+        }
+        acc.add(x, N, mx, c);
+    };
+    // tiles of nt vectors; the row's ends belong to the first segment
+    const int tiles = (sp.nv + nt - 1) / nt;
+    int end = tiles;
+    if (a.V > TK_NEAR) {
+        end = (tiles + 3) / 4;
+        float mx = NEG_INF;
+        for (int t = 0; t < end; ++t) {
+            const int i = t * nt + tid;
+            if (i < sp.nv) {
+                Pack<T, N> v;
+                v.load(body + (size_t)i * N);
+                mx = fmaxf(mx, top_of(v));
             }
         }
-    });
+        sp.ends(tid, nt, [&](int, int, const Pack<T, N>& v, int) { mx = fmaxf(mx, top_of(v)); });
+        s.mx[tid] = mx;
+        __syncthreads();
+        if (tid < 64) {
+            const uint32_t t = kth_prefix(nt, a.k, [&](int i) { return order_key(s.mx[i]); });
+            if (lane == 0) s.tau = t;
+        }
+    }
+    if (tid == 0) s.n = s.nn = 0;
     __syncthreads();
-    int n = s.n;
-    MaxSum rest = block_maxsum(acc, c, s.ms);
-    if (n > TK_CAP || rest.s != rest.s) {
+    if (a.V > TK_NEAR) tau = prefix_value(s.tau);
+    sp.ends(tid, nt, [&](int, int i0, const Pack<T, N>& v, int cnt) { eat(i0, v, cnt); });
+    int n = 0;
+    for (int t = 0;;) {
+        for (; t + U <= end; t += U) {
+            Pack<T, N> v[U];
+            const int i = t * nt + tid;
+            if (i + (U - 1) * nt < sp.nv) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) v[u].load(body + (size_t)(i + u * nt) * N);
+#pragma unroll
+                for (int u = 0; u < U; ++u) eat(sp.head + (i + u * nt) * N, v[u], N);
+            } else {
+                for (int u = 0; u < U; ++u)
+                    if (i + u * nt < sp.nv) {
+                        v[0].load(body + (size_t)(i + u * nt) * N);
+                        eat(sp.head + (i + u * nt) * N, v[0], N);
+                    }
+            }
+        }
+        for (; t < end; ++t) {
+            const int i = t * nt + tid;
+            if (i < sp.nv) {
+                Pack<T, N> v;
+                v.load(body + (size_t)i * N);
+                eat(sp.head + i * N, v, N);
+            }
+        }
+        __syncthreads();
+        n = s.n;
+        if (end >= tiles || n > CAP) break;
+        if (n >= a.k) {
+            if (tid < 64) {
+                const uint32_t p = kth_prefix(n, a.k, [&](int i) { return s.key[i]; });
+                if (lane == 0) s.tau = p;
+            }
+            __syncthreads();
+            tau = fmaxf(tau, prefix_value(s.tau));
+        }
+        end = 2 * end < tiles ? 2 * end : tiles;
+    }
+    MaxSum rest = block_maxsum(acc.done(c), c, s.ms);
+    // the values of the vectors set aside: value e of vector i is f(pair)
+    auto each = [&](auto f) {
+        for (int j = tid; j < n * N; j += nt) {
+            const int i = j / N, e = j % N;
+            if (e < (int)s.cnt[i]) {
+                const uint32_t w = reinterpret_cast<const uint32_t*>(&s.raw[i])[e * (int)sizeof(T) / 4];
+                const float v = sizeof(T) == 4 ? __uint_as_float(w)
+                                               : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+                f(order_pair(order_key(v), (int)s.idx[i] + e));
+            }
+        }
+    };
+    bool exact = n > CAP || rest.s != rest.s;  // too much near the top, or a NaN below it
+    if (!exact) {
+        uint32_t low = 0;
+        if (n > 64) {
+            if (tid < 64) {
+                const uint32_t p = kth_prefix(n, a.k, [&](int i) { return s.key[i]; });
+                if (lane == 0) s.tau = p;
+            }
+            __syncthreads();
+            low = n >= a.k ? s.tau << 16 : 0u;
+        }
+        each([&](uint64_t p) {
+            if ((uint32_t)(p >> 32) >= low) {
+                const int at = atomicAdd(&s.nn, 1);
+                if (at < TK_NEAR) s.near[at] = p;
+            }
+        });
+        __syncthreads();
+        exact = s.nn > TK_NEAR;
+    }
+    if (exact) {
         __syncthreads();
         rest = block_maxsum(top_exact<T>(a, sp, s), c, s.ms);
-        n = a.k;
     }
-    // rank the candidates; the first k are the record, the others join the rest
-    if (n > TK_RANK) {
-        int m = 1024;
-        while (m < n) m <<= 1;
-        for (int i = n + tid; i < m; i += nt) s.cand[i] = 0;
-        for (int len = 2; len <= m; len <<= 1)
-            for (int st = len >> 1; st > 0; st >>= 1) {
-                __syncthreads();
-                for (int i = tid; i < m / 2; i += nt) {
-                    const int x = (i / st) * 2 * st + i % st, y = x + st;
-                    const uint64_t p = s.cand[x], q = s.cand[y];
-                    if ((p < q) == ((x & len) == 0)) {
-                        s.cand[x] = q;
-                        s.cand[y] = p;
-                    }
-                }
-            }
-        __syncthreads();
-    }
-    const int per = n > TK_RANK ? 1 : (n + nt - 1) / nt;
-    uint64_t mine[4];
-    int rank[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int i = tid + q * nt;
-        rank[q] = -1;
-        if (n <= TK_RANK && q < per && i < n) {
-            mine[q] = s.cand[i];
-            int b = 0;
-            for (int j = 0; j < n; ++j) b += s.cand[j] > mine[q];
-            rank[q] = b;
-        }
-    }
-    __syncthreads();
-    if (n <= TK_RANK) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            if (rank[q] >= 0) s.cand[rank[q]] = mine[q];
-        __syncthreads();
-    }
+    const int nn = s.nn;
     T* val = static_cast<T*>(a.values) + (size_t)r * a.k;
     int64_t* idx = a.indices + (size_t)r * a.k;
-    for (int i = tid; i < a.k; i += nt) {
-        val[i] = (T)key_value((uint32_t)(s.cand[i] >> 32));
-        idx[i] = (int64_t)(uint32_t)~(uint32_t)s.cand[i];
+    for (int i = tid; i < nn; i += nt) {
+        const uint64_t p = s.near[i];
+        int b = 0;
+        for (int j = 0; j < nn; ++j) b += s.near[j] > p;
+        if (b < a.k) {
+            val[b] = (T)key_value((uint32_t)(p >> 32));
+            idx[b] = (int64_t)(uint32_t)~(uint32_t)p;
+        }
+        if (b == a.k - 1) s.sum[0] = p;
     }
-    MaxSum more{NEG_INF, 0.f};
-    for (int i = a.k + tid; i < n; i += nt) more.add1(key_value((uint32_t)(s.cand[i] >> 32)), c);
-    more = block_maxsum(more, c, s.ms);
-    rest.merge(more.m, more.s, c);
+    __syncthreads();
+    if (!exact) {
+        // what is below the k-th joins the rest.  The vectors' order is the atomics', so their
+        // exponentials are added as integers, 2^-40 of the largest
+        const uint64_t edge = s.sum[0];
+        float em = NEG_INF;
+        int bad = 0;
+        each([&](uint64_t p) {
+            if (p < edge) {
+                const float v = key_value((uint32_t)(p >> 32));
+                em = fmaxf(em, v);
+                bad |= v != v;
+            }
+        });
+        bad = __syncthreads_or(bad);
+        const MaxSum e = block_maxsum(MaxSum{em, 0.f}, c, s.ms);
+        uint64_t add = 0;
+        if (e.m != NEG_INF && e.m != __builtin_inff())
+            each([&](uint64_t p) {
+                if (p < edge)
+                    add += (uint64_t)((double)exp2_raw((key_value((uint32_t)(p >> 32)) - e.m) * c) * 0x1p40 + 0.5);
+            });
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) add += __shfl_xor((unsigned long long)add, o, 64);
+        if (lane == 0) s.sum[tid / 64] = add;
+        __syncthreads();
+        add = 0;
+        for (int i = 0; i < nt / 64; ++i) add += s.sum[i];
+        rest.merge(e.m, e.m == __builtin_inff() ? 1.f : (float)((double)add * 0x1p-40), c);
+        if (bad) rest.s = __builtin_nanf("");
+    }
     if (tid == 0) a.rest[r] = rest_logit(rest, a.T);
 }
 
@@ -895,8 +1053,9 @@ template <typename T> __global__ void __launch_bounds__(256) top_wave_kernel(Top
         rank += kj > key || (kj == key && j < lane);
     }
     const bool kept = lane < a.V && rank < a.k;
-    MaxSum rest{NEG_INF, 0.f};
-    if (!kept && lane < a.V) rest.add1(v, a.c);
+    RunSum acc;
+    if (!kept && lane < a.V) acc.add1(v, a.c);
+    MaxSum rest = acc.done(a.c);
     rest.wave(a.c);
     if (kept) {
         static_cast<T*>(a.values)[(size_t)r * a.k + rank] = (T)key_value(key);
@@ -920,7 +1079,7 @@ template <typename T, int VR> __global__ void __launch_bounds__(256) top_map_ker
         for (int i = 0; i < VR; ++i) key[i] = i < a.V ? order_key((float)z[(size_t)i * a.inner]) : 0u;
     }
     uint64_t last = ~0ull;
-    MaxSum rest{NEG_INF, 0.f};
+    RunSum rest;
     for (int j = 0; j <= a.k; ++j) {
         uint64_t best = 0;
         auto see = [&](uint32_t kv, int i) {
@@ -943,7 +1102,7 @@ template <typename T, int VR> __global__ void __launch_bounds__(256) top_map_ker
             idx[(size_t)j * a.inner] = (int64_t)(uint32_t)~(uint32_t)best;
         }
     }
-    a.rest[r] = rest_logit(rest, a.T);
+    a.rest[r] = rest_logit(rest.done(a.c), a.T);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1022,9 +1181,11 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
     } else if (V <= 64) {
         TOP_GO((top_wave_kernel<float>), (top_wave_kernel<__bf16>), cdiv(N, 4), 256);
     } else {
-        // twice as many maxima as entries keep the candidates near k
-        const int nt = k <= 64 && V <= 4096 ? 128 : k <= 128 && V <= 16384 ? 256 : 512;
-        TOP_GO((top_row_kernel<float>), (top_row_kernel<__bf16>), N, nt);
+        // twice as many maxima as entries keep the first bound near the k-th; about 3.2 k vectors
+        // are set aside (all, up to 512 classes)
+        if (k <= 64 && V <= 4096) TOP_GO((top_row_kernel<float, 128, 256>), (top_row_kernel<__bf16, 128, 256>), N, 128);
+        else if (k <= 128 && V <= 16384) TOP_GO((top_row_kernel<float, 256, 512>), (top_row_kernel<__bf16, 256, 512>), N, 256);
+        else TOP_GO((top_row_kernel<float, 512, 1024>), (top_row_kernel<__bf16, 512, 1024>), N, 512);
     }
 #undef TOP_GO
     return check_launch("top_logits");
@@ -1095,11 +1256,18 @@ static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, bool
         const Split sp = row_split(rows, a.V);
         auto lds = [&](int span) { return (unsigned)(((span + 3 * RowVec<T>::N + 31) / 32) * 4); };
         if (sp.n == 1) {
-            const int nt = a.V <= 8192 ? 256 : 512;
-            if (al)
-                hipLaunchKernelGGL((distill_row_kernel<T, true>), dim3((unsigned)rows), dim3(nt), lds(a.V), s, a);
-            else
-                hipLaunchKernelGGL((distill_row_kernel<T, false>), dim3((unsigned)rows), dim3(nt), lds(a.V), s, a);
+#define DISTILL_ROW(AL, NT) \
+    hipLaunchKernelGGL((distill_row_kernel<T, AL, NT>), dim3((unsigned)rows), dim3(NT), lds(a.V), s, a)
+            // (4096 x 32768 bf16 with its gradient: 135 us at 512 threads, 143 at 256, 154 at 1024;
+            // rows held in registers instead of read again: 173)
+            if (a.V <= 8192) {
+                if (al) DISTILL_ROW(true, 256);
+                else DISTILL_ROW(false, 256);
+            } else {
+                if (al) DISTILL_ROW(true, 512);
+                else DISTILL_ROW(false, 512);
+            }
+#undef DISTILL_ROW
         } else {
             float* part = reinterpret_cast<float*>(static_cast<double*>(ws) + (backward ? 0 : rows));
             const unsigned g = (unsigned)(rows * sp.n);

@@ -34,10 +34,18 @@ __device__ __forceinline__ float gn_act_bwd(float dy, float p, int act) {
 // ---------------------------------------------------------------- two passes
 // Block (b, chunk, column block): cb vector columns x `rows` pixel rows of threads, each
 // thread keeps its V channels and steps over the chunk's pixels.
+constexpr int GN_NT = 512;  // threads of a block
+// pixels a thread has in flight: 4 of x, 2 of x and dy (8 and 4 time the same; 512 threads
+// beat 256 by 7 % and 1024 by 3 % over forward and backward of 16 x 256^2 x 64 fp32)
+constexpr int GN_U = 4, GN_UB = 2;
+constexpr int GN_FG = 256;       // groups a block folds itself at most
+constexpr int GN_FOLD = 1 << 14;  // partials of a sample that a block folds itself at most
+
 struct GnGeom {
     int64_t P, ppc;  // pixels of a sample, pixels per chunk
     int C, G, cpg;
     int cb, rows, ncol, nchunk;
+    int fold;  // the second pass merges the partials itself (no merge launch)
 };
 struct GnPos {
     int b, chunk, c, row;  // c: first channel of the thread's vector
@@ -57,12 +65,16 @@ template <int V> __device__ __forceinline__ GnPos gn_pos(const GnGeom& g, unsign
     r.p1 = r.p0 + g.ppc < g.P ? r.p0 + g.ppc : g.P;
     return r;
 }
+__device__ __forceinline__ double gn_count(const GnGeom& g, int chunk) {
+    const int64_t left = g.P - (int64_t)chunk * g.ppc;
+    return (double)(left < g.ppc ? left : g.ppc);
+}
 
 // per-channel (mean, M2) of a chunk -> part[b][chunk][2][C]
 template <typename T, int V>
-__global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, GnGeom g, float* part) {
-    constexpr int U = 8;
-    __shared__ float s_mean[256 * V], s_m2[256 * V], s_n[256];
+__global__ void __launch_bounds__(GN_NT) gn_stats_kernel(const T* x, GnGeom g, float* part) {
+    constexpr int U = GN_U;
+    __shared__ float s_mean[GN_NT * V], s_m2[GN_NT * V], s_n[GN_NT];
     const GnPos q = gn_pos<V>(g, blockIdx.x);
     float n = 0.f, mean[V], m2[V];
 #pragma unroll
@@ -110,8 +122,8 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, GnGeom g, flo
     const int t = threadIdx.x;
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        s_mean[e * 256 + t] = mean[e];
-        s_m2[e * 256 + t] = m2[e];
+        s_mean[e * GN_NT + t] = mean[e];
+        s_m2[e * GN_NT + t] = m2[e];
     }
     s_n[t] = n;
     int top = 1;
@@ -125,11 +137,11 @@ __global__ void __launch_bounds__(256) gn_stats_kernel(const T* x, GnGeom g, flo
                 const float rn = 1.f / (n + nb);
 #pragma unroll
                 for (int e = 0; e < V; ++e) {
-                    const float dm = s_mean[e * 256 + o] - mean[e];
+                    const float dm = s_mean[e * GN_NT + o] - mean[e];
                     mean[e] = fmaf(dm, nb * rn, mean[e]);
-                    m2[e] += fmaf(dm * dm, n * nb * rn, s_m2[e * 256 + o]);
-                    s_mean[e * 256 + t] = mean[e];
-                    s_m2[e * 256 + t] = m2[e];
+                    m2[e] += fmaf(dm * dm, n * nb * rn, s_m2[e * GN_NT + o]);
+                    s_mean[e * GN_NT + t] = mean[e];
+                    s_m2[e * GN_NT + t] = m2[e];
                 }
                 n += nb;
                 s_n[t] = n;
@@ -156,81 +168,173 @@ __global__ void __launch_bounds__(256) gn_merge_kernel(const float* part, GnGeom
     const float* pb = part + (size_t)b * g.nchunk * 2 * g.C + gr * g.cpg;
     const int n = g.nchunk * g.cpg;
     const double cnt = (double)g.P * g.cpg;
-    double s = 0;
+    // about the first partial's mean: the squares cancel nothing
+    const double ref = pb[0];
+    double s = 0, q = 0;
+#pragma unroll 4
     for (int i = lane; i < n; i += 64) {
         const int ch = i / g.cpg, c = i % g.cpg;
-        const int64_t left = g.P - (int64_t)ch * g.ppc;
-        const double np = left < g.ppc ? left : g.ppc;
-        s += np * (double)pb[(size_t)ch * 2 * g.C + c];
-    }
-    const double mu = wave_sum_d(s) / cnt;
-    double q = 0;
-    for (int i = lane; i < n; i += 64) {
-        const int ch = i / g.cpg, c = i % g.cpg;
-        const int64_t left = g.P - (int64_t)ch * g.ppc;
-        const double np = left < g.ppc ? left : g.ppc;
-        const double d = (double)pb[(size_t)ch * 2 * g.C + c] - mu;
+        const double np = gn_count(g, ch), d = (double)pb[(size_t)ch * 2 * g.C + c] - ref;
+        s += np * d;
         q += (double)pb[((size_t)ch * 2 + 1) * g.C + c] + np * d * d;
     }
-    q = wave_sum_d(q);
+    s = wave_sum_d(s) / cnt;
+    q = wave_sum_d(q) / cnt - s * s;
     if (lane == 0) {
-        mean[id] = (float)mu;
-        rstd[id] = (float)(1.0 / sqrt(q / cnt + (double)eps));
+        mean[id] = (float)(ref + s);
+        rstd[id] = (float)(1.0 / sqrt((q > 0 ? q : q != q ? q : 0.0) + (double)eps));
+    }
+}
+
+// Group sums of two per-channel quantities: `each(c, first, step)` gives the caller's share of
+// channel c over the partials first, first + step, ... (fp32, a few dozen terms at most); L
+// lanes a group add the shares in fp64, in a fixed order.  Every thread of the block calls it;
+// the sums are in f->gs.  (Shares in fp64 cost every block of the second pass 10 us where
+// 1024 blocks merge 64 chunks of 128 channels.)
+struct GnFold {
+    float red[2][GN_NT];
+    double gs[2][GN_FG];
+};
+template <typename F>
+__device__ __forceinline__ void gn_fold(const GnGeom& g, GnFold* f, F each) {
+    const int t = threadIdx.x;
+    const int ct = g.C < GN_NT ? g.C : GN_NT, parts = GN_NT / ct;
+    for (int k = t; k < g.G; k += GN_NT) f->gs[0][k] = f->gs[1][k] = 0;
+    for (int c0 = 0; c0 < g.C; c0 += ct) {
+        const int cl = t % ct, pi = t / ct, c = c0 + cl;
+        float a = 0.f, b = 0.f;
+        if (pi < parts && c < g.C) each(c, pi, parts, a, b);
+        f->red[0][t] = a;
+        f->red[1][t] = b;
+        __syncthreads();
+        const int c1 = c0 + ct < g.C ? c0 + ct : g.C;
+        const int k0 = c0 / g.cpg, k1 = (c1 - 1) / g.cpg;
+        int L = 64;
+        while (L > 1 && (k1 - k0 + 1) * L > GN_NT) L >>= 1;
+        const int l = t & (L - 1);
+        for (int kb = k0; kb <= k1; kb += GN_NT / L) {
+            const int k = kb + t / L;
+            double x = 0, y = 0;
+            if (k <= k1) {
+                const int lo = (k * g.cpg > c0 ? k * g.cpg : c0) - c0;
+                const int wd = ((k + 1) * g.cpg < c1 ? (k + 1) * g.cpg : c1) - c0 - lo;
+                for (int j = l; j < wd * parts; j += L) {
+                    const int at = j / wd * ct + lo + j % wd;
+                    x += f->red[0][at];
+                    y += f->red[1][at];
+                }
+            }
+            for (int o = L >> 1; o > 0; o >>= 1) {
+                x += __shfl_xor(x, o, 64);
+                y += __shfl_xor(y, o, 64);
+            }
+            // (a group that spans tiles: one tile after the other, a barrier between)
+            if (l == 0 && k <= k1) {
+                f->gs[0][k] += x;
+                f->gs[1][k] += y;
+            }
+        }
+        __syncthreads();
     }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) gn_apply_kernel(const T* x, GnGeom g, const float* mean,
-                                                       const float* rstd, const float* gamma,
-                                                       const float* beta, int act, T* y) {
-    constexpr int U = 4;
-    const GnPos q = gn_pos<V>(g, blockIdx.x);
+__global__ void __launch_bounds__(GN_NT) gn_apply_kernel(const T* x, GnGeom g, const float* part,
+                                                         float eps, float* mean, float* rstd,
+                                                         const float* gamma, const float* beta,
+                                                         int act, T* y) {
+    constexpr int U = GN_U;
+    __shared__ GnFold fold;
+    GnFold* const f = &fold;
+    // the last block of the first pass first: its values are the likeliest still cached
+    const GnPos q = gn_pos<V>(g, gridDim.x - 1 - blockIdx.x);
+    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
+    const int64_t step = g.rows;
+    int64_t p = q.p0 + q.row;
+    Pack<T, V> v[U];
+    bool full = q.on && p + (U - 1) * step < q.p1;
+    if (full) {  // on their way while the statistics are merged
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u].load(x + base + (size_t)(p + u * step) * g.C);
+    }
+    if (g.fold) {
+        const float* pb = part + (size_t)q.b * g.nchunk * 2 * g.C;
+        gn_fold(g, f, [&](int c, int first, int step, float& s, float& v) {
+            // about the group's first mean: the squares cancel nothing
+            const float ref = pb[c / g.cpg * g.cpg];
+            const float whole = (float)g.ppc, last = (float)(g.P - (int64_t)(g.nchunk - 1) * g.ppc);
+#pragma unroll 8
+            for (int ch = first; ch < g.nchunk; ch += step) {
+                const float np = ch == g.nchunk - 1 ? last : whole;
+                const float d = pb[(size_t)ch * 2 * g.C + c] - ref;
+                s = fmaf(np, d, s);
+                v += fmaf(np * d, d, pb[((size_t)ch * 2 + 1) * g.C + c]);
+            }
+        });
+        const double cnt = (double)g.P * g.cpg;
+        for (int k = threadIdx.x; k < g.G; k += GN_NT) {
+            const double s = f->gs[0][k] / cnt, v = f->gs[1][k] / cnt - s * s;
+            const double m = (double)pb[k * g.cpg] + s;
+            const double r = 1.0 / sqrt((v > 0 ? v : v != v ? v : 0.0) + (double)eps);
+            f->gs[0][k] = m;
+            f->gs[1][k] = r;
+            if (q.chunk == 0) {
+                mean[(size_t)q.b * g.G + k] = (float)m;
+                rstd[(size_t)q.b * g.G + k] = (float)r;
+            }
+        }
+        __syncthreads();
+    }
     if (!q.on) return;
     float mu[V], a[V], h[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int gi = q.b * g.G + (q.c + e) / g.cpg;
-        mu[e] = mean[gi];
-        a[e] = rstd[gi] * (gamma ? gamma[q.c + e] : 1.f);
+        const int k = (q.c + e) / g.cpg;
+        mu[e] = g.fold ? (float)f->gs[0][k] : mean[(size_t)q.b * g.G + k];
+        a[e] = (g.fold ? (float)f->gs[1][k] : rstd[(size_t)q.b * g.G + k]) * (gamma ? gamma[q.c + e] : 1.f);
         h[e] = beta ? beta[q.c + e] : 0.f;
     }
-    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
-    const int64_t step = g.rows;
-    int64_t p = q.p0 + q.row;
-    for (; p + (U - 1) * step < q.p1; p += U * step) {
-        Pack<T, V> v[U];
+    auto one = [&](const Pack<T, V>& in, int64_t at) {
+        Pack<T, V> o;
 #pragma unroll
-        for (int u = 0; u < U; ++u) v[u].load(x + base + (size_t)(p + u * step) * g.C);
+        for (int e = 0; e < V; ++e) o.set(e, gn_act(fmaf(in.get(e) - mu[e], a[e], h[e]), act));
+        o.store(y + base + (size_t)at * g.C);
+    };
+    while (full) {
+        Pack<T, V> w[U];
+        const int64_t pn = p + U * step;
+        const bool next = pn + (U - 1) * step < q.p1;
+        if (next) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                o.set(e, gn_act(fmaf(v[u].get(e) - mu[e], a[e], h[e]), act));
-            o.store(y + base + (size_t)(p + u * step) * g.C);
+            for (int u = 0; u < U; ++u) w[u].load(x + base + (size_t)(pn + u * step) * g.C);
         }
+#pragma unroll
+        for (int u = 0; u < U; ++u) one(v[u], p + u * step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = w[u];
+        p = pn;
+        full = next;
     }
     for (; p < q.p1; p += step) {
-        Pack<T, V> v, o;
-        v.load(x + base + (size_t)p * g.C);
-#pragma unroll
-        for (int e = 0; e < V; ++e) o.set(e, gn_act(fmaf(v.get(e) - mu[e], a[e], h[e]), act));
-        o.store(y + base + (size_t)p * g.C);
+        v[0].load(x + base + (size_t)p * g.C);
+        one(v[0], p);
     }
 }
 
-// per-channel (sum dp, sum dp*xh, sum xh) of a chunk -> part[b][chunk][3][C]
-template <typename T, typename TD, int V>
-__global__ void __launch_bounds__(256) gn_bwd_reduce_kernel(const TD* dy, const T* x, GnGeom g,
-                                                            const float* mean, const float* rstd,
-                                                            const float* gamma, const float* beta,
-                                                            int act, float* part) {
-    constexpr int U = 4;
-    __shared__ float s_a[256 * V], s_b[256 * V], s_x[256 * V];
+// per-channel (sum dp, sum dp*xh[, sum xh]) of a chunk -> part[b][chunk][2 or 3][C]
+template <typename T, typename TD, int V, bool X>
+__global__ void __launch_bounds__(GN_NT) gn_bwd_reduce_kernel(const TD* dy, const T* x, GnGeom g,
+                                                              const float* mean, const float* rstd,
+                                                              const float* gamma, const float* beta,
+                                                              int act, float* part) {
+    constexpr int U = GN_UB, K = X ? 3 : 2;
+    __shared__ float sh[GN_NT * V];
     const GnPos q = gn_pos<V>(g, blockIdx.x);
-    float sa[V], sb[V], sx[V], mu[V], rs[V], w[V], h[V];
+    float sum[K][V], mu[V], rs[V], w[V], h[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e) sa[e] = sb[e] = sx[e] = 0.f;
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[k][e] = 0.f;
     if (q.on) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -248,9 +352,9 @@ __global__ void __launch_bounds__(256) gn_bwd_reduce_kernel(const TD* dy, const 
             for (int e = 0; e < V; ++e) {
                 const float xh = (v.get(e) - mu[e]) * rs[e];
                 const float dp = gn_act_bwd(d.get(e), fmaf(xh, w[e], h[e]), act);
-                sa[e] += dp;
-                sb[e] = fmaf(dp, xh, sb[e]);
-                sx[e] += xh;
+                sum[0][e] += dp;
+                sum[1][e] = fmaf(dp, xh, sum[1][e]);
+                if constexpr (X) sum[2][e] += xh;
             }
         };
         for (; p + (U - 1) * step < q.p1; p += U * step) {
@@ -273,39 +377,30 @@ __global__ void __launch_bounds__(256) gn_bwd_reduce_kernel(const TD* dy, const 
         }
     }
     const int t = threadIdx.x;
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        s_a[e * 256 + t] = sa[e];
-        s_b[e * 256 + t] = sb[e];
-        s_x[e * 256 + t] = sx[e];
-    }
     int top = 1;
     while (top < g.rows) top <<= 1;
-    for (int s = top >> 1; s > 0; s >>= 1) {
-        __syncthreads();
-        if (q.on && q.row < s && q.row + s < g.rows) {
-            const int o = t + s * g.cb;
+    float* o = part + ((size_t)(q.b * (int64_t)g.nchunk + q.chunk) * K) * g.C + q.c;
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                s_a[e * 256 + t] += s_a[e * 256 + o];
-                s_b[e * 256 + t] += s_b[e * 256 + o];
-                s_x[e * 256 + t] += s_x[e * 256 + o];
+    for (int k = 0; k < K; ++k) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) sh[e * GN_NT + t] = sum[k][e];
+        for (int s = top >> 1; s > 0; s >>= 1) {
+            __syncthreads();
+            if (q.on && q.row < s && q.row + s < g.rows) {
+#pragma unroll
+                for (int e = 0; e < V; ++e) sh[e * GN_NT + t] += sh[e * GN_NT + t + s * g.cb];
             }
         }
-    }
-    if (q.on && q.row == 0) {
-        float* o = part + ((size_t)(q.b * (int64_t)g.nchunk + q.chunk) * 3) * g.C + q.c;
+        if (q.on && q.row == 0) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            o[e] = s_a[e * 256 + t];
-            o[g.C + e] = s_b[e * 256 + t];
-            o[2 * g.C + e] = s_x[e * 256 + t];
+            for (int e = 0; e < V; ++e) o[k * g.C + e] = sh[e * GN_NT + t];
         }
     }
 }
 
-// block per (sample, group): the chunks' sums per channel -> tot[b][3][C], and the group's
-// s1, s2 -> sums[b][G][2]
+// block per (sample, group): the chunks' sums per channel (part with K = 3) -> tot[b][3][C],
+// and the group's s1, s2 -> sums[b][G][2]
 __global__ void __launch_bounds__(256) gn_bwd_merge_kernel(const float* part, GnGeom g,
                                                            const float* gamma, float* tot,
                                                            float* sums) {
@@ -319,13 +414,15 @@ __global__ void __launch_bounds__(256) gn_bwd_merge_kernel(const float* part, Gn
         const int c = gr * g.cpg + c0 + cl;
         const bool on = pi < parts && c0 + cl < g.cpg;
         double a = 0, bb = 0, xx = 0;
-        if (on)
+        if (on) {
+#pragma unroll 4
             for (int ch = pi; ch < g.nchunk; ch += parts) {
                 const float* pb = part + ((size_t)(b * (int64_t)g.nchunk + ch) * 3) * g.C + c;
                 a += pb[0];
                 bb += pb[g.C];
                 xx += pb[2 * g.C];
             }
+        }
         sh[0][t] = a;
         sh[1][t] = bb;
         sh[2][t] = xx;
@@ -364,9 +461,10 @@ __global__ void __launch_bounds__(256) gn_bwd_merge_kernel(const float* part, Gn
 
 // dgamma, dbeta and the sum of dx per channel (the gradient of a bias added to x), from the
 // samples' totals: sum_p dx = rstd * (gamma*A - P*s1 - s2*X) per sample, A = sum dp, X = sum xh
-__device__ void gn_param_grads(int c, int B, int64_t P, int C, int G, int cpg, const float* tot,
-                               const float* sums, const float* rstd, const float* gamma,
-                               float* dgamma, float* dbeta, float* dxsum) {
+__device__ __forceinline__ void gn_param_grads(int c, int B, int64_t P, int C, int G, int cpg,
+                                               const float* tot, const float* sums,
+                                               const float* rstd, const float* gamma,
+                                               float* dgamma, float* dbeta, float* dxsum) {
     double a = 0, bb = 0, d = 0;
     const int gr = c / cpg;
     const double w = gamma ? (double)gamma[c] : 1.0;
@@ -383,35 +481,93 @@ __device__ void gn_param_grads(int c, int B, int64_t P, int C, int G, int cpg, c
     if (dxsum) dxsum[c] = (float)d;
 }
 
-// dx; the blocks past `napply` sum the parameters' gradients over the samples
-template <typename T, typename TD, typename TO, int V>
-__global__ void __launch_bounds__(256) gn_bwd_apply_kernel(
-    const TD* dy, const T* x, GnGeom g, int B, unsigned napply, const float* mean,
-    const float* rstd, const float* gamma, const float* beta, int act, const float* tot,
-    const float* sums, TO* dx, float* dgamma, float* dbeta, float* dxsum) {
-    constexpr int U = 4;
-    if (blockIdx.x >= napply) {
-        const int c = (blockIdx.x - napply) * 256 + threadIdx.x;
-        if (c < g.C)
+// the parameters' gradients of 64 channels a block: over all the chunks' partials (fold), or
+// over the samples' totals
+__device__ __forceinline__ void gn_params(const GnGeom& g, int B, unsigned id, const float* part,
+                                          const float* tot, const float* sums, const float* rstd,
+                                          const float* gamma, float* dgamma, float* dbeta, float* dxsum) {
+    const int c = id * 64 + (threadIdx.x & 63), pi = threadIdx.x / 64;
+    if (!g.fold) {
+        if (c < g.C && pi == 0)
             gn_param_grads(c, B, g.P, g.C, g.G, g.cpg, tot, sums, rstd, gamma, dgamma, dbeta, dxsum);
         return;
     }
-    const GnPos q = gn_pos<V>(g, blockIdx.x);
+    __shared__ double red[2][GN_NT];
+    double a = 0, b = 0;
+    if (c < g.C) {
+#pragma unroll 8
+        for (int64_t k = pi; k < (int64_t)B * g.nchunk; k += GN_NT / 64) {
+            a += part[(size_t)k * 2 * g.C + c];
+            b += part[((size_t)k * 2 + 1) * g.C + c];
+        }
+    }
+    red[0][threadIdx.x] = a;
+    red[1][threadIdx.x] = b;
+    __syncthreads();
+    if (c < g.C && pi == 0) {
+        for (int k = 1; k < GN_NT / 64; ++k) {
+            a += red[0][threadIdx.x + 64 * k];
+            b += red[1][threadIdx.x + 64 * k];
+        }
+        if (dbeta) dbeta[c] = (float)a;
+        if (dgamma) dgamma[c] = (float)b;
+    }
+}
+
+// dx; the first `nparam` blocks sum the parameters' gradients, 64 channels each
+template <typename T, typename TD, typename TO, int V>
+__global__ void __launch_bounds__(GN_NT) gn_bwd_apply_kernel(
+    const TD* dy, const T* x, GnGeom g, int B, unsigned nparam, const float* mean, const float* rstd,
+    const float* gamma, const float* beta, int act, const float* part, const float* tot,
+    const float* sums, TO* dx, float* dgamma, float* dbeta, float* dxsum) {
+    constexpr int U = GN_UB;
+    __shared__ GnFold fold;
+    GnFold* const f = &fold;
+    if (blockIdx.x < nparam) {
+        gn_params(g, B, blockIdx.x, part, tot, sums, rstd, gamma, dgamma, dbeta, dxsum);
+        return;
+    }
+    const GnPos q = gn_pos<V>(g, gridDim.x - 1 - blockIdx.x);
+    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
+    const int64_t step = g.rows;
+    int64_t p = q.p0 + q.row;
+    Pack<T, V> v[U];
+    Pack<TD, V> d[U];
+    bool full = q.on && p + (U - 1) * step < q.p1;
+    if (full) {  // on their way while the sums are merged
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u].load(x + base + (size_t)(p + u * step) * g.C);
+            d[u].load(dy + base + (size_t)(p + u * step) * g.C);
+        }
+    }
+    if (g.fold) {
+        const float* pb = part + (size_t)q.b * g.nchunk * 2 * g.C;
+        gn_fold(g, f, [&](int c, int first, int step, float& s, float& t) {
+#pragma unroll 8
+            for (int ch = first; ch < g.nchunk; ch += step) {
+                s += pb[(size_t)ch * 2 * g.C + c];
+                t += pb[((size_t)ch * 2 + 1) * g.C + c];
+            }
+            const float w = gamma ? gamma[c] : 1.f;
+            s *= w;
+            t *= w;
+        });
+    }
     if (!q.on) return;
+    const double rcnt = 1.0 / ((double)g.P * g.cpg);
     float mu[V], rs[V], w[V], h[V], s1[V], s2[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int gi = q.b * g.G + (q.c + e) / g.cpg;
+        const int k = (q.c + e) / g.cpg, gi = q.b * g.G + k;
         mu[e] = mean[gi];
         rs[e] = rstd[gi];
         w[e] = gamma ? gamma[q.c + e] : 1.f;
         h[e] = beta ? beta[q.c + e] : 0.f;
-        s1[e] = sums[2 * gi];
-        s2[e] = sums[2 * gi + 1];
+        s1[e] = g.fold ? (float)(f->gs[0][k] * rcnt) : sums[2 * gi];
+        s2[e] = g.fold ? (float)(f->gs[1][k] * rcnt) : sums[2 * gi + 1];
     }
-    const size_t base = ((size_t)q.b * g.P) * g.C + q.c;
-    const int64_t step = g.rows;
-    auto one = [&](const Pack<T, V>& v, const Pack<TD, V>& d, size_t off) {
+    auto one = [&](const Pack<T, V>& v, const Pack<TD, V>& d, int64_t at) {
         Pack<TO, V> o;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
@@ -419,26 +575,34 @@ __global__ void __launch_bounds__(256) gn_bwd_apply_kernel(
             const float dp = gn_act_bwd(d.get(e), fmaf(xh, w[e], h[e]), act);
             o.set(e, rs[e] * fmaf(-xh, s2[e], fmaf(w[e], dp, -s1[e])));
         }
-        o.store(dx + off);
+        o.store(dx + base + (size_t)at * g.C);
     };
-    int64_t p = q.p0 + q.row;
-    for (; p + (U - 1) * step < q.p1; p += U * step) {
-        Pack<T, V> v[U];
-        Pack<TD, V> d[U];
+    while (full) {
+        Pack<T, V> vn[U];
+        Pack<TD, V> dn[U];
+        const int64_t pn = p + U * step;
+        const bool next = pn + (U - 1) * step < q.p1;
+        if (next) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            v[u].load(x + base + (size_t)(p + u * step) * g.C);
-            d[u].load(dy + base + (size_t)(p + u * step) * g.C);
+            for (int u = 0; u < U; ++u) {
+                vn[u].load(x + base + (size_t)(pn + u * step) * g.C);
+                dn[u].load(dy + base + (size_t)(pn + u * step) * g.C);
+            }
         }
 #pragma unroll
-        for (int u = 0; u < U; ++u) one(v[u], d[u], base + (size_t)(p + u * step) * g.C);
+        for (int u = 0; u < U; ++u) one(v[u], d[u], p + u * step);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u] = vn[u];
+            d[u] = dn[u];
+        }
+        p = pn;
+        full = next;
     }
     for (; p < q.p1; p += step) {
-        Pack<T, V> v;
-        Pack<TD, V> d;
-        v.load(x + base + (size_t)p * g.C);
-        d.load(dy + base + (size_t)p * g.C);
-        one(v, d, base + (size_t)p * g.C);
+        v[0].load(x + base + (size_t)p * g.C);
+        d[0].load(dy + base + (size_t)p * g.C);
+        one(v[0], d[0], p);
     }
 }
 
@@ -730,17 +894,24 @@ static GnGeom gn_geom(int B, int64_t P, int C, int G, int V) {
     g.G = G;
     g.cpg = C / G;
     const int cv = C / V;
-    g.ncol = (int)cdiv(cv, 256);
+    g.ncol = (int)cdiv(cv, GN_NT);
     g.cb = (int)cdiv(cv, g.ncol);
-    g.rows = 256 / g.cb;
-    // about 2048 blocks (8 per CU), no chunk below 8 pixels a thread, at most 512 chunks
-    int64_t want = cdiv(2048, (int64_t)B * g.ncol);
-    const int64_t most = cdiv(P, (int64_t)g.rows * 8);
+    g.rows = GN_NT / g.cb;
+    // about 1024 blocks (4 per CU), no chunk below 4 pixels a thread, at most 1024 chunks
+    int64_t want = cdiv(1024, (int64_t)B * g.ncol);
+    const int64_t most = cdiv(P, (int64_t)g.rows * 4);
     if (want > most) want = most;
-    if (want > 512) want = 512;
+    if (want > 1024) want = 1024;
     if (want < 1) want = 1;
+    // every block of the second pass merges a sample's partials again: at most 4096 of them,
+    // or down to 512 blocks (16 x 128^2 x 128 bf16 forward: 44 us at 32 chunks, 52 at 64;
+    // 16 x 256^2 x 64 fp32 forward and backward: 398 us at 1024 blocks, 426 at 512)
+    const int64_t light = 4096 / C > 1 ? 4096 / C : 1;
+    const int64_t fill = cdiv(512, (int64_t)B * g.ncol);
+    if (want > light) want = light > fill ? light : (want < fill ? want : fill);
     g.ppc = cdiv(P, want);
     g.nchunk = (int)cdiv(P, g.ppc);
+    g.fold = g.ncol == 1 && G <= GN_FG && (int64_t)g.nchunk * C <= GN_FOLD;
     return g;
 }
 
@@ -818,11 +989,12 @@ static int gn_fwd_run(const ugpg_group_norm_t* d, void* y, void* ws, hipStream_t
     const GnGeom g = gn_geom(B, P, C, G, V);
     const unsigned nb = (unsigned)((int64_t)B * g.nchunk * g.ncol);
     float* part = static_cast<float*>(ws);
-    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3(nb), dim3(256), 0, s, xt, g, part);
-    hipLaunchKernelGGL(gn_merge_kernel, dim3((unsigned)cdiv((int64_t)B * G, 4)), dim3(256), 0, s,
-                       part, g, B, eps, mean, rstd);
-    hipLaunchKernelGGL((gn_apply_kernel<T, V>), dim3(nb), dim3(256), 0, s, xt, g, mean, rstd, gamma,
-                       beta, act, static_cast<T*>(y));
+    hipLaunchKernelGGL((gn_stats_kernel<T, V>), dim3(nb), dim3(GN_NT), 0, s, xt, g, part);
+    if (!g.fold)
+        hipLaunchKernelGGL(gn_merge_kernel, dim3((unsigned)cdiv((int64_t)B * G, 4)), dim3(256), 0, s,
+                           part, g, B, eps, mean, rstd);
+    hipLaunchKernelGGL((gn_apply_kernel<T, V>), dim3(nb), dim3(GN_NT), 0, s, xt, g, part, eps, mean,
+                       rstd, gamma, beta, act, static_cast<T*>(y));
     return check_launch("group_norm_fwd");
 }
 
@@ -883,15 +1055,22 @@ static int gn_bwd_run(const ugpg_group_norm_t* p, const void* dy, void* dx, floa
                                rstd, gamma, dgamma, dbeta, dxsum);
         return check_launch("group_norm_bwd");
     }
-    const GnGeom g = gn_geom(B, P, C, G, V);
+    GnGeom g = gn_geom(B, P, C, G, V);
+    g.fold = g.fold && !dxsum;  // (the sum of dx needs the totals)
     const unsigned nb = (unsigned)((int64_t)B * g.nchunk * g.ncol);
-    hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, TD, V>), dim3(nb), dim3(256), 0, s, dt, xt, g, mean,
-                       rstd, gamma, beta, act, part);
-    hipLaunchKernelGGL(gn_bwd_merge_kernel, dim3((unsigned)((int64_t)B * G)), dim3(256), 0, s, part,
-                       g, gamma, tot, sums);
-    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, TD, TO, V>), dim3(nb + pblocks), dim3(256), 0, s, dt, xt,
-                       g, B, nb, mean, rstd, gamma, beta, act, tot, sums, static_cast<TO*>(dx),
-                       dgamma, dbeta, dxsum);
+    if (g.fold) {
+        hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, TD, V, false>), dim3(nb), dim3(GN_NT), 0, s, dt, xt, g,
+                           mean, rstd, gamma, beta, act, part);
+    } else {
+        hipLaunchKernelGGL((gn_bwd_reduce_kernel<T, TD, V, true>), dim3(nb), dim3(GN_NT), 0, s, dt, xt, g,
+                           mean, rstd, gamma, beta, act, part);
+        hipLaunchKernelGGL(gn_bwd_merge_kernel, dim3((unsigned)((int64_t)B * G)), dim3(256), 0, s, part,
+                           g, gamma, tot, sums);
+    }
+    const unsigned np = dgamma || dbeta || dxsum ? (unsigned)cdiv(C, 64) : 0;
+    hipLaunchKernelGGL((gn_bwd_apply_kernel<T, TD, TO, V>), dim3(nb + np), dim3(GN_NT), 0, s, dt, xt, g, B,
+                       np, mean, rstd, gamma, beta, act, part, tot, sums, static_cast<TO*>(dx), dgamma,
+                       dbeta, dxsum);
     return check_launch("group_norm_bwd");
 }
 
