@@ -70,3 +70,22 @@ def test_c_entries_refuse_before_any_launch():
     assert bwd(n=nb - 1) == -3
     for kw in (dict(dy=None), dict(dx=None), dict(dyt=1), dict(dxt=1), dict(d=1, dyt=1)):
         assert bwd(**kw) == -1, kw
+
+
+def test_models_take_a_norm():
+    """norm="group" keeps the parameter names and drops the running buffers; the default is
+    the reference's BatchNorm; anything else, and groups that do not divide, are refused."""
+    import torch.nn as nn
+    import ugpg
+    a, b = ugpg.PGUNet1(3, 1), ugpg.PGUNet1(3, 1, norm="group", groups=16)
+    assert [k for k, _ in a.named_parameters()] == [k for k, _ in b.named_parameters()]
+    assert isinstance(a.inc.conv.conv_op[1], nn.BatchNorm2d) and not list(b.buffers())
+    assert b.inc.conv.conv_op[1].num_groups == 16
+    p = ugpg.ProgressiveUNet(3, 1, norm="group")
+    assert all(isinstance(p.stages[s].inc.conv.conv_op[1], nn.GroupNorm) for s in p.stages)
+    with pytest.raises(ValueError, match="norm must be"):
+        ugpg.DoubleConv(3, 64, norm="layer")
+    with pytest.raises(ValueError):
+        ugpg.DoubleConv(3, 64, norm="group", groups=48)
+    state, copied = ugpg.transfer_state(b.state_dict(), ugpg.PGUNet2(3, 1, norm="group", groups=16).state_dict())
+    assert len(copied) > 10

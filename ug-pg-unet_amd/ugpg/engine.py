@@ -5,7 +5,9 @@ UG_unet_parts.py:5-81) plus optional 1x1 deep-supervision *heads*
 (UG_unet_parts.py:84-91, UG_unet.py:294-303).  Every block output is kept as a
 lazily-activated NHWC tensor ``Act(y, scale, shift)``: the second conv's raw
 output plus its folded BatchNorm affine; consumers (max-pool, bilinear x2, the
-next conv, the heads) apply ``relu(scale*y+shift)`` while loading.  The
+next conv, the heads) apply ``relu(scale*y+shift)`` while loading.  (A group
+norm's coefficients differ from sample to sample: its result is written out, an
+``Act`` without coefficients.)  The
 backward pass is an explicit schedule (heads -> decoder -> encoder -> inc) that
 writes parameter gradients straight into caller-provided tensors (views of one
 flat gradient buffer) and accumulates activation gradients in place, so no
@@ -60,6 +62,9 @@ class BlockCtx:
     extra: dict = field(default_factory=dict)
     part2: torch.Tensor = None  # BN2-backward partials written by the last producer of da2
     route2: tuple = None  # (route, has_base): the deferred last producer of da2 (bn_relu_bwd)
+    a1: Act = None  # the second conv's input
+    gn1: object = None  # ops.GroupNormCall of each conv's norm where that is a group norm
+    gn2: object = None
 
 
 def _grad_like(y):
@@ -75,8 +80,12 @@ def _bn_mode(bn):
     return bn.training or not bn.track_running_stats
 
 
+def _is_group(norm):
+    return isinstance(norm, torch.nn.GroupNorm)
+
+
 def double_conv_forward(mod, srcs, ctx: BlockCtx, save: bool):
-    """conv3x3 -> BN -> ReLU, twice (UG_unet_parts.py:9-16) on Act inputs."""
+    """conv3x3 -> norm -> ReLU, twice (UG_unet_parts.py:9-16) on Act inputs."""
     B, H, W, _ = srcs[0].shape
     cin = sum(s.C for s in srcs)
     cur = srcs
@@ -90,7 +99,8 @@ def double_conv_forward(mod, srcs, ctx: BlockCtx, save: bool):
         store16 = _store16(W) and (wpk.ugpg_fmt == ops.WFMT_BF16 or (cin == 8 and cout in (64, 128)))
         y = ops.empty(B, H, W, cout, like=srcs[0].y,
                       dtype=torch.bfloat16 if store16 else torch.float32)
-        train = _bn_mode(bn)
+        group = _is_group(bn)
+        train = not group and _bn_mode(bn)
         stats = None
         ntiles = 0
         if train:
@@ -99,7 +109,12 @@ def double_conv_forward(mod, srcs, ctx: BlockCtx, save: bool):
         bias = conv.bias.detach() if conv.bias is not None else None
         ops.conv3x3_fwd(cur, wpk, bias, cout, [y], stats=stats,
                         flops=2.0 * B * H * W * cout * 9 * w.shape[1])
-        if train:
+        if group:
+            gn = ops.GroupNormCall(y, bn.num_groups, bn.weight.detach() if bn.affine else None,
+                                   bn.bias.detach() if bn.affine else None, float(bn.eps), "relu")
+            cur = [Act(gn.forward())]
+            st = (None, None, None, None)
+        elif train:
             if bn.momentum is None:
                 raise NotImplementedError("BatchNorm2d(momentum=None) is not supported")
             track = bn.track_running_stats and bn.running_mean is not None
@@ -113,14 +128,29 @@ def double_conv_forward(mod, srcs, ctx: BlockCtx, save: bool):
                                               bn.running_mean, bn.running_var, float(bn.eps),
                                               owner=bn)
             st = (None, None, scale, shift)
+        if not group:
+            gn, cur = None, [Act(y, scale, shift)]
         if save:
             if i == 0:
-                ctx.y1, ctx.st1 = y, st
+                ctx.y1, ctx.st1, ctx.gn1, ctx.a1 = y, st, gn, cur[0]
             else:
-                ctx.y2, ctx.st2 = y, st
-        cur = [Act(y, scale, shift)]
+                ctx.y2, ctx.st2, ctx.gn2 = y, st, gn
         cin = cout
     return cur[0]
+
+
+def _group_norm_wgrad(conv, norm, call, in_srcs, da, grads):
+    """As _bn_relu_wgrad, through a group norm: da becomes dy in place, or a bf16 tensor where
+    x is stored in bf16 and the weight gradient reads that."""
+    dy, dw = da, grads.get(conv.weight)
+    if call.x.dtype == torch.bfloat16 and all(s.C % 64 == 0 for s in in_srcs):
+        dy = ops.empty(*da.shape, like=da, dtype=torch.bfloat16)
+    ops.group_norm_bwd(call, da, dy, grads.get(norm.weight), grads.get(norm.bias),
+                       grads.get(conv.bias) if conv.bias is not None else None)
+    if dw is not None:
+        co, ci = conv.weight.shape[:2]
+        ops.conv3x3_wgrad(in_srcs, dy, dw, None, ci, flops=2.0 * dy.numel() / co * co * 9 * ci)
+    return dy
 
 
 def _bn_relu_wgrad(conv, bn, y, st, in_srcs, da, grads, part=None, route=None, need_dy=True):
@@ -189,10 +219,12 @@ def double_conv_backward(mod, ctx: BlockCtx, da2, targets, acc_flags, grads, pad
     pad_out: padded channel count of a single dgrad target (the image input)."""
     (c1, b1), (c2, b2) = _conv_bn(mod.conv_op)
     B, H, W, cout = ctx.y2.shape
-    a1 = Act(ctx.y1, ctx.st1[2], ctx.st1[3])
-    # stage 2: BN2/ReLU backward, wgrad(conv2), dgrad(conv2) -> dL/d(a1)
-    dy2 = _bn_relu_wgrad(c2, b2, ctx.y2, ctx.st2, [a1], da2, grads, part=ctx.part2,
-                         route=ctx.route2)
+    # stage 2: norm2/ReLU backward, wgrad(conv2), dgrad(conv2) -> dL/d(a1)
+    if ctx.gn2 is not None:
+        dy2 = _group_norm_wgrad(c2, b2, ctx.gn2, [ctx.a1], da2, grads)
+    else:
+        dy2 = _bn_relu_wgrad(c2, b2, ctx.y2, ctx.st2, [ctx.a1], da2, grads, part=ctx.part2,
+                             route=ctx.route2)
     cmid = c2.weight.shape[1]
     npix = B * H * W
     wpk2 = ops.pack_conv3x3(c2.weight.detach(), cmid, 1)
@@ -212,8 +244,11 @@ def double_conv_backward(mod, ctx: BlockCtx, da2, targets, acc_flags, grads, pad
     ops.conv3x3_fwd([Act(dy2)], wpk2, None, cmid, [da1], flops=2.0 * npix * cmid * 9 * cout,
                     bnb=bnb)
     # stage 1: BN1/ReLU backward, wgrad(conv1), dgrad(conv1) -> source targets
-    dy1 = _bn_relu_wgrad(c1, b1, ctx.y1, ctx.st1, ctx.srcs, da1, grads, part=part,
-                         need_dy=any(t is not None for t in targets))
+    if ctx.gn1 is not None:
+        dy1 = _group_norm_wgrad(c1, b1, ctx.gn1, ctx.srcs, da1, grads)
+    else:
+        dy1 = _bn_relu_wgrad(c1, b1, ctx.y1, ctx.st1, ctx.srcs, da1, grads, part=part,
+                             need_dy=any(t is not None for t in targets))
     if not any(t is not None for t in targets):
         return
     cin = c1.weight.shape[1]
@@ -262,7 +297,7 @@ class UNetGraph:
         call double_conv_forward makes), computed on the current stream."""
         for blk in self.blocks:
             for _, bn in _conv_bn(blk.mod.conv_op):
-                if not _bn_mode(bn):
+                if not _is_group(bn) and not _bn_mode(bn):
                     ops.bn_eval_params(bn.weight.detach(), bn.bias.detach(), bn.running_mean,
                                        bn.running_var, float(bn.eps), owner=bn)
 

@@ -86,7 +86,11 @@ class MoNuSegTester:
             stage, state = 4, ckpt
         else:
             raise RuntimeError(f"Unrecognized checkpoint format for: {model_path}")
-        model = _STAGE_MODELS.get(stage, PGUNet4)(in_channels=3, num_classes=1)
+        # a model without running statistics was trained with norm="group"
+        group = not any(k.endswith("running_mean") for k in state)
+        model = _STAGE_MODELS.get(stage, PGUNet4)(in_channels=3, num_classes=1,
+                                                  norm="group" if group else "batch",
+                                                  groups=int(ckpt.get("norm_groups", 32)) if group else 32)
         model.load_state_dict(state)
         self.stage = stage
         return model.to(self.device)

@@ -30,6 +30,7 @@ import torch.nn.functional as F
 
 from . import functional as Fn
 from . import ops
+from .distill import DistillationLoss
 from .flat import ensure_flat
 from .loss import UncertaintyGuidedLoss
 from .dist import (allreduce_gradients, allreduce_metrics, broadcast_buffers,
@@ -101,11 +102,12 @@ def _dropout(x, p, training):
 
 
 class HerlevClassificationModel(nn.Module):
-    def __init__(self, stage: int, num_classes: int, pretrained_unet_path: str = None):
+    def __init__(self, stage: int, num_classes: int, pretrained_unet_path: str = None,
+                 norm: str = "batch", norm_groups: int = 32):
         super().__init__()
         self.stage = stage
         self.num_classes = num_classes
-        self.unet = STAGE_CLASSES[stage](in_channels=3, num_classes=1)
+        self.unet = STAGE_CLASSES[stage](in_channels=3, num_classes=1, norm=norm, groups=norm_groups)
         if pretrained_unet_path and os.path.exists(pretrained_unet_path):
             print(f"Loading pretrained U-Net weights from: {pretrained_unet_path}")
             sd = torch.load(pretrained_unet_path, map_location="cpu", weights_only=True)
@@ -183,7 +185,13 @@ class HerlevClassificationModel(nn.Module):
 class HerlevTrainer:
     """HerlevTrainer (train_herlev.py:124-489): stage configs, models,
     class-weighted criterion, Adam + ReduceLROnPlateau, classifier weight transfer,
-    forward pass, train/validate epochs, progressive driver with early stop."""
+    forward pass, train/validate epochs, progressive driver with early stop.
+
+    Config keys beyond the reference's, all optional:
+      norm, norm_groups: the encoders' normalisation ("batch", or "group" for small batches);
+      distill_weight (0): from stage 2 on adds distill_weight * T^2 * KL(previous stage ||
+        current stage) to the loss, from the previous stage's distill_top (3) largest logits
+        and the rest's, at temperature distill_temperature (2)."""
 
     def __init__(self, config):
         self.config = config
@@ -199,10 +207,18 @@ class HerlevTrainer:
         for stage in range(1, 5):
             self.models[stage] = HerlevClassificationModel(
                 stage, config["num_classes"],
-                config.get("pretrained_unet_paths", {}).get(stage)).to(self.device)
+                config.get("pretrained_unet_paths", {}).get(stage),
+                norm=config.get("norm", "batch"),
+                norm_groups=config.get("norm_groups", 32)).to(self.device)
         self.setup_loss_function()
         self.uncertainty_loss = UncertaintyGuidedLoss(self.device)
         self.uncertainty_alpha = config.get("uncertainty_alpha", 1.0)
+        scale = float(config.get("distill_weight", 0.0))
+        self.distillation = None
+        if scale != 0.0:
+            self.distillation = DistillationLoss(
+                min(int(config.get("distill_top", 3)), config["num_classes"]),
+                float(config.get("distill_temperature", 2.0)), scale)
         self.history = {k: [] for k in ("train_loss", "val_loss", "train_acc", "val_acc",
                                         "uncertainty_weights_mean", "uncertainty_weights_std",
                                         "base_loss", "stage_transitions")}
@@ -243,10 +259,15 @@ class HerlevTrainer:
             with torch.no_grad():
                 prev = pm(ops.resize_nchw(data.float().contiguous(), r, r, ops.RESIZE_BILINEAR))
         if self.config["num_classes"] <= 2:
-            return self._forward_binary(output, target, prev)
-        out = torch.empty(5, dtype=torch.float32, device=output.device)
-        final = _CEUGFn.apply(output, target.contiguous(), prev, self.class_weights,
-                              float(self.uncertainty_alpha), out)
+            output, final, out = self._forward_binary(output, target, prev)
+        else:
+            out = torch.empty(5, dtype=torch.float32, device=output.device)
+            final = _CEUGFn.apply(output, target.contiguous(), prev, self.class_weights,
+                                  float(self.uncertainty_alpha), out)
+        if prev is not None and self.distillation is not None:
+            distill = self.distillation(output, prev)  # the previous stage as the teacher
+            final = final + distill
+            out[0] += distill.detach()
         return output, final, out
 
     def _forward_binary(self, output, target, prev):

@@ -60,8 +60,11 @@ class MetricsReadback:
 
 
 class UncertaintyGuidedProgressiveTrainer:
-    def __init__(self, in_channels=3, num_classes=1, device="cuda", uncertainty_alpha=1.0):
+    def __init__(self, in_channels=3, num_classes=1, device="cuda", uncertainty_alpha=1.0,
+                 norm="batch", norm_groups=32):
+        """norm, norm_groups: the models' normalisation (PGUNet1-4's `norm`, `groups`)."""
         self.device = device
+        self.norm, self.norm_groups = norm, norm_groups
         self.in_channels = in_channels
         self.num_classes = num_classes
         self.uncertainty_alpha = uncertainty_alpha
@@ -71,7 +74,7 @@ class UncertaintyGuidedProgressiveTrainer:
             3: {"resolution": 128, "epochs_per_stage": 40, "lr": 1e-4},
             4: {"resolution": 256, "epochs_per_stage": 40, "lr": 1e-4},
         }
-        self.models = {s: cls(in_channels, num_classes).to(device)
+        self.models = {s: cls(in_channels, num_classes, norm, norm_groups).to(device)
                        for s, cls in ((1, PGUNet1), (2, PGUNet2), (3, PGUNet3), (4, PGUNet4))}
         self.current_stage = 1
         self.current_model = self.models[1]
@@ -396,7 +399,9 @@ class UncertaintyGuidedProgressiveTrainer:
                                     "optimizer_state_dict": self.optimizer.state_dict(),
                                     "val_dice": va[2], "train_dice": tr[2],
                                     "uncertainty_alpha": self.uncertainty_alpha,
-                                    "history": self.history},
+                                    "history": self.history,
+                                    **({"norm_groups": self.norm_groups}
+                                       if getattr(self, "norm", "batch") == "group" else {})},
                                    save_path / f"ug_pgunet_stage{stage}_best.pth")
                 print("-" * 60)
             # the finished stage becomes the next stage's U-map producer: one BN state

@@ -38,14 +38,16 @@ _LAYOUT = {
 class _PGUNetBase(nn.Module):
     STAGE = 0
 
-    def __init__(self, in_channels, num_classes):
+    def __init__(self, in_channels, num_classes, norm="batch", groups=32):
+        """norm: "batch" (the reference's BatchNorm2d) or "group" (GroupNorm over `groups`
+        groups in every DoubleConv, for small batches)."""
         super().__init__()
         width, enc, dec, heads = _LAYOUT[self.STAGE]
-        self.inc = InConv(in_channels, width)
+        self.inc = InConv(in_channels, width, norm, groups)
         for name, cin, cout in enc:
-            setattr(self, name, Down(cin, cout))
+            setattr(self, name, Down(cin, cout, norm, groups))
         for name, cin, cout in dec:
-            setattr(self, name, Up(cin, cout))
+            setattr(self, name, Up(cin, cout, norm=norm, groups=groups))
         for name, (_, _, cout) in zip(heads, dec):
             setattr(self, name, OutConv(cout, num_classes))
         self._graph_cache = None
@@ -170,7 +172,8 @@ class ProgressiveUNet(nn.Module):
     Also accepts the README spelling ``ProgressiveUNet(in_channels=3,
     out_channels=2, stage=1)``."""
 
-    def __init__(self, in_channels, num_classes=None, *, out_channels=None, stage=1):
+    def __init__(self, in_channels, num_classes=None, *, out_channels=None, stage=1, norm="batch",
+                 groups=32):
         super().__init__()
         if num_classes is None:
             num_classes = out_channels
@@ -180,10 +183,10 @@ class ProgressiveUNet(nn.Module):
         self.num_classes = num_classes
         self.current_stage = 1
         self.stage_resolutions = dict(STAGE_RESOLUTIONS)
-        self.stage1 = PGUNet1(in_channels, num_classes)
-        self.stage2 = PGUNet2(in_channels, num_classes)
-        self.stage3 = PGUNet3(in_channels, num_classes)
-        self.stage4 = PGUNet4(in_channels, num_classes)
+        self.stage1 = PGUNet1(in_channels, num_classes, norm, groups)
+        self.stage2 = PGUNet2(in_channels, num_classes, norm, groups)
+        self.stage3 = PGUNet3(in_channels, num_classes, norm, groups)
+        self.stage4 = PGUNet4(in_channels, num_classes, norm, groups)
         self.stages = {1: self.stage1, 2: self.stage2, 3: self.stage3, 4: self.stage4}
         if stage != 1:
             self.set_stage(stage)

@@ -17,8 +17,19 @@ from . import ops
 from .engine import Block, UNetGraph, _grad_like
 
 
-def _conv_bn_relu_layers(cin: int, cout: int):
-    return [nn.Conv2d(cin, cout, kernel_size=3, padding=1), nn.BatchNorm2d(cout), nn.ReLU(inplace=True)]
+def _norm_layer(cout: int, norm: str, groups: int):
+    """"batch": the reference's BatchNorm2d; "group": GroupNorm over `groups` groups, for
+    batches too small for batch statistics (same parameter names, no running buffers)."""
+    if norm == "batch":
+        return nn.BatchNorm2d(cout)
+    if norm == "group":
+        return nn.GroupNorm(groups, cout)
+    raise ValueError(f"norm must be 'batch' or 'group', got {norm!r}")
+
+
+def _conv_norm_relu_layers(cin: int, cout: int, norm: str, groups: int):
+    return [nn.Conv2d(cin, cout, kernel_size=3, padding=1), _norm_layer(cout, norm, groups),
+            nn.ReLU(inplace=True)]
 
 
 def _own_params(module):
@@ -26,12 +37,13 @@ def _own_params(module):
 
 
 class DoubleConv(nn.Module):
-    """[conv3x3(pad 1, bias) -> BatchNorm2d -> ReLU] x 2 (UG_unet_parts.py:5-19)."""
+    """[conv3x3(pad 1, bias) -> BatchNorm2d -> ReLU] x 2 (UG_unet_parts.py:5-19); with
+    norm="group" GroupNorm in BatchNorm's place."""
 
-    def __init__(self, in_channels, out_channels):
+    def __init__(self, in_channels, out_channels, norm="batch", groups=32):
         super().__init__()
-        layers = _conv_bn_relu_layers(in_channels, out_channels)
-        layers += _conv_bn_relu_layers(out_channels, out_channels)
+        layers = _conv_norm_relu_layers(in_channels, out_channels, norm, groups)
+        layers += _conv_norm_relu_layers(out_channels, out_channels, norm, groups)
         self.conv_op = nn.Sequential(*layers)
 
     def forward(self, x):
@@ -42,9 +54,9 @@ class DoubleConv(nn.Module):
 class InConv(nn.Module):
     """First DoubleConv of every stage (UG_unet_parts.py:21-28)."""
 
-    def __init__(self, in_channels, out_channels):
+    def __init__(self, in_channels, out_channels, norm="batch", groups=32):
         super().__init__()
-        self.conv = DoubleConv(in_channels, out_channels)
+        self.conv = DoubleConv(in_channels, out_channels, norm, groups)
 
     def forward(self, x):
         return self.conv(x)
@@ -53,9 +65,9 @@ class InConv(nn.Module):
 class Down(nn.Module):
     """MaxPool2d(2) then DoubleConv (UG_unet_parts.py:44-54)."""
 
-    def __init__(self, in_channels, out_channels):
+    def __init__(self, in_channels, out_channels, norm="batch", groups=32):
         super().__init__()
-        self.mpconv = nn.Sequential(nn.MaxPool2d(2), DoubleConv(in_channels, out_channels))
+        self.mpconv = nn.Sequential(nn.MaxPool2d(2), DoubleConv(in_channels, out_channels, norm, groups))
 
     @property
     def double_conv(self):
@@ -70,9 +82,9 @@ class Up(nn.Module):
     """bilinear x2 (align_corners=True) of x1, cat([x2, x1]), DoubleConv
     (UG_unet_parts.py:70-81).  `bilinear` is accepted and ignored, as in the reference."""
 
-    def __init__(self, in_channels, out_channels, bilinear=True):
+    def __init__(self, in_channels, out_channels, bilinear=True, norm="batch", groups=32):
         super().__init__()
-        self.conv = DoubleConv(in_channels, out_channels)
+        self.conv = DoubleConv(in_channels, out_channels, norm, groups)
 
     @property
     def double_conv(self):
