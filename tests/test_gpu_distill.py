@@ -395,12 +395,17 @@ def test_strides_alignment_and_mixed_types(dev):
                                      ((2, 12, 5, 6), 4)])
 def test_writes_stay_inside(dev, shape, k):
     import ctypes as C
+    import ugpg
     from tests._guard import guarded
     from ugpg import _C, ops
     for dtype in (F32, BF16):
         z, v, i, r, w = record(shape, k, dev, dtype, 2.0)
-        call = ops.DistillCall(z, v, i, r, w, 2.0, 1.0)
-        d, need = call.desc, call.nbytes
+        N, V = shape[:2]
+        inner = z.numel() // (N * V)
+        stride, code = V * inner, ops._dtype_code(z)
+        d = _C.DistillDesc(z.data_ptr(), code, N, V, inner, stride, v.data_ptr(), code, i.data_ptr(), 64, k,
+                           r.data_ptr(), w.data_ptr(), 2.0, 1.0)
+        need = _C.lib.ugpg_distill_workspace(C.byref(d), 0)
         work = guarded((need,), dev, torch.uint8)
         loss, rows = guarded((1,), dev), guarded((z.numel() // shape[1],), dev)
         dz = guarded(shape, dev, dtype)
@@ -408,12 +413,13 @@ def test_writes_stay_inside(dev, shape, k):
                                          work.t.data_ptr(), need, ops.stream()), "distill_fwd")
         for n, t in (("ws", work), ("loss", loss), ("rows", rows), ("dlogits", dz)):
             t.check(n)
-        want, grad = call.forward(grad=True)
-        assert torch.equal(want.view(1), loss.t) and torch.equal(grad, dz.t)
+        zr = z.clone().requires_grad_(True)
+        want = ugpg.distillation_loss(zr, (v, i, r), 2.0, weight=w, reduction="sum")
+        (grad,) = torch.autograd.grad(want, (zr,))
+        assert torch.equal(want.detach().view(1), loss.t) and torch.equal(grad, dz.t)
         # a partial record's buffers too
         vals, idx, rest = guarded(v.shape, dev, dtype), guarded((2 * i.numel(),), dev, torch.int32), guarded(r.shape, dev)
-        xx, N, V, inner, stride = ops._class_layout(z)
-        _C.check(_C.lib.ugpg_top_logits(xx.data_ptr(), ops._dtype_code(xx), N, V, inner, stride, k, 2.0,
+        _C.check(_C.lib.ugpg_top_logits(z.data_ptr(), code, N, V, inner, stride, k, 2.0,
                                         vals.t.data_ptr(), idx.t.data_ptr(), rest.t.data_ptr(), ops.stream()), "top")
         for n, t in (("values", vals), ("indices", idx), ("rest", rest)):
             t.check(n)

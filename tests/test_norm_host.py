@@ -89,3 +89,16 @@ def test_models_take_a_norm():
         ugpg.DoubleConv(3, 64, norm="group", groups=48)
     state, copied = ugpg.transfer_state(b.state_dict(), ugpg.PGUNet2(3, 1, norm="group", groups=16).state_dict())
     assert len(copied) > 10
+
+
+def test_autograd_nodes_are_built_from_these_sources():
+    import importlib.util
+    from pathlib import Path
+    from ugpg import _nodes
+    root = Path(__file__).resolve().parent.parent
+    spec = importlib.util.spec_from_file_location("_b", root / "ug-pg-unet_amd" / "build.py")
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    assert _nodes.nodes().build_id == b.autograd_id()
+    with pytest.raises(ImportError, match="stale"):
+        _nodes._check_fresh("0" * 32)

@@ -131,8 +131,11 @@ def build(force: bool = False, verbose: bool = True, defines=(), out: Path | Non
         force = True
     srcs = _sources()
     jobs = min(len(srcs), int(os.environ.get("MAX_JOBS", "8")))
-    with cf.ThreadPoolExecutor(max_workers=max(1, jobs)) as ex:
+    with cf.ThreadPoolExecutor(max_workers=max(1, jobs) + 1) as ex:
+        nodes = ex.submit(build_autograd, force) if out is None and not defines else None
         objs = list(ex.map(lambda s: _compile(s, force, bdir, defines), srcs))
+        if nodes is not None:
+            nodes.result()
     sid = source_id(defines)
     objs.append(_id_object(bdir, sid))
     newest = max(o.stat().st_mtime for o in objs)
@@ -149,6 +152,46 @@ def build(force: bool = False, verbose: bool = True, defines=(), out: Path | Non
     if verbose:
         print(f"built {LIB_} ({LIB_.stat().st_size / 1e6:.1f} MB)")
     return LIB_
+
+
+AUTOGRAD = HERE / "ugpg" / "_autograd.so"
+
+
+def autograd_id() -> str:
+    """Content hash of the autograd nodes' source and the header they share with libugpg, and
+    the torch they are compiled against."""
+    import torch
+    h = hashlib.sha256(torch.__version__.encode())
+    for f in (CSRC / "autograd.cpp", INCLUDE / "ugpg.h"):
+        h.update(f.read_bytes() + b"\0")
+    return h.hexdigest()[:32]
+
+
+def build_autograd(force: bool = False) -> Path:
+    """The autograd nodes (csrc/autograd.cpp, host C++ against torch) -> ugpg/_autograd.so.
+    Rebuilt when its id, recorded beside the objects, changes."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    BUILD.mkdir(parents=True, exist_ok=True)
+    sid, stamp = autograd_id(), BUILD / "autograd_id.txt"
+    if not force and AUTOGRAD.exists() and stamp.exists() and stamp.read_text() == sid:
+        return AUTOGRAD
+    lib = Path(torch.__file__).parent / "lib"
+    inc = [*cpp_extension.include_paths("cuda"), sysconfig.get_paths()["include"], "/opt/rocm/include"]
+    tmp = AUTOGRAD.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-DTORCH_EXTENSION_NAME=_autograd", f'-DUGPG_AUTOGRAD_ID="{sid}"', *[f"-I{i}" for i in inc],
+           str(CSRC / "autograd.cpp"), "-o", str(tmp), f"-L{lib}", "-lc10", "-lc10_hip", "-ltorch_cpu",
+           "-ltorch", "-ltorch_python", f"-Wl,-rpath,{lib}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"autograd nodes failed:\n{r.stderr}")
+    os.replace(tmp, AUTOGRAD)
+    stamp.write_text(sid)
+    return AUTOGRAD
 
 
 SAN_FLAGS = ["-Xarch_host", "-fsanitize=address", "-Xarch_host", "-fsanitize=undefined"]

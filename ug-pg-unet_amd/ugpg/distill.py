@@ -14,6 +14,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import ops
+from ._nodes import nodes
 
 
 class TopLogits(NamedTuple):
@@ -54,34 +55,7 @@ def teacher_top_logits(logits, k, temperature=1.0):
     if not isinstance(k, int) or not 1 <= k <= min(logits.shape[1], ops.TOP_MAX):
         raise ValueError(f"{what}: k must be an int in 1..{min(logits.shape[1], ops.TOP_MAX)}, got {k!r}")
     _check_device(what, logits)
-    with torch.no_grad(), ops.on_device(logits):
-        return TopLogits(*ops.top_logits(logits.detach(), k, temperature))
-
-
-class _DistillFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, values, indices, rest, weight, temperature, scale, per_row, grad):
-        # With a gradient to come, a scalar loss writes it here, for an upstream gradient of 1,
-        # while each row is in the caches: one reading of the logits instead of two.
-        with ops.on_device(logits):
-            call = ops.DistillCall(logits, values, indices, rest, weight, temperature, scale)
-            loss, dz = call.forward(per_row, grad and not per_row)
-        if grad:
-            ctx.save_for_backward(logits, values, indices, rest, weight)
-            ctx.call, ctx.dz = call, dz
-        return loss
-
-    @staticmethod
-    def backward(ctx, gout):
-        dz, ctx.dz = ctx.dz, None  # handed out once; a second backward writes its own
-        ctx.saved_tensors  # (raises if one was written in place since)
-        twice = torch.is_grad_enabled()  # create_graph
-        if gout.dtype != torch.float32 or not gout.is_contiguous():
-            gout = gout.detach().float().contiguous()
-        dz = ctx.call.backward(gout, dz)
-        if twice:
-            (dz,) = ops.differentiable_once("distillation_loss", (dz,))
-        return dz, None, None, None, None, None, None, None, None
+    return TopLogits(*nodes().top_logits(logits, k, temperature))
 
 
 def distillation_loss(logits, top, temperature=1.0, weight=None, reduction="mean", scale=1.0):
@@ -136,11 +110,15 @@ def distillation_loss(logits, top, temperature=1.0, weight=None, reduction="mean
     _check_device(what, logits)
     if reduction == "mean":
         scale = float(scale) / (lead[0] * spatial)
-    grad = torch.is_grad_enabled() and logits.requires_grad
-    return _DistillFn.apply(logits, values.contiguous(), indices.contiguous(),
-                            None if rest is None else rest.contiguous(),
-                            None if weight is None else weight.contiguous(), float(temperature),
-                            float(scale), reduction == "none", grad)
+    if not values.is_contiguous():
+        values = values.contiguous()
+    if not indices.is_contiguous():
+        indices = indices.contiguous()
+    if rest is not None and not rest.is_contiguous():
+        rest = rest.contiguous()
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    return nodes().distill(logits, values, indices, rest, weight, temperature, scale, reduction == "none")
 
 
 class DistillationLoss:

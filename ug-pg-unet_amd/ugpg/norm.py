@@ -11,32 +11,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-
-
-class _GroupNormActFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, grad):
-        with ops.on_device(x):
-            call = ops.GroupNormCall(x, groups, weight, bias, eps, act)
-            y = call.forward()
-        if grad:
-            ctx.save_for_backward(x, weight, bias)
-            ctx.call = call
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        ctx.saved_tensors  # (raises if one was written in place since)
-        need = ctx.needs_input_grad
-        twice = torch.is_grad_enabled()  # create_graph
-        if dy.dtype != ctx.call.x.dtype or not dy.is_contiguous():
-            dy = dy.detach().to(ctx.call.x.dtype).contiguous()
-        dx, dw, db = ctx.call.backward(dy, need[1], need[2])
-        if not need[0]:
-            dx = None
-        if twice:
-            dx, dw, db = ops.differentiable_once("group_norm_act", (dx, dw, db))
-        return dx, dw, db, None, None, None, None
+from ._nodes import nodes
 
 
 def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="relu"):
@@ -70,12 +45,13 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
         raise RuntimeError("ugpg: tensor is not on a ROCm/HIP device (no CPU fallback)")
     if x.numel() == 0:
         raise ValueError(f"group_norm_act: empty input {tuple(x.shape)}")
-    grad = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias))
-    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    x = x if x.is_contiguous() else x.contiguous()
-    return _GroupNormActFn.apply(x, weight, bias, num_groups, float(eps), activation, grad)
+    if not x.is_contiguous():
+        x = x.contiguous()
+    if weight is not None and not weight.is_contiguous():
+        weight = weight.contiguous()
+    if bias is not None and not bias.is_contiguous():
+        bias = bias.contiguous()
+    return nodes().group_norm_act(x, weight, bias, num_groups, eps, ops.ACTIVATIONS[activation])
 
 
 class GroupNormAct(nn.GroupNorm):

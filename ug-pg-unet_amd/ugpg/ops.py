@@ -6,14 +6,13 @@ Activations are NHWC fp32 ``(B, H, W, C)`` tensors.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 
 import torch
 
-from ._C import (Bnb, BnLazy, BwdRoute, ConvDesc, DistillDesc, GroupNormDesc, PackItem, Src,
-                 WgradDesc, check, lib)
+from ._C import (Bnb, BnLazy, BwdRoute, ConvDesc, GroupNormDesc, PackItem, Src, WgradDesc,
+                 check, lib)
 
 F32 = torch.float32
 
@@ -22,31 +21,8 @@ def stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
-def differentiable_once(what, grads):
-    """The gradients of a backward that runs with create_graph: differentiating through one of
-    them raises, whether or not the upstream gradient required one."""
-    live = [g.detach().requires_grad_(True) for g in grads if g is not None]
-    err = torch._C._functions.DelayedError(f"{what} can be differentiated only once".encode(), len(live))
-    out = err(*live)
-    out = iter(out if isinstance(out, tuple) else (out,))
-    return tuple(None if g is None else next(out) for g in grads)
-
-
-_NO_CONTEXT = contextlib.nullcontext()
-
-
-def on_device(t):
-    """Context: the device of `t` is current (a launch goes to its stream, whatever device
-    the caller left current)."""
-    if t.is_cuda and t.get_device() != torch.cuda.current_device():
-        return torch.cuda.device(t.device)
-    return _NO_CONTEXT
-
-
 def stream_of(t) -> int:
-    """The current stream of the device `t` lies on, without building a Stream object (the
-    autograd thread pays several times over for every Python object it shares with the
-    calling thread: stream() costs 18 us there, this 1)."""
+    """The current stream of the device `t` lies on, without building a Stream object."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
@@ -499,15 +475,14 @@ def _dtype_code(t):
 
 class GroupNormCall:
     """A group normalisation of x (B, ..., C), channels last: its descriptor over tensors it
-    keeps, filled once; the backward (on the autograd thread) adds only its own tensors."""
-    __slots__ = ("x", "gamma", "beta", "mean", "rstd", "code", "desc", "ref", "nbytes")
+    keeps, filled once for the forward and the backward (group_norm_bwd)."""
+    __slots__ = ("x", "gamma", "beta", "mean", "rstd", "desc", "ref", "nbytes")
 
     def __init__(self, x, groups, gamma, beta, eps, act):
         B, c = x.shape[0], x.shape[-1]
         self.x, self.gamma, self.beta = x, gamma, beta
         self.mean, self.rstd = torch.empty(2, B, groups, dtype=F32, device=x.device)
-        self.code = _dtype_code(x)
-        self.desc = GroupNormDesc(ptr(x), self.code, B, x.numel() // (B * c), c, groups, ptr(gamma),
+        self.desc = GroupNormDesc(ptr(x), _dtype_code(x), B, x.numel() // (B * c), c, groups, ptr(gamma),
                                   ptr(beta), eps, ACTIVATIONS[act], self.mean.data_ptr(),
                                   self.rstd.data_ptr())
         self.ref = C.byref(self.desc)
@@ -520,19 +495,6 @@ class GroupNormCall:
         check(lib.ugpg_group_norm_fwd(self.ref, y.data_ptr(), ws.data_ptr(), self.nbytes, stream_of(x)),
               "group_norm_fwd")
         return y
-
-    def backward(self, dy, need_gamma, need_beta):
-        """-> (dx, dgamma or None, dbeta or None); dy contiguous, of x's type."""
-        x, code = self.x, self.code
-        dx = torch.empty_like(x)
-        dgamma = torch.empty_like(self.gamma) if need_gamma else None
-        dbeta = torch.empty_like(self.beta) if need_beta else None
-        ws = torch.empty(self.nbytes, dtype=torch.uint8, device=x.device)
-        check(lib.ugpg_group_norm_bwd(
-            self.ref, dy.data_ptr(), code, dx.data_ptr(), code,
-            dgamma.data_ptr() if need_gamma else None, dbeta.data_ptr() if need_beta else None, None,
-            ws.data_ptr(), self.nbytes, stream_of(x)), "group_norm_bwd")
-        return dx, dgamma, dbeta
 
 
 def group_norm_bwd(call, dy, dx, dgamma=None, dbeta=None, dxsum=None):
@@ -897,84 +859,9 @@ def ce_ug_bwd(x, y, wts, class_weights, gout):
     return dx
 
 
-# ------------------------------------------------------------------ distillation
+# limits of teacher_top_logits and distillation_loss (csrc/distill.hip)
 TOP_MAX = 256        # entries of a teacher's record
 MAP_CLASSES = 1024   # classes of the maps distillation reads
-
-
-def _class_layout(logits):
-    """(logits, N, V, inner, row stride) of (N, V) rows -- any row stride, unit column stride
-    -- or (N, V, *spatial) class maps; other strides are copied."""
-    N, V = logits.shape[:2]
-    inner = logits.numel() // (N * V)
-    if inner > 1:
-        return logits.contiguous(), N, V, inner, V * inner
-    rows = logits.reshape(N, V)
-    if (V > 1 and rows.stride(1) != 1) or (N > 1 and rows.stride(0) < V):
-        rows = rows.contiguous()
-    return rows, N, V, 1, max(rows.stride(0), V)
-
-
-def _dev_ptr(t):
-    if not t.is_cuda:
-        raise RuntimeError("ugpg: tensor is not on a ROCm/HIP device (no CPU fallback)")
-    return t.data_ptr()
-
-
-def top_logits(logits, k, temperature):
-    """-> (values, indices, rest) of ugpg_top_logits, shaped (N, k, *spatial) and (N, *spatial)."""
-    x, N, V, inner, stride = _class_layout(logits)
-    sp = logits.shape[2:]
-    values = torch.empty(N, k, *sp, dtype=x.dtype, device=x.device)
-    indices = torch.empty(N, k, *sp, dtype=torch.int64, device=x.device)
-    rest = torch.empty(N, *sp, dtype=F32, device=x.device)
-    check(lib.ugpg_top_logits(_dev_ptr(x), _dtype_code(x), N, V, inner, stride, int(k),
-                              float(temperature), values.data_ptr(), indices.data_ptr(),
-                              rest.data_ptr(), stream_of(x)), "top_logits")
-    return values, indices, rest
-
-
-class DistillCall:
-    """A distillation descriptor over tensors it keeps, checked and sized once; its backward
-    reuses it (no further Python there than the call)."""
-    __slots__ = ("desc", "ref", "nbytes", "nback", "logits", "keep")
-
-    def __init__(self, logits, values, indices, rest, weight, temperature, scale):
-        x, N, V, inner, stride = _class_layout(logits)
-        self.desc = DistillDesc(_dev_ptr(x), _dtype_code(x), N, V, inner, stride, ptr(values),
-                                _dtype_code(values), ptr(indices),
-                                32 if indices.dtype == torch.int32 else 64, values.shape[1],
-                                ptr(rest), ptr(weight), temperature, scale)
-        self.ref = C.byref(self.desc)
-        self.logits, self.keep = logits, (x, values, indices, rest, weight)
-        self.nbytes = lib.ugpg_distill_workspace(self.ref, 0)
-        if self.nbytes == 0:
-            check(-1, "distill_workspace")
-        self.nback = lib.ugpg_distill_workspace(self.ref, 1)
-
-    def forward(self, per_row=False, grad=False):
-        """-> (loss, dlogits or None): loss a scalar, or (per_row) one value a row."""
-        z = self.logits
-        loss = torch.empty((z.shape[0], *z.shape[2:]) if per_row else (), dtype=F32, device=z.device)
-        dz = torch.empty(z.shape, dtype=z.dtype, device=z.device) if grad else None
-        ws = torch.empty(self.nbytes, dtype=torch.uint8, device=z.device)
-        p = loss.data_ptr()
-        check(lib.ugpg_distill_fwd(self.ref, None if per_row else p, p if per_row else None,
-                                   None if dz is None else dz.data_ptr(), ws.data_ptr(), self.nbytes,
-                                   stream_of(z)), "distill_fwd")
-        return loss, dz
-
-    def backward(self, gout, dz=None):
-        """dlogits for the upstream gradient gout (float32; a scalar, or one value a row).
-        dz: the gradient forward() wrote, kept where gout is 1 and written anew elsewhere."""
-        z, skip = self.logits, dz is not None
-        if not skip:
-            dz = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-        n = self.nback
-        ws = torch.empty(n, dtype=torch.uint8, device=z.device) if n else None
-        check(lib.ugpg_distill_bwd(self.ref, gout.data_ptr(), gout.dim() > 0, skip, dz.data_ptr(),
-                                   ws.data_ptr() if n else None, n, stream_of(z)), "distill_bwd")
-        return dz
 
 
 def adam_step(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0):
