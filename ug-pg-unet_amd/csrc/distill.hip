@@ -215,77 +215,66 @@ __device__ __forceinline__ float distill_value(const DistillArgs& a, size_t at) 
                  : static_cast<const float*>(a.values)[at];
 }
 
-// what a row's k + 1 classes give (computed by one wave over entries in LDS)
+// What a row's k + 1 classes give (computed by one wave over entries in LDS), in fp64: a loss is
+// the difference of logarithms of nearly equal probabilities, and fp32 exponentials alone
+// put a single row's KL 2e-7 off.
 struct RowTerms {
-    double kl;       // NaN / inf as they come out
-    double M, m, iT; // the teacher's and the student's maximum, 1 / T
-    float rsq, rs;   // 1 / sums
-    float restdiff;  // (p_rest - q_rest) / s_rest (0 where the student's rest is empty)
-    bool empty;      // the record says nothing: no loss, no gradient
-    // exp((t - M) / T): the quotient in fp64, rounded once
-    __device__ __forceinline__ float q(float t) const { return expf((float)(((double)t - M) * iT)); }
-    __device__ __forceinline__ float p(float z) const { return expf((float)(((double)z - m) * iT)); }
+    double kl;         // NaN / inf as they come out
+    double M, m, iT;   // the teacher's and the student's maximum, 1 / T
+    double rsq, rs;    // 1 / sums
+    double restdiff;   // (p_rest - q_rest) / s_rest (0 where the student's rest is empty)
+    bool empty;        // the record says nothing: no loss, no gradient
+    __device__ __forceinline__ double q(float t) const { return exp(((double)t - M) * iT); }
+    __device__ __forceinline__ double p(float z) const { return exp(((double)z - m) * iT); }
     __device__ __forceinline__ float grad(double g, float t, float z) const {
-        return (float)(g * ((double)(p(z) * rs) - (double)(q(t) * rsq)));
+        return (float)(g * (p(z) * rs - q(t) * rsq));
     }
 };
 
-// One wave; idx < 0: absent.  r: the student's rest.  The exponentials are fp32 (their errors,
-// 2^-22 of each probability, do not favour one side), what the loss is the difference of --
-// logarithms of probabilities -- fp64.
+// one wave; idx < 0: absent.  r: the student's rest
 __device__ __forceinline__ RowTerms row_terms(const int* idx, const float* t, const float* z, int k,
                                               float rest, MaxSum r, double T) {
     const int lane = threadIdx.x & 63;
-    const double iT = 1.0 / T;
     RowTerms o;
+    o.iT = 1.0 / T;
     float M = rest, m = r.m;
     for (int j = lane; j < k; j += 64)
         if (idx[j] >= 0) {
             M = fmaxf(M, t[j]);
             m = fmaxf(m, z[j]);
         }
-    M = wave_max(M);
-    m = wave_max(m);
-    o.M = M;
-    o.m = m;
-    o.iT = iT;
-    float sq = 0.f, ss = 0.f;
+    o.M = M = wave_max(M);
+    o.m = m = wave_max(m);
+    double sq = 0, ss = 0, kl = 0;
     for (int j = lane; j < k; j += 64)
         if (idx[j] >= 0) {
-            sq += o.q(t[j]);
+            const double e = o.q(t[j]);
+            sq += e;
             ss += o.p(z[j]);
+            if (!(e == 0.0)) kl += e * (((double)t[j] - o.M) - ((double)z[j] - o.m));
         }
-    sq = wave_sum(sq);
-    ss = wave_sum(ss);
-    const float er = rest == NEG_INF ? 0.f : o.q(rest);
-    const float sr = r.m == NEG_INF ? r.s : r.s * o.p(r.m);  // (an empty rest's sum is 0, or a NaN)
+    sq = wave_sum_d(sq);
+    ss = wave_sum_d(ss);
+    kl = wave_sum_d(kl) * o.iT;
+    const double er = rest == NEG_INF ? 0.0 : o.q(rest);
+    const double sr = r.m == NEG_INF ? (double)r.s : (double)r.s * o.p(r.m);  // (empty: 0, or a NaN)
+    // the rest's log q - log p, but for the logarithms of the sums
+    if (!(er == 0.0))
+        kl += er * (r.m == NEG_INF ? (double)__builtin_inff()
+                                   : (((double)rest - o.M) - ((double)r.m - o.m)) * o.iT - log((double)r.s));
     sq += er;
     ss += sr;
-    o.rsq = 1.f / sq;
-    o.rs = 1.f / ss;
-    // log q_j - log p_j = (t_j - M)/T - (z_j - m)/T - shift
-    const double lq = log((double)sq), ls = log((double)ss);
-    double kl = 0;
-    for (int j = lane; j < k; j += 64)
-        if (idx[j] >= 0) {
-            const float q = o.q(t[j]) * o.rsq;
-            if (!(q == 0.f))
-                kl += (double)q * ((((double)t[j] - o.M) * iT - lq) - (((double)z[j] - o.m) * iT - ls));
-        }
-    o.kl = wave_sum_d(kl);
-    const float qr = er * o.rsq;
-    if (!(qr == 0.f)) {
-        const double logr = r.m == NEG_INF ? (double)NEG_INF : ((double)r.m - o.m) * iT + log((double)r.s);
-        o.kl += (double)qr * ((((double)rest - o.M) * iT - lq) - (logr - ls));
-    }
-    o.restdiff = r.m == NEG_INF ? 0.f : (sr * o.rs - qr) / r.s;
+    o.rsq = 1.0 / sq;
+    o.rs = 1.0 / ss;
+    o.kl = kl * o.rsq + log(ss * o.rsq);  // (the q_j add up to 1)
+    o.restdiff = r.m == NEG_INF ? 0.0 : (sr * o.rs - er * o.rsq) / (double)r.s;
     o.empty = M == NEG_INF;
     return o;
 }
 
 // ---------------------------------------------------------------- rows, a block each
 struct RowShared {
-    int idx[DK_MAX];
+    alignas(16) int idx[DK_MAX];
     float t[DK_MAX], z[DK_MAX], ms[2 * 16];
     int dup;
     float a, mr;
@@ -293,38 +282,63 @@ struct RowShared {
     RowTerms o;
 };
 
-// the record's entries into LDS, the student's logits at them, and the bitmap of the kept
-// classes within the span; an index given twice counts the first time only
+// the bitmap of the kept classes within the span
+template <typename T>
+__device__ __forceinline__ void row_marks(const DistillArgs& a, int64_t r, const RowSpan<T>& sp, uint32_t* bits) {
+    const int tid = threadIdx.x, nt = blockDim.x;
+    for (int i = tid; i < (sp.bits() + 31) / 32; i += nt) bits[i] = 0;
+    __syncthreads();
+    for (int j = tid; j < a.k; j += nt) {
+        const int i = distill_index(a, (size_t)r * a.k + j);
+        if (i >= sp.lo && i < sp.hi) atomicOr(&bits[sp.bit(i) >> 5], 1u << (sp.bit(i) & 31));
+    }
+    __syncthreads();
+}
+
+// the record's entries into LDS, the student's logits at them, and that bitmap; an index given
+// twice counts the first time only
 template <typename T>
 __device__ __forceinline__ void row_entries(const DistillArgs& a, int64_t r, const RowSpan<T>& sp,
                                             RowShared& s, uint32_t* bits) {
     const int tid = threadIdx.x, nt = blockDim.x;
     for (int i = tid; i < (sp.bits() + 31) / 32; i += nt) bits[i] = 0;
     if (tid == 0) s.dup = 0;
-    for (int j = tid; j < a.k; j += nt) {
-        const size_t at = (size_t)r * a.k + j;
-        const int i = distill_index(a, at);
+    const int kp = (a.k + 3) & ~3;
+    for (int j = tid; j < kp; j += nt) {
+        int i = -1;
+        if (j < a.k) {
+            const size_t at = (size_t)r * a.k + j;
+            i = distill_index(a, at);
+            s.t[j] = distill_value(a, at);
+            s.z[j] = i >= 0 ? (float)sp.z[i] : NEG_INF;
+        }
         s.idx[j] = i;
-        s.t[j] = distill_value(a, at);
-        s.z[j] = i >= 0 ? (float)sp.z[i] : NEG_INF;
     }
     __syncthreads();
+    // entries up to j that equal j's index (four a read): one, unless it occurred before
+    auto upto = [&](int j) {
+        const int i = s.idx[j];
+        int n = 0;
+        for (int l = 0; l <= j; l += 4) {
+            const int4 q = *reinterpret_cast<const int4*>(&s.idx[l]);
+            n += (q.x == i) + (l + 1 <= j && q.y == i) + (l + 2 <= j && q.z == i) + (l + 3 <= j && q.w == i);
+        }
+        return n;
+    };
     for (int j = tid; j < a.k; j += nt) {
         const int i = s.idx[j];
         if (i >= sp.lo && i < sp.hi) {
             const int b = sp.bit(i);
             const uint32_t old = atomicOr(&bits[b >> 5], 1u << (b & 31));
             if (old >> (b & 31) & 1) s.dup = 1;
-        } else if (i >= 0) {
-            for (int l = 0; l < j; ++l)  // outside the span: no bitmap to ask
-                if (s.idx[l] == i) s.dup = 1;
+        } else if (i >= 0 && upto(j) > 1) {  // outside the span: no bitmap to ask
+            s.dup = 1;
         }
     }
     __syncthreads();
     if (s.dup) {  // (no correct record has one)
         unsigned drop = 0;
-        for (int q = 0, j = tid; j < a.k; j += nt, ++q)
-            for (int l = 0; l < j; ++l) drop |= (unsigned)(s.idx[l] == s.idx[j]) << q;
+        for (int q = 0, j = tid; j < a.k; j += nt, ++q) drop |= (unsigned)(upto(j) > 1) << q;
         __syncthreads();
         for (int q = 0, j = tid; j < a.k; j += nt, ++q)
             if (drop >> q & 1) s.idx[j] = -1;
@@ -414,7 +428,7 @@ __device__ __forceinline__ void row_finish(const DistillArgs& a, int64_t r, MaxS
             if (first && a.row_out) a.row_out[r] = (float)l;
             const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
             s.g = none ? 0.0 : a.coef * a.T * (double)w * go;
-            s.a = none ? 0.f : (float)(s.g * (double)o.restdiff);
+            s.a = none ? 0.f : (float)(s.g * o.restdiff);
             s.mr = rest.m;
             s.o = o;
             s.o.empty = none;
@@ -441,14 +455,14 @@ template <typename T>
 __global__ void __launch_bounds__(256) distill_part_kernel(DistillArgs a, int split, int chunk,
                                                            float* part) {
     extern __shared__ uint32_t bits[];
-    __shared__ RowShared s;
+    __shared__ float ms[8];
     if (distill_skip(a)) return;
     const int64_t r = blockIdx.x / split;
     const int c = blockIdx.x % split, lo = c * chunk;
     const RowSpan<T> sp(static_cast<const T*>(a.logits) + r * a.stride, lo < a.V ? lo : a.V,
                         lo + chunk < a.V ? lo + chunk : a.V);
-    row_entries<T>(a, r, sp, s, bits);
-    const MaxSum rest = block_maxsum(row_rest(a, sp, bits), a.c, s.ms);
+    row_marks<T>(a, r, sp, bits);
+    const MaxSum rest = block_maxsum(row_rest(a, sp, bits), a.c, ms);
     if (threadIdx.x == 0) {
         part[2 * blockIdx.x] = rest.m;
         part[2 * blockIdx.x + 1] = rest.s;
@@ -536,7 +550,7 @@ __device__ __forceinline__ double distill_wave_row(const DistillArgs& a, int64_t
         T* d = static_cast<T*>(a.dz) + (size_t)r * a.V;
         const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
         const double g = none ? 0.0 : a.coef * a.T * (double)w * go;
-        const float f = none || rest.m == NEG_INF ? 0.f : (float)(g * (double)o.restdiff);
+        const float f = none || rest.m == NEG_INF ? 0.f : (float)(g * o.restdiff);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int x = lane + 64 * i;
@@ -585,10 +599,122 @@ __global__ void __launch_bounds__(256) distill_wave_kernel(DistillArgs a) {
 }
 
 // ---------------------------------------------------------------- class maps, a thread each
+// the sum of a block's losses -> row_loss[block]
+__device__ __forceinline__ void map_sum(const DistillArgs& a, double l) {
+    __shared__ double red[4];
+    l = wave_sum_d(l);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = l;
+    __syncthreads();
+    if (threadIdx.x == 0 && a.row_loss) a.row_loss[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
+// At most VR classes and KR entries: a pixel's logits and record stay in registers, read once.
+// Exponentials are fp32 here (a map's loss is a mean over its pixels), sums and differences
+// fp64.  16 maps of 8 x 256^2 fp32 at 3 entries, with the gradient: 34 us against 55 for the form
+// below; its floor, 113 MB at a copy's 4.8 TB/s, is 24.
+template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) distill_map_small_kernel(DistillArgs a) {
+    if (distill_skip(a)) return;
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    double l = 0;
+    if (r < a.rows) {
+        const int64_t n = r / a.inner, p = r % a.inner;
+        const T* z = static_cast<const T*>(a.logits) + (size_t)n * a.V * a.inner + p;
+        const size_t rec = (size_t)n * a.k * a.inner + p;
+        const float c = a.c, iT = (float)(1.0 / a.T);
+        float x[VR], t[KR], zj[KR];
+        int idx[KR];
+#pragma unroll
+        for (int i = 0; i < VR; ++i) x[i] = i < a.V ? (float)z[(size_t)i * a.inner] : NEG_INF;
+#pragma unroll
+        for (int j = 0; j < KR; ++j) {
+            idx[j] = -1;
+            t[j] = NEG_INF;
+            if (j < a.k) {
+                idx[j] = distill_index(a, rec + (size_t)j * a.inner);
+                t[j] = distill_value(a, rec + (size_t)j * a.inner);
+            }
+        }
+        const float w = a.weight ? a.weight[r] : 1.f;
+        const float rest = a.rest ? a.rest[r] : NEG_INF;
+        uint32_t mask = 0;
+        float M = rest, m = NEG_INF;
+#pragma unroll
+        for (int j = 0; j < KR; ++j) {
+            const uint32_t b = idx[j] >= 0 ? 1u << idx[j] : 0u;
+            if (mask & b) idx[j] = -1;  // an index seen before is absent
+            mask |= b;
+            zj[j] = NEG_INF;
+#pragma unroll
+            for (int i = 0; i < VR; ++i) zj[j] = idx[j] == i ? x[i] : zj[j];
+            if (idx[j] >= 0) {
+                M = fmaxf(M, t[j]);
+                m = fmaxf(m, zj[j]);
+            }
+        }
+        RunSum acc;
+#pragma unroll
+        for (int i0 = 0; i0 < VR; i0 += 8) {
+            float y[8], mx = NEG_INF;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                y[e] = mask >> (i0 + e) & 1 ? NEG_INF : x[i0 + e];
+                mx = fmaxf(mx, y[e]);
+            }
+            acc.add(y, 8, mx, c);
+        }
+        const MaxSum rs = acc.done(c);
+        const bool has = rs.m != NEG_INF;
+        m = fmaxf(m, rs.m);
+        // as row_terms
+        double sq = 0, ss = 0, kl = 0;
+        float eq[KR], ep[KR];
+#pragma unroll
+        for (int j = 0; j < KR; ++j) {
+            eq[j] = ep[j] = 0.f;
+            if (idx[j] >= 0) {
+                eq[j] = expf((t[j] - M) * iT);
+                ep[j] = expf((zj[j] - m) * iT);
+                sq += eq[j];
+                ss += ep[j];
+                if (!(eq[j] == 0.f)) kl += (double)eq[j] * (((double)t[j] - M) - ((double)zj[j] - m));
+            }
+        }
+        kl /= a.T;
+        const float er = rest == NEG_INF ? 0.f : expf((rest - M) * iT);
+        const float sr = has ? rs.s * expf((rs.m - m) * iT) : rs.s;
+        if (!(er == 0.f))
+            kl += has ? (double)er * ((((double)rest - M) - ((double)rs.m - m)) / a.T - (double)logf(rs.s))
+                      : (double)__builtin_inff();
+        sq += er;
+        ss += sr;
+        const double rsq = 1.0 / sq, rss = 1.0 / ss;
+        const bool none = M == NEG_INF || w == 0.f;
+        l = none ? 0.0 : a.coef * a.T * a.T * (double)w * (kl * rsq + log(ss * rsq));
+        if (a.row_out) a.row_out[r] = (float)l;
+        if (a.dz) {
+            T* d = static_cast<T*>(a.dz) + (size_t)n * a.V * a.inner + p;
+            const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
+            const double g = none ? 0.0 : a.coef * a.T * (double)w * go;
+            const float f = none || !has ? 0.f : (float)(g * ((double)sr * rss - (double)er * rsq) / (double)rs.s);
+            float dk[KR];
+#pragma unroll
+            for (int j = 0; j < KR; ++j) dk[j] = none ? 0.f : (float)(g * ((double)ep[j] * rss - (double)eq[j] * rsq));
+#pragma unroll
+            for (int i = 0; i < VR; ++i) {
+                if (i >= a.V) break;
+                float v = f == 0.f ? 0.f : f * exp2_raw((x[i] - rs.m) * c);
+#pragma unroll
+                for (int j = 0; j < KR; ++j) v = idx[j] == i ? dk[j] : v;
+                d[(size_t)i * a.inner] = (T)v;
+            }
+        }
+    }
+    map_sum(a, l);
+}
+
 constexpr int DM_MAX = 1024;  // classes
 template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(DistillArgs a) {
     extern __shared__ uint32_t bits[];  // [ceil(V / 32)][256]
-    __shared__ double red[4];
     if (distill_skip(a)) return;
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
     double l = 0;
@@ -678,10 +804,7 @@ template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(
             }
         }
     }
-    l = wave_sum_d(l);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = l;
-    __syncthreads();
-    if (threadIdx.x == 0 && a.row_loss) a.row_loss[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+    map_sum(a, l);
 }
 
 __global__ void __launch_bounds__(1024) distill_sum_kernel(const double* part, int64_t n, float* loss) {
@@ -716,6 +839,7 @@ struct TopArgs {
     int64_t rows, inner, stride;
     int V, k;
     float T, c;  // temperature, log2(e) / T
+    int first;   // the first segment is this part of the tiles
     void* values;
     int64_t* indices;
     float* rest;
@@ -817,20 +941,24 @@ __device__ MaxSum top_exact(const TopArgs& a, const RowSpan<T>& sp, S& s) {
     return acc.done(a.c);
 }
 
-// one wave: the upper 16 bits of the k-th largest of n <= 64 * R keys (key(i): the i-th), bit
-// by bit, counting with ballots (shuffles would cost several times the comparisons)
+// one wave: the upper 16 bits of the k-th largest of n <= 64 * R keys (key(i): the i-th),
+// counting with ballots (shuffles would cost several times the comparisons)
 template <int R, typename F> __device__ __forceinline__ uint32_t kth_prefix_of(int n, int k, F key) {
     const int lane = threadIdx.x & 63;
     uint32_t v[R];
 #pragma unroll
     for (int i = 0; i < R; ++i) v[i] = lane + 64 * i < n ? key(lane + 64 * i) >> 16 : 0u;
     uint32_t t = 0;
-    for (int b = 15; b >= 0; --b) {
-        const uint32_t up = t | 1u << b;
-        int c = 0;
+    for (int b = 14; b >= 0; b -= 2) {  // two bits a step: three independent counts
+        const uint32_t u1 = t | 1u << b, u2 = t | 2u << b, u3 = t | 3u << b;
+        int c1 = 0, c2 = 0, c3 = 0;
 #pragma unroll
-        for (int i = 0; i < R; ++i) c += __popcll(__ballot(v[i] >= up));
-        if (c >= k) t = up;
+        for (int i = 0; i < R; ++i) {
+            c1 += __popcll(__ballot(v[i] >= u1));
+            c2 += __popcll(__ballot(v[i] >= u2));
+            c3 += __popcll(__ballot(v[i] >= u3));
+        }
+        t = c3 >= k ? u3 : c2 >= k ? u2 : c1 >= k ? u1 : t;
     }
     return t;
 }
@@ -895,15 +1023,21 @@ template <typename T, int NT, int CAP> __global__ void __launch_bounds__(NT, 8) 
     const int tiles = (sp.nv + nt - 1) / nt;
     int end = tiles;
     if (a.V > TK_NEAR) {
-        end = (tiles + 3) / 4;
+        end = (tiles + a.first - 1) / a.first;
         float mx = NEG_INF;
-        for (int t = 0; t < end; ++t) {
-            const int i = t * nt + tid;
-            if (i < sp.nv) {
-                Pack<T, N> v;
-                v.load(body + (size_t)i * N);
-                mx = fmaxf(mx, top_of(v));
-            }
+        const int last = end * nt < sp.nv ? end * nt : sp.nv;
+        int i = tid;
+        for (; i + (U - 1) * nt < last; i += U * nt) {
+            Pack<T, N> v[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) v[u].load(body + (size_t)(i + u * nt) * N);
+#pragma unroll
+            for (int u = 0; u < U; ++u) mx = fmaxf(mx, top_of(v[u]));
+        }
+        for (; i < last; i += nt) {
+            Pack<T, N> v;
+            v.load(body + (size_t)i * N);
+            mx = fmaxf(mx, top_of(v));
         }
         sp.ends(tid, nt, [&](int, int, const Pack<T, N>& v, int) { mx = fmaxf(mx, top_of(v)); });
         s.mx[tid] = mx;
@@ -1164,7 +1298,10 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
         set_error("top_logits: values, indices and rest must be given");
         return UGPG_ERR_INVALID;
     }
-    TopArgs a{logits, N * inner, inner, stride, V, k, temperature, (float)(LOG2E / temperature), values, indices, rest};
+    TopArgs a{logits, N * inner, inner, stride, V, k, temperature, (float)(LOG2E / temperature), 4, values, indices, rest};
+    // few rows wait for their own steps, not for memory: a bound from the whole row, read twice,
+    // saves two of them (64 x 131072 bf16, k = 128: 28 us against 36; 512 rows: 55 against 49)
+    if (N <= 128) a.first = 1;
     hipStream_t s = as_stream(stream);
     const bool f32 = dtype == UGPG_DT_F32;
 #define TOP_GO(KF, KH, grid, nt)                                              \
@@ -1231,8 +1368,15 @@ static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, bool
     a.row_loss = loss ? static_cast<double*>(ws) : nullptr;
     if (p->inner > 1) {
         nsum = cdiv(rows, 256);
-        hipLaunchKernelGGL((distill_map_kernel<T>), dim3((unsigned)nsum), dim3(256),
-                           (unsigned)(cdiv(a.V, 32) * 1024), s, a);
+        const dim3 grid((unsigned)nsum);
+        if (a.V <= 8 && a.k <= 4)
+            hipLaunchKernelGGL((distill_map_small_kernel<T, 8, 4>), grid, dim3(256), 0, s, a);
+        else if (a.V <= 16 && a.k <= 8)
+            hipLaunchKernelGGL((distill_map_small_kernel<T, 16, 8>), grid, dim3(256), 0, s, a);
+        else if (a.V <= 32 && a.k <= 8)
+            hipLaunchKernelGGL((distill_map_small_kernel<T, 32, 8>), grid, dim3(256), 0, s, a);
+        else
+            hipLaunchKernelGGL((distill_map_kernel<T>), grid, dim3(256), (unsigned)(cdiv(a.V, 32) * 1024), s, a);
     } else if (a.V <= DW_MAX) {
         // up to 64 rows: one block of 16 waves, which also sums them
         const bool one = rows <= 64;
