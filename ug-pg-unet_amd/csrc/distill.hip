@@ -24,6 +24,7 @@ namespace ugpg {
 constexpr int DK_MAX = 256;              // entries of a record
 constexpr float NEG_INF = -__builtin_inff();
 constexpr double LOG2E = 1.4426950408889634074;
+constexpr double LN2 = 0.69314718055994530942;
 
 __device__ __forceinline__ float exp2_raw(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -217,7 +218,9 @@ __device__ __forceinline__ float distill_value(const DistillArgs& a, size_t at) 
 
 // What a row's k + 1 classes give (computed by one wave over entries in LDS), in fp64: a loss is
 // the difference of logarithms of nearly equal probabilities, and fp32 exponentials alone
-// put a single row's KL 2e-7 off.
+// put a single row's KL 2e-7 off.  1 / T is c * ln 2 with the rounded c that the rest's fp32
+// exponentials use: all parts share one temperature, 2^-24 beside the given one at most,
+// which moves the KL by as little of itself, not of 1.
 struct RowTerms {
     double kl;         // NaN / inf as they come out
     double M, m, iT;   // the teacher's and the student's maximum, 1 / T
@@ -233,10 +236,10 @@ struct RowTerms {
 
 // one wave; idx < 0: absent.  r: the student's rest
 __device__ __forceinline__ RowTerms row_terms(const int* idx, const float* t, const float* z, int k,
-                                              float rest, MaxSum r, double T) {
+                                              float rest, MaxSum r, float c) {
     const int lane = threadIdx.x & 63;
     RowTerms o;
-    o.iT = 1.0 / T;
+    o.iT = (double)c * LN2;
     float M = rest, m = r.m;
     for (int j = lane; j < k; j += 64)
         if (idx[j] >= 0) {
@@ -420,7 +423,7 @@ __device__ __forceinline__ void row_finish(const DistillArgs& a, int64_t r, MaxS
     const float w = a.weight ? a.weight[r] : 1.f;
     if (threadIdx.x < 64) {
         const float tr = a.rest ? a.rest[r] : NEG_INF;
-        const RowTerms o = row_terms(s.idx, s.t, s.z, a.k, tr, rest, a.T);
+        const RowTerms o = row_terms(s.idx, s.t, s.z, a.k, tr, rest, a.c);
         if (threadIdx.x == 0) {
             const bool none = o.empty || w == 0.f;
             const double l = none ? 0.0 : a.coef * a.T * a.T * (double)w * o.kl;
@@ -543,7 +546,7 @@ __device__ __forceinline__ double distill_wave_row(const DistillArgs& a, int64_t
     MaxSum rest = acc.done(a.c);
     rest.wave(a.c);
     const float tr = a.rest ? a.rest[r] : NEG_INF;
-    const RowTerms o = row_terms(s.idx, s.t, s.z, a.k, tr, rest, a.T);
+    const RowTerms o = row_terms(s.idx, s.t, s.z, a.k, tr, rest, a.c);
     const bool none = o.empty || w == 0.f;
     const double l = none ? 0.0 : a.coef * a.T * a.T * (double)w * o.kl;
     if (a.dz) {
@@ -620,7 +623,8 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
         const int64_t n = r / a.inner, p = r % a.inner;
         const T* z = static_cast<const T*>(a.logits) + (size_t)n * a.V * a.inner + p;
         const size_t rec = (size_t)n * a.k * a.inner + p;
-        const float c = a.c, iT = (float)(1.0 / a.T);
+        const float c = a.c;
+        const double iT = (double)c * LN2;  // (see RowTerms)
         float x[VR], t[KR], zj[KR];
         int idx[KR];
 #pragma unroll
@@ -672,18 +676,18 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
         for (int j = 0; j < KR; ++j) {
             eq[j] = ep[j] = 0.f;
             if (idx[j] >= 0) {
-                eq[j] = expf((t[j] - M) * iT);
-                ep[j] = expf((zj[j] - m) * iT);
+                eq[j] = exp2_raw((t[j] - M) * c);
+                ep[j] = exp2_raw((zj[j] - m) * c);
                 sq += eq[j];
                 ss += ep[j];
                 if (!(eq[j] == 0.f)) kl += (double)eq[j] * (((double)t[j] - M) - ((double)zj[j] - m));
             }
         }
-        kl /= a.T;
-        const float er = rest == NEG_INF ? 0.f : expf((rest - M) * iT);
-        const float sr = has ? rs.s * expf((rs.m - m) * iT) : rs.s;
+        kl *= iT;
+        const float er = rest == NEG_INF ? 0.f : exp2_raw((rest - M) * c);
+        const float sr = has ? rs.s * exp2_raw((rs.m - m) * c) : rs.s;
         if (!(er == 0.f))
-            kl += has ? (double)er * ((((double)rest - M) - ((double)rs.m - m)) / a.T - (double)logf(rs.s))
+            kl += has ? (double)er * ((((double)rest - M) - ((double)rs.m - m)) * iT - log((double)rs.s))
                       : (double)__builtin_inff();
         sq += er;
         ss += sr;
@@ -727,8 +731,6 @@ template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(
         for (int i = 0; i < nw; ++i) mine[256 * i] = 0;
         const float w = a.weight ? a.weight[r] : 1.f;
         const float rest = a.rest ? a.rest[r] : NEG_INF;
-        const float fT = (float)a.T;
-        const float iT = 1.f / fT;
         // kept classes: marks (an index seen before is absent), maxima
         float M = rest, m = NEG_INF;
         for (int j = 0; j < a.k; ++j) {
@@ -766,13 +768,13 @@ template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(
         };
         double sq = 0, ss = 0;
         entries(false, [&](int, float t, float zi) {
-            sq += expf((t - M) * iT);
-            ss += expf((zi - m) * iT);
+            sq += exp2_raw((t - M) * a.c);
+            ss += exp2_raw((zi - m) * a.c);
         });
-        const float er = rest == NEG_INF ? 0.f : expf((rest - M) * iT);
-        const double iTd = 1.0 / a.T;
+        const float er = rest == NEG_INF ? 0.f : exp2_raw((rest - M) * a.c);
+        const double iTd = (double)a.c * LN2;  // (see RowTerms)
         const double logr = has ? ((double)rs.m - (double)m) * iTd + log((double)rs.s) : (double)NEG_INF;
-        const float er_s = has ? rs.s * expf((rs.m - m) * iT) : rs.s;
+        const float er_s = has ? rs.s * exp2_raw((rs.m - m) * a.c) : rs.s;
         sq += er;
         ss += er_s;
         const double lq = log(sq), ls = log(ss), rsq = 1.0 / sq, rss = 1.0 / ss;
@@ -782,10 +784,10 @@ template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(
         T* d = static_cast<T*>(a.dz) + (a.dz ? (size_t)n * a.V * a.inner + p : 0);
         double kl = 0;
         entries(true, [&](int i, float t, float zi) {
-            const double q = (double)expf((t - M) * iT) * rsq;
+            const double q = (double)exp2_raw((t - M) * a.c) * rsq;
             if (!(q == 0.0))
                 kl += q * ((((double)t - (double)M) * iTd - lq) - (((double)zi - (double)m) * iTd - ls));
-            if (a.dz) d[(size_t)i * a.inner] = (T)(none ? 0.f : (float)(g * ((double)expf((zi - m) * iT) * rss - q)));
+            if (a.dz) d[(size_t)i * a.inner] = (T)(none ? 0.f : (float)(g * ((double)exp2_raw((zi - m) * a.c) * rss - q)));
         });
         const double qr = (double)er * rsq;
         if (!(qr == 0.0)) kl += qr * ((((double)rest - (double)M) * iTd - lq) - (logr - ls));
