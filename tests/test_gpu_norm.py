@@ -293,6 +293,53 @@ def test_other_stream_and_captured_graph(dev):
             assert all(torch.equal(a, c) for a, c in zip(outs, ex)), k
 
 
+def test_capture_beside_a_living_eager_graph_is_refused(dev):
+    """The leaves' accumulators then belong to the default stream, which a captured backward
+    may not touch; without the eager graph, or with it on another stream, capture works."""
+    import ugpg
+    x, w, b, dy = make((2, 12, 10, 64), 8, dev, torch.float32, "silu")
+    leaf = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    want = torch.autograd.grad(ugpg.group_norm_act(leaf[0], 8, *leaf[1:], activation="silu"), leaf, dy)
+    for which in range(3):
+        alive = leaf[which] * 1.0
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(RuntimeError, match="default stream"):
+                ugpg.group_norm_act(leaf[0], 8, *leaf[1:], activation="silu")
+            still = ugpg.group_norm_act(leaf[0].detach(), 8, *(t.detach() for t in leaf[1:]), activation="silu")
+        del alive
+        graph.replay()
+        assert torch.isfinite(still).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = ugpg.group_norm_act(leaf[0], 8, *leaf[1:], activation="silu")
+        got = torch.autograd.grad(y, leaf, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("C,G", [(64, 8), (16, 1), (4, 4)])
+def test_a_chunk_far_from_the_others(dev, C, G):
+    """The first pixels of each group's first channel lie 10^4 away from all other values, which
+    are equal: the partials' merge must not lose these others' digits.  An output is
+    (x - mean) * rstd; mean and rstd are within a few dozen roundings of themselves (a share's
+    sums, each about its own first mean), which against x - mean makes EPS32 of
+    |x - mean| * rstd + |mean error| * rstd, mean error <= EPS32 * (|mean - x| + |x|)."""
+    import ugpg
+    x = torch.full((1, 128, 128, C), 0.5, device=dev)
+    x[:, 0, :, ::C // G] = 1.0e4
+    y = ugpg.group_norm_act(x, G, activation="none")
+    xd = x.double().reshape(1, -1, G, C // G)
+    mean = xd.mean((1, 3), keepdim=True)
+    rstd = ((xd - mean) ** 2).mean((1, 3), keepdim=True).add(1e-5).rsqrt()
+    want = ((xd - mean) * rstd).reshape(x.shape)
+    lim = EPS32 * (((xd - mean).abs() + (xd - mean).abs() + xd.abs()) * rstd).reshape(x.shape)
+    err = (y.double() - want).abs()
+    assert (err <= lim).all(), (err / lim).max().item()
+
+
 def test_differentiable_once(dev):
     """Second derivatives are refused, not silently left out; create_graph alone is fine."""
     import ugpg

@@ -199,12 +199,12 @@ __global__ void __launch_bounds__(256) gn_merge_kernel(const float* part, GnGeom
 }
 
 // Group sums of two per-channel quantities: `each(c, first, step)` gives the caller's share of
-// channel c over the partials first, first + step, ... (fp32, a few dozen terms at most); L
-// lanes a group add the shares in fp64, in a fixed order.  Every thread of the block calls it;
-// the sums are in f->gs.  (Shares in fp64 cost every block of the second pass 10 us where
+// channel c over the partials first, first + step, ... (a few dozen at most, summed in fp32); L lanes a
+// group add the shares in fp64, in a fixed order.  Every thread of the block calls it; the
+// sums are in f->gs.  (Sums of a share in fp64 cost every block of the second pass 10 us where
 // 1024 blocks merge 64 chunks of 128 channels.)
 struct GnFold {
-    float red[2][GN_NT];
+    double red[2][GN_NT];
     double gs[2][GN_FG];
 };
 template <typename F>
@@ -214,8 +214,8 @@ __device__ __forceinline__ void gn_fold(const GnGeom& g, GnFold* f, F each) {
     for (int k = t; k < g.G; k += GN_NT) f->gs[0][k] = f->gs[1][k] = 0;
     for (int c0 = 0; c0 < g.C; c0 += ct) {
         const int cl = t % ct, pi = t / ct, c = c0 + cl;
-        float a = 0.f, b = 0.f;
-        if (pi < parts && c < g.C) each(c, pi, parts, a, b);
+        double a = 0, b = 0;
+        if (pi < parts && pi < g.nchunk && c < g.C) each(c, pi, parts, a, b);
         f->red[0][t] = a;
         f->red[1][t] = b;
         __syncthreads();
@@ -271,17 +271,25 @@ __global__ void __launch_bounds__(GN_NT) gn_apply_kernel(const T* x, GnGeom g, c
     }
     if (g.fold) {
         const float* pb = part + (size_t)q.b * g.nchunk * 2 * g.C;
-        gn_fold(g, f, [&](int c, int first, int step, float& s, float& v) {
-            // about the group's first mean: the squares cancel nothing
-            const float ref = pb[c / g.cpg * g.cpg];
-            const float whole = (float)g.ppc, last = (float)(g.P - (int64_t)(g.nchunk - 1) * g.ppc);
+        gn_fold(g, f, [&](int c, int first, int step, double& s, double& v) {
+            // a share about its own first mean, then about the group's: a chunk far from the
+            // others must not cost the others their digits
+            const float own = pb[(size_t)first * 2 * g.C + c];
+            const int64_t rest = g.P - (int64_t)(g.nchunk - 1) * g.ppc;
+            const float whole = (float)g.ppc, last = (float)rest;
+            float fs = 0.f, fv = 0.f;
 #pragma unroll 8
             for (int ch = first; ch < g.nchunk; ch += step) {
                 const float np = ch == g.nchunk - 1 ? last : whole;
-                const float d = pb[(size_t)ch * 2 * g.C + c] - ref;
-                s = fmaf(np, d, s);
-                v += fmaf(np * d, d, pb[((size_t)ch * 2 + 1) * g.C + c]);
+                const float d = pb[(size_t)ch * 2 * g.C + c] - own;
+                fs = fmaf(np, d, fs);
+                fv += fmaf(np * d, d, pb[((size_t)ch * 2 + 1) * g.C + c]);
             }
+            const int m = (g.nchunk - 1 - first) / step;  // chunks before the share's last
+            const double n = (double)m * g.ppc + (first + m * step == g.nchunk - 1 ? rest : g.ppc);
+            const double e = (double)own - pb[c / g.cpg * g.cpg];
+            s = fs + n * e;
+            v = fv + e * (2.0 * fs + n * e);
         });
         const double cnt = (double)g.P * g.cpg;
         for (int k = threadIdx.x; k < g.G; k += GN_NT) {
@@ -555,15 +563,16 @@ __global__ void __launch_bounds__(GN_NT) gn_bwd_apply_kernel(
     }
     if (g.fold) {
         const float* pb = part + (size_t)q.b * g.nchunk * 2 * g.C;
-        gn_fold(g, f, [&](int c, int first, int step, float& s, float& t) {
+        gn_fold(g, f, [&](int c, int first, int step, double& s, double& t) {
+            float a = 0.f, b = 0.f;
 #pragma unroll 8
             for (int ch = first; ch < g.nchunk; ch += step) {
-                s += pb[(size_t)ch * 2 * g.C + c];
-                t += pb[((size_t)ch * 2 + 1) * g.C + c];
+                a += pb[(size_t)ch * 2 * g.C + c];
+                b += pb[((size_t)ch * 2 + 1) * g.C + c];
             }
-            const float w = gamma ? gamma[c] : 1.f;
-            s *= w;
-            t *= w;
+            const double w = gamma ? gamma[c] : 1.f;
+            s = w * a;
+            t = w * b;
         });
     }
     if (!q.on) return;
@@ -939,8 +948,8 @@ static int gn_check(const char* what, const ugpg_group_norm_t* p, bool tensors) 
                   p->dtype, p->B, (long long)p->HW, p->C, p->G, (double)p->eps, p->act);
         return UGPG_ERR_INVALID;
     }
-    if (tensors && (!p->x || !p->mean || !p->rstd)) {
-        set_error("%s: x, mean and rstd must be given", what);
+    if (tensors && (!p->x || !p->mean || !p->rstd || (uintptr_t)p->x % (p->dtype == UGPG_DT_F32 ? 4 : 2))) {
+        set_error("%s: x, mean and rstd must be given, x aligned to its type", what);
         return UGPG_ERR_INVALID;
     }
     // (grids: B*G blocks, B * column blocks; offsets are 64-bit)
@@ -1023,8 +1032,8 @@ static int gn_ws_check(const char* what, const ugpg_group_norm_t* p, int backwar
 extern "C" int ugpg_group_norm_fwd(const ugpg_group_norm_t* p, void* y, void* ws, size_t ws_bytes,
                                    void* stream) {
     if (int rc = gn_check("group_norm_fwd", p, true)) return rc;
-    if (!y) {
-        set_error("group_norm_fwd: no output");
+    if (!y || (uintptr_t)y % (p->dtype == UGPG_DT_F32 ? 4 : 2)) {
+        set_error("group_norm_fwd: no output, or not aligned to its type");
         return UGPG_ERR_INVALID;
     }
     if (int rc = gn_ws_check("group_norm_fwd", p, 0, ws, ws_bytes)) return rc;
@@ -1095,8 +1104,9 @@ extern "C" int ugpg_group_norm_bwd(const ugpg_group_norm_t* p, const void* dy, i
     const bool hhh = dtype == H && dy_dtype == H && dx_dtype == H;
     const bool hfh = dtype == H && dy_dtype == F && dx_dtype == H;
     const bool hff = dtype == H && dy_dtype == F && dx_dtype == F;
-    if (!dy || !dx || !(fff || hhh || hfh || hff)) {
-        set_error("group_norm_bwd: bad arguments (x, dy, dx types %d %d %d)", dtype, dy_dtype,
+    if (!dy || !dx || !(fff || hhh || hfh || hff) || (uintptr_t)dy % (dy_dtype == F ? 4 : 2) ||
+        (uintptr_t)dx % (dx_dtype == F ? 4 : 2)) {
+        set_error("group_norm_bwd: bad arguments or alignment (x, dy, dx types %d %d %d)", dtype, dy_dtype,
                   dx_dtype);
         return UGPG_ERR_INVALID;
     }

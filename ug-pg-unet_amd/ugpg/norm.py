@@ -45,6 +45,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
         raise RuntimeError("ugpg: tensor is not on a ROCm/HIP device (no CPU fallback)")
     if x.numel() == 0:
         raise ValueError(f"group_norm_act: empty input {tuple(x.shape)}")
+    if x.shape[0] > 1 << 30 or c > 1 << 20:
+        raise ValueError(f"group_norm_act: {x.shape[0]} samples of {c} channels are too many")
     if not x.is_contiguous():
         x = x.contiguous()
     if weight is not None and not weight.is_contiguous():
