@@ -15,6 +15,7 @@ def test_top_logits_refuses_bad_arguments():
                            ((z, 2.0), ValueError, "k must"), ((torch.zeros(2, 999), 257), ValueError, "k must"),
                            ((z, 3, 0.0), ValueError, "temperature"), ((z, 3, -1.0), ValueError, "temperature"),
                            ((z, 3, float("nan")), ValueError, "temperature"),
+                           ((z, 3, 1e-31), ValueError, "temperature"), ((z, 3, 1e31), ValueError, "temperature"),
                            ((z, 3), RuntimeError, "no CPU fallback")]:
         with pytest.raises(err, match=msg):
             ugpg.teacher_top_logits(*args)
@@ -73,7 +74,8 @@ def test_c_entries_refuse_before_any_launch():
         f.update(kw)
         return _C.DistillDesc(*f.values())
     for kw in (dict(logits=None), dict(dtype=3), dict(values=None), dict(indices=None), dict(values_dtype=2),
-               dict(index_bits=16), dict(k=0), dict(temperature=-1.0), dict(scale=float("nan")), dict(stride=3),
+               dict(index_bits=16), dict(k=0), dict(temperature=-1.0),
+               dict(temperature=1e-31), dict(temperature=2e30), dict(scale=float("nan")), dict(stride=3),
                dict(inner=2, V=1025, stride=2050, k=3)):
         d = desc(**kw)
         assert lib.ugpg_distill_workspace(C.byref(d), 0) == 0
@@ -89,7 +91,11 @@ def test_c_entries_refuse_before_any_launch():
         if nb:
             assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, p, p, nb - 1, None) == -3
             assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, p, None, nb, None) == -3
+    d = desc(N=1 << 22, V=1 << 30, stride=1 << 30)  # more blocks than a grid takes
+    assert lib.ugpg_distill_workspace(C.byref(d), 0) == 0
     d = desc()
+    assert lib.ugpg_distill_fwd(C.byref(d), p, None, p + 2, p, 1 << 20, None) == -1
+    assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, p + 2, p, 1 << 20, None) == -1
     assert lib.ugpg_distill_fwd(C.byref(d), None, None, None, p, 1 << 20, None) == -1
     assert lib.ugpg_distill_bwd(C.byref(d), None, 0, 0, p, p, 1 << 20, None) == -1
     assert lib.ugpg_distill_bwd(C.byref(d), p, 0, 0, None, p, 1 << 20, None) == -1

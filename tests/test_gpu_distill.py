@@ -375,6 +375,21 @@ def test_confident_rows_keep_their_rest(dev):
         assert (dz[:, rest] != 0).all() and (zr.grad[:, rest] != 0).all()
 
 
+def test_many_short_rows(dev):
+    """More rows than the waves in flight: every block steps over several."""
+    import ugpg
+    for shape, k in (((200003, 7), 3), ((140001, 33), 5)):
+        z, v, i, r, w = record(shape, k, dev, F32, 2.0, seed=19)
+        rows, dz, size, unit = ref_loss(z, v, i, r, w, 2.0, 1.0 / shape[0])
+        zr = z.clone().requires_grad_(True)
+        loss = ugpg.distillation_loss(zr, (v, i, r), 2.0, weight=w)
+        check_loss(loss, rows, unit)
+        loss.backward()
+        check_grad(zr.grad, dz, size)
+        out = ugpg.distillation_loss(z, (v, i, r), 2.0, weight=w, reduction="none")
+        assert ((out.double() - rows * shape[0]).abs() <= REL * unit * shape[0] + 2.0 ** -23 * out.double().abs()).all()
+
+
 def test_strides_alignment_and_mixed_types(dev):
     import ugpg
     for dtype in (F32, BF16):
@@ -473,6 +488,29 @@ def test_other_stream_and_captured_graph(dev):
             torch.cuda.synchronize()
             ex = step(x.detach().clone().requires_grad_(True), t.clone())
             assert all(torch.equal(a, b) for a, b in zip(outs, ex)), n
+
+
+def test_capture_beside_a_living_eager_graph_is_refused(dev):
+    import ugpg
+    z, v, i, r, w = record((70, 33), 5, dev, F32, 2.0, seed=23)
+    leaf = z.clone().requires_grad_(True)
+    want = torch.autograd.grad(ugpg.distillation_loss(leaf, (v, i, r), 2.0), leaf)[0]
+    alive = leaf * 1.0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="default stream"):
+            ugpg.distillation_loss(leaf, (v, i, r), 2.0)
+        still = ugpg.distillation_loss(leaf.detach(), (v, i, r), 2.0)
+    del alive
+    graph.replay()
+    assert torch.isfinite(still)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ugpg.distillation_loss(leaf, (v, i, r), 2.0), leaf)[0]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
 
 
 def test_offsets_past_32_bits(dev):

@@ -7,6 +7,7 @@
 // elementwise product and its gradient).  These nodes keep Python out of the backward.
 // Arguments are checked by the Python callers (ugpg/norm.py, ugpg/distill.py); the entries are
 // bound at import by address, so this module runs the very library ugpg._C loaded.
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -56,6 +57,20 @@ const float* floats(const Maybe& t) { return t.has_value() && t->defined() ? t->
 Maybe some(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 Tensor scratch(size_t bytes, const Tensor& like) {
     return torch::empty({(int64_t)bytes}, like.options().dtype(torch::kByte));
+}
+
+// A graph capture must not take in a node of the default stream: its backward would make that
+// stream, which cannot be captured, wait on the captured one, and the process ends.  An
+// input's node, or a leaf's accumulator while an eager graph of the same leaf lives, is one.
+void check_capture(const char* what, std::initializer_list<const Tensor*> inputs) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    for (const Tensor* t : inputs) {
+        if (!t->defined() || !t->requires_grad()) continue;
+        const auto node = t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto s = node ? node->stream() : std::nullopt;
+        TORCH_CHECK(!s || s->id() != 0, what, ": captured while a graph of the same input lives on the "
+                    "default stream; drop that graph first, or run it on another stream");
+    }
 }
 
 // The gradients of a backward that runs with create_graph: differentiating through one of them
@@ -119,6 +134,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     static variable_list backward(AutogradContext* ctx, variable_list up) {
         const variable_list s = ctx->get_saved_variables();  // (raises if one was written in place since)
         const Tensor &x = s[0], &w = s[1], &b = s[2];
+        c10::OptionalDeviceGuard guard(x.device());
         const Tensor dy = up[0].detach().to(x.scalar_type()).contiguous();
         const ugpg_group_norm_t d = gn_desc(x, ctx->saved_data["groups"].toInt(), some(w), some(b), 0.0,
                                             ctx->saved_data["act"].toInt(), s[3]);
@@ -139,12 +155,14 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
     }
 };
 
-bool wants(const Tensor& t) { return t.defined() && t.requires_grad(); }
+bool wants(const Maybe& t) { return t.has_value() && t->defined() && t->requires_grad(); }
 
 Tensor group_norm_act(const Tensor& x, const Maybe& w, const Maybe& b, int64_t groups, double eps, int64_t act) {
-    if (c10::GradMode::is_enabled() &&
-        (wants(x) || wants(w.value_or(Tensor())) || wants(b.value_or(Tensor()))))
+    if (c10::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) {
+        const Tensor none;
+        check_capture("group_norm_act", {&x, w ? &*w : &none, b ? &*b : &none});
         return GroupNormAct::apply(x, w, b, groups, eps, act);
+    }
     Tensor stats;
     c10::AutoGradMode off(false);
     return gn_forward(x, groups, w, b, eps, act, stats);
@@ -220,6 +238,7 @@ struct Distill : torch::autograd::Function<Distill> {
     static variable_list backward(AutogradContext* ctx, variable_list up) {
         const variable_list s = ctx->get_saved_variables();  // (raises if one was written in place since)
         const Tensor& logits = s[0];
+        c10::OptionalDeviceGuard guard(logits.device());
         const Tensor z = class_rows(logits.detach());
         const ugpg_distill_t d = ds_desc(logits, z, s[1], s[2], some(s[3]), some(s[4]),
                                          ctx->saved_data["T"].toDouble(), ctx->saved_data["scale"].toDouble());
@@ -246,8 +265,10 @@ struct Distill : torch::autograd::Function<Distill> {
 
 Tensor distill(const Tensor& logits, const Tensor& values, const Tensor& indices, const Maybe& rest,
                const Maybe& weight, double T, double scale, bool per_row) {
-    if (c10::GradMode::is_enabled() && logits.requires_grad())
+    if (c10::GradMode::is_enabled() && logits.requires_grad()) {
+        check_capture("distillation_loss", {&logits});
         return Distill::apply(logits, values, indices, rest, weight, T, scale, per_row);
+    }
     c10::AutoGradMode off(false);
     return ds_forward(logits, values, indices, rest, weight, T, scale, per_row, nullptr);
 }

@@ -492,6 +492,14 @@ __global__ void __launch_bounds__(256) distill_join_kernel(DistillArgs a, int sp
     if (a.dz) row_grad<T, ALIGNED>(a, r, sp, s);
 }
 
+// the sum of the waves' losses -> row_loss[block] (256 threads)
+__device__ __forceinline__ void block_loss(const DistillArgs& a, double l) {
+    __shared__ double red[4];
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = l;
+    __syncthreads();
+    if (threadIdx.x == 0 && a.row_loss) a.row_loss[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
+}
+
 // ---------------------------------------------------------------- short rows, a wave each
 constexpr int DW_MAX = 512;  // classes
 struct WaveShared {
@@ -588,29 +596,21 @@ __global__ void __launch_bounds__(1024) distill_wave_one_kernel(DistillArgs a, f
         loss[0] = (float)acc;
     }
 }
+// the blocks step over the rows; row_loss: a block's sum
 template <typename T, int NV>
 __global__ void __launch_bounds__(256) distill_wave_kernel(DistillArgs a) {
     __shared__ WaveShared s[4];
     if (distill_skip(a)) return;
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    if (r >= a.rows) return;
-    const double l = distill_wave_row<T, NV>(a, r, s[threadIdx.x / 64]);
-    if ((threadIdx.x & 63) == 0) {
-        if (a.row_loss) a.row_loss[r] = l;
-        if (a.row_out) a.row_out[r] = (float)l;
+    double acc = 0;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; r < a.rows; r += (int64_t)gridDim.x * 4) {
+        const double l = distill_wave_row<T, NV>(a, r, s[threadIdx.x / 64]);
+        if (a.row_out && (threadIdx.x & 63) == 0) a.row_out[r] = (float)l;
+        acc += l;
     }
+    block_loss(a, acc);
 }
 
 // ---------------------------------------------------------------- class maps, a thread each
-// the sum of a block's losses -> row_loss[block]
-__device__ __forceinline__ void map_sum(const DistillArgs& a, double l) {
-    __shared__ double red[4];
-    l = wave_sum_d(l);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x / 64] = l;
-    __syncthreads();
-    if (threadIdx.x == 0 && a.row_loss) a.row_loss[blockIdx.x] = red[0] + red[1] + red[2] + red[3];
-}
-
 // At most VR classes and KR entries: a pixel's logits and record stay in registers, read once.
 // Exponentials are fp32 here (a map's loss is a mean over its pixels), sums and differences
 // fp64.  16 maps of 8 x 256^2 fp32 at 3 entries, with the gradient: 34 us against 55 for the form
@@ -713,7 +713,7 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
             }
         }
     }
-    map_sum(a, l);
+    block_loss(a, wave_sum_d(l));
 }
 
 constexpr int DM_MAX = 1024;  // classes
@@ -806,12 +806,13 @@ template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(
             }
         }
     }
-    map_sum(a, l);
+    block_loss(a, wave_sum_d(l));
 }
 
 __global__ void __launch_bounds__(1024) distill_sum_kernel(const double* part, int64_t n, float* loss) {
     __shared__ double s[16];
     double acc = 0;
+#pragma unroll 16
     for (int64_t i = threadIdx.x; i < n; i += 1024) acc += part[i];
     acc = wave_sum_d(acc);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x / 64] = acc;
@@ -1246,7 +1247,7 @@ template <typename T, int VR> __global__ void __launch_bounds__(256) top_map_ker
 static int rows_check(const char* what, const void* logits, int dtype, int64_t N, int V, int64_t inner,
                       int64_t stride, int k, double T) {
     if (!logits || (dtype != UGPG_DT_F32 && dtype != UGPG_DT_BF16) || N <= 0 || V <= 0 || inner <= 0 ||
-        k < 1 || k > V || !(T > 0.0) || !(T < 1e30)) {
+        k < 1 || k > V || !(T >= 9e-31) || !(T <= 1.1e30)) {
         set_error("%s: bad arguments (dtype=%d N=%lld V=%d inner=%lld k=%d T=%g)", what, dtype,
                   (long long)N, V, (long long)inner, k, T);
         return UGPG_ERR_INVALID;
@@ -1330,6 +1331,12 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
     return check_launch("top_logits");
 }
 
+// blocks of four waves for short rows: up to 16 rounds of the card's 2048
+static int64_t wave_blocks(int64_t rows) {
+    const int64_t n = cdiv(rows, 4);
+    return n < 32768 ? n : 32768;
+}
+
 static int distill_check(const char* what, const ugpg_distill_t* p) {
     if (!p) {
         set_error("%s: no descriptor", what);
@@ -1341,6 +1348,10 @@ static int distill_check(const char* what, const ugpg_distill_t* p) {
         (p->index_bits != 32 && p->index_bits != 64) || !(p->scale == p->scale)) {
         set_error("%s: bad record (values type %d, %d-bit indices) or scale %g", what, p->values_dtype,
                   p->index_bits, p->scale);
+        return UGPG_ERR_INVALID;
+    }
+    if (p->inner == 1 && p->V > DW_MAX && (double)p->N * row_split(p->N, p->V).n * 512 > 4e9) {
+        set_error("%s: N=%lld V=%d is too large", what, (long long)p->N, p->V);
         return UGPG_ERR_INVALID;
     }
     if (p->inner > 1 && p->V > DM_MAX) {
@@ -1383,12 +1394,13 @@ static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, bool
         // up to 64 rows: one block of 16 waves, which also sums them
         const bool one = rows <= 64;
         const int nv = (int)cdiv(a.V, 64);
+        if (!one) nsum = wave_blocks(rows);
 #define DISTILL_WAVE(NV)                                                                          \
     do {                                                                                          \
         if (one)                                                                                  \
             hipLaunchKernelGGL((distill_wave_one_kernel<T, NV>), dim3(1), dim3(1024), 0, s, a, loss); \
         else                                                                                      \
-            hipLaunchKernelGGL((distill_wave_kernel<T, NV>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a); \
+            hipLaunchKernelGGL((distill_wave_kernel<T, NV>), dim3((unsigned)nsum), dim3(256), 0, s, a);   \
     } while (0)
         if (nv <= 1) DISTILL_WAVE(1);
         else if (nv <= 4) DISTILL_WAVE(4);
@@ -1465,8 +1477,8 @@ static int distill_ws_check(const char* what, const ugpg_distill_t* p, int backw
 extern "C" int ugpg_distill_fwd(const ugpg_distill_t* p, float* loss, float* row_loss, void* dlogits,
                                 void* ws, size_t ws_bytes, void* stream) {
     if (int rc = distill_check("distill_fwd", p)) return rc;
-    if (!loss && !row_loss) {
-        set_error("distill_fwd: neither loss nor row_loss given");
+    if ((!loss && !row_loss) || (uintptr_t)dlogits % (p->dtype == UGPG_DT_F32 ? 4 : 2)) {
+        set_error("distill_fwd: neither loss nor row_loss given, or dlogits not aligned to its type");
         return UGPG_ERR_INVALID;
     }
     if (int rc = distill_ws_check("distill_fwd", p, 0, ws, ws_bytes)) return rc;
@@ -1480,7 +1492,7 @@ extern "C" int ugpg_distill_fwd(const ugpg_distill_t* p, float* loss, float* row
 extern "C" int ugpg_distill_bwd(const ugpg_distill_t* p, const float* gout, int per_row, int skip_one,
                                 void* dlogits, void* ws, size_t ws_bytes, void* stream) {
     if (int rc = distill_check("distill_bwd", p)) return rc;
-    if (!gout || !dlogits || (per_row && skip_one)) {
+    if (!gout || !dlogits || (per_row && skip_one) || (uintptr_t)dlogits % (p->dtype == UGPG_DT_F32 ? 4 : 2)) {
         set_error("distill_bwd: bad arguments (per_row=%d skip_one=%d)", per_row, skip_one);
         return UGPG_ERR_INVALID;
     }

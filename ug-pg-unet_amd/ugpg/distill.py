@@ -33,11 +33,13 @@ def _check_logits(what, logits):
         raise TypeError(f"{what}: logits must be float32 or bfloat16, got {logits.dtype}")
     if logits.numel() == 0:
         raise ValueError(f"{what}: empty logits {tuple(logits.shape)}")
+    if logits.shape[1] > 1 << 30:
+        raise ValueError(f"{what}: {logits.shape[1]} classes are too many")
 
 
 def _check_temperature(what, t):
-    if not 0.0 < float(t) < 1e30:
-        raise ValueError(f"{what}: temperature must be positive, got {t}")
+    if not 1e-30 <= float(t) <= 1e30:
+        raise ValueError(f"{what}: temperature must lie in 1e-30..1e30, got {t}")
 
 
 def _check_device(what, logits):
