@@ -37,6 +37,30 @@ def test_module_refuses_bad_arguments():
     assert sorted(m.state_dict()) == ["bias", "weight"]
 
 
+def test_checkpoints_of_group_norm_models_name_their_groups(tmp_path):
+    """The group count is no part of a state_dict: it is recorded, given, or refused."""
+    import ugpg
+    state = ugpg.PGUNet1(3, 1, norm="group", groups=8).state_dict()
+    bare, full = tmp_path / "bare.pth", tmp_path / "full.pth"
+    torch.save({"model_state_dict": state, "stage": 1}, bare)
+    torch.save({"model_state_dict": state, "stage": 1, "norm_groups": 8}, full)
+    for path, groups in ((full, None), (full, 8), (bare, 8)):
+        t = ugpg.MoNuSegTester(str(path), device="cpu", norm_groups=groups)
+        assert t.model.inc.conv.conv_op[1].num_groups == 8
+    for path, groups in ((bare, None), (full, 16)):
+        with pytest.raises(RuntimeError, match="norm_groups"):
+            ugpg.MoNuSegTester(str(path), device="cpu", norm_groups=groups)
+    tr = ugpg.UncertaintyGuidedProgressiveTrainer(3, 1, device="cpu", norm="group", norm_groups=16)
+    with pytest.raises(ValueError, match="8 norm groups"):
+        tr.load_stage_weights(1, str(full))
+
+
+def test_one_logit_cannot_be_distilled():
+    from ugpg.herlev import HerlevTrainer
+    with pytest.raises(ValueError, match="at least 2 classes"):
+        HerlevTrainer({"num_classes": 1, "epochs_per_stage": 1, "distill_weight": 0.5, "device": "cpu"})
+
+
 def test_c_entries_refuse_before_any_launch():
     import ctypes as C
     from ugpg import _C
@@ -50,7 +74,7 @@ def test_c_entries_refuse_before_any_launch():
              dict(eps=float("nan")), dict(act=3), dict(act=-1), dict(C=1 << 21, G=1), dict(B=1 << 22, G=8),
              dict(HW=1 << 41))
     big = 1 << 40
-    for kw in (*sizes, dict(x=None), dict(mean=None), dict(rstd=None)):
+    for kw in (*sizes, dict(x=None), dict(x=p + 2), dict(mean=None), dict(rstd=None)):
         assert lib.ugpg_group_norm_fwd(desc(**kw), p, p, big, None) == -1, kw
         assert b"group_norm_fwd" in lib.ugpg_last_error()
         assert lib.ugpg_group_norm_bwd(desc(**kw), p, kw.get("dtype", 0), p, kw.get("dtype", 0), None, None,

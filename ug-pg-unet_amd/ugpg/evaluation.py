@@ -66,10 +66,15 @@ def calculate_metrics(pred_mask, gt_mask) -> Dict[str, float]:
 
 
 class MoNuSegTester:
-    """Evaluation driver with the reference's model loading and metric reporting."""
+    """Evaluation driver with the reference's model loading and metric reporting.
 
-    def __init__(self, model_path: str | None = None, device="cuda", model: nn.Module | None = None):
+    norm_groups: the groups of a model trained with norm="group", where its checkpoint does
+    not say (the trainer's checkpoints do)."""
+
+    def __init__(self, model_path: str | None = None, device="cuda", model: nn.Module | None = None,
+                 norm_groups: int | None = None):
         self.device = torch.device(device)
+        self.norm_groups = norm_groups
         if model is None and model_path is None:
             raise ValueError("MoNuSegTester needs model_path or model")
         self.model = model.to(self.device) if model is not None else self.load_model(model_path)
@@ -87,10 +92,13 @@ class MoNuSegTester:
         else:
             raise RuntimeError(f"Unrecognized checkpoint format for: {model_path}")
         # a model without running statistics was trained with norm="group"
-        group = not any(k.endswith("running_mean") for k in state)
-        model = _STAGE_MODELS.get(stage, PGUNet4)(in_channels=3, num_classes=1,
-                                                  norm="group" if group else "batch",
-                                                  groups=int(ckpt.get("norm_groups", 32)) if group else 32)
+        norm, groups = "batch", 32
+        if not any(k.endswith("running_mean") for k in state):
+            norm, groups = "group", ckpt.get("norm_groups", self.norm_groups)
+            if groups is None or (self.norm_groups or groups) != groups:
+                raise RuntimeError(f"{model_path} holds a group-norm model of {groups or 'unknown'} groups: "
+                                   f"give norm_groups (given: {self.norm_groups})")
+        model = _STAGE_MODELS.get(stage, PGUNet4)(in_channels=3, num_classes=1, norm=norm, groups=int(groups))
         model.load_state_dict(state)
         self.stage = stage
         return model.to(self.device)

@@ -197,6 +197,14 @@ class HerlevTrainer:
         self.config = config
         self.device = config["device"]
         e = config["epochs_per_stage"]
+        scale = float(config.get("distill_weight", 0.0))
+        self.distillation = None
+        if scale != 0.0:
+            if config["num_classes"] < 2:
+                raise ValueError("distill_weight needs at least 2 classes (one logit has no distribution)")
+            self.distillation = DistillationLoss(
+                min(int(config.get("distill_top", 3)), config["num_classes"]),
+                float(config.get("distill_temperature", 2.0)), scale)
         res4 = config.get("stage4_resolution", 224)
         self.stage_configs = {1: {"resolution": 32, "epochs": e, "lr": 3e-4},
                               2: {"resolution": 64, "epochs": e, "lr": 1e-4},
@@ -213,12 +221,6 @@ class HerlevTrainer:
         self.setup_loss_function()
         self.uncertainty_loss = UncertaintyGuidedLoss(self.device)
         self.uncertainty_alpha = config.get("uncertainty_alpha", 1.0)
-        scale = float(config.get("distill_weight", 0.0))
-        self.distillation = None
-        if scale != 0.0:
-            self.distillation = DistillationLoss(
-                min(int(config.get("distill_top", 3)), config["num_classes"]),
-                float(config.get("distill_temperature", 2.0)), scale)
         self.history = {k: [] for k in ("train_loss", "val_loss", "train_acc", "val_acc",
                                         "uncertainty_weights_mean", "uncertainty_weights_std",
                                         "base_loss", "stage_transitions")}

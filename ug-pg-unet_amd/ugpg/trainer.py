@@ -440,6 +440,10 @@ class UncertaintyGuidedProgressiveTrainer:
         models[stage] (uncertainty_guided_trainer.py:469-473).  COLLECTIVE under data
         parallelism: every rank calls it, then rank 0's weights are broadcast."""
         ck = torch.load(checkpoint_path, map_location=self.device, weights_only=True)
+        groups = ck.get("norm_groups")
+        if groups is not None and groups != self.norm_groups:
+            raise ValueError(f"{checkpoint_path} was trained with {groups} norm groups, this trainer "
+                             f"has {self.norm_groups}")
         self.models[stage].load_state_dict(ck["model_state_dict"] if "model_state_dict" in ck else ck)
         self.sync_replicas([stage])
         print(f"Loaded weights for stage {stage} from {checkpoint_path}")
