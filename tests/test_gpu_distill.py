@@ -163,6 +163,45 @@ def test_top_logits(dev, dtype, kind):
             assert ok.all(), (shape, k, top.rest[~ok][:3], r[~ok][:3])
 
 
+@pytest.mark.parametrize("shape,k", [((2, 20, 300, 240), 6), ((2, 24, 270, 250), 20), ((1, 100, 37, 41), 2),
+                                     ((3, 70, 8, 9), 4), ((1, 1000, 5, 13), 5), ((1, 5000, 3, 5), 9),
+                                     ((1, 35, 1, 2), 35)])
+def test_top_logits_of_maps(dev, shape, k):
+    """One thread or four a pixel, one reading or several."""
+    import ugpg
+    for kind in ("random", "ties", "equal", "ascending", "masked", "nan", "inf"):
+        z = fill(kind, shape, dev, F32 if kind != "ties" else BF16, seed=5)
+        top = ugpg.teacher_top_logits(z, k, 1.5)
+        v, i, r = ref_top(z, k, 1.5)
+        assert torch.equal(top.indices, i), kind
+        assert torch.equal(top.values.double().nan_to_num(7e7), v.nan_to_num(7e7)), kind
+        same = (top.rest.double() == r) | (top.rest.isnan() & r.isnan())
+        assert (same | ((top.rest.double() - r).abs() <= 1.5 * REL + 2.0 ** -23 * r.abs())).all(), kind
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,k", [((2, 16, 19, 21), 12), ((1, 40, 65, 3), 5), ((3, 257, 7, 11), 100),
+                                     ((1, 1024, 3, 23), 256), ((2, 64, 128, 128), 8)])
+def test_loss_of_maps_in_parts(dev, shape, k, dtype):
+    """Four threads a pixel; entries absent, repeated, and rows without weight among them."""
+    import ugpg
+    z, v, i, r, w = record(shape, k, dev, dtype, 2.0, seed=k)
+    i = i.clone()
+    i[:, 1, ::2] = -1
+    if k <= 16:
+        i[:, 3, :, ::3] = i[:, 0, :, ::3]
+    w = w.clone()
+    w[..., ::5] = 0.0
+    rows, dz, size, unit = ref_loss(z, v, i, r, w, 2.0, 1.0)
+    zr = z.clone().requires_grad_(True)
+    loss = ugpg.distillation_loss(zr, (v, i, r), 2.0, weight=w, reduction="sum")
+    check_loss(loss, rows, unit)
+    loss.backward()
+    check_grad(zr.grad, dz, size)
+    out = ugpg.distillation_loss(z, (v, i, r), 2.0, weight=w, reduction="none")
+    assert ((out.double() - rows).abs() <= REL * unit + 2.0 ** -23 * rows.abs()).all()
+
+
 def test_top_logits_strides_and_alignment(dev):
     import ugpg
     for dtype in (F32, BF16):

@@ -716,95 +716,157 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
     block_loss(a, wave_sum_d(l));
 }
 
+// More classes or entries: 64 pixels a block, the classes in four parts, a wave each; the first
+// wave reads the record and joins the parts.  Marks of the kept classes lie in LDS.
 constexpr int DM_MAX = 1024;  // classes
-template <typename T> __global__ void __launch_bounds__(256) distill_map_kernel(DistillArgs a) {
-    extern __shared__ uint32_t bits[];  // [ceil(V / 32)][256]
+template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map_kernel(DistillArgs a) {
+    extern __shared__ uint32_t bits[];  // [ceil(V / 32)][64]
+    __shared__ float sm[256], ss[256];
     if (distill_skip(a)) return;
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    double l = 0;
-    if (r < a.rows) {
-        const int64_t n = r / a.inner, p = r % a.inner;
-        const T* z = static_cast<const T*>(a.logits) + (size_t)n * a.V * a.inner + p;
-        const size_t rec = (size_t)n * a.k * a.inner + p;
-        uint32_t* mine = bits + threadIdx.x;
-        const int nw = (a.V + 31) / 32;
-        for (int i = 0; i < nw; ++i) mine[256 * i] = 0;
-        const float w = a.weight ? a.weight[r] : 1.f;
-        const float rest = a.rest ? a.rest[r] : NEG_INF;
-        // kept classes: marks (an index seen before is absent), maxima
-        float M = rest, m = NEG_INF;
-        for (int j = 0; j < a.k; ++j) {
-            const int i = distill_index(a, rec + (size_t)j * a.inner);
-            if (i < 0 || (mine[256 * (i >> 5)] >> (i & 31) & 1)) continue;
-            mine[256 * (i >> 5)] |= 1u << (i & 31);
-            M = fmaxf(M, distill_value(a, rec + (size_t)j * a.inner));
-            m = fmaxf(m, (float)z[(size_t)i * a.inner]);
+    const int tid = threadIdx.x, px = tid & 63, sl = tid / 64;
+    const int64_t at = (int64_t)blockIdx.x * 64 + px;
+    const bool on = at < a.rows;
+    const int64_t r = on ? at : a.rows - 1;  // (a thread beyond the last pixel reads that one)
+    const int64_t n = r / a.inner, p = r % a.inner;
+    const T* z = static_cast<const T*>(a.logits) + (size_t)n * a.V * a.inner + p;
+    const size_t rec = (size_t)n * a.k * a.inner + p;
+    uint32_t* mine = bits + px;
+    const float c = a.c;
+    for (int i = sl; i < (a.V + 31) / 32; i += 4) mine[64 * i] = 0;
+    __syncthreads();
+    // The record's entries, each index once: read on pass 0, which marks them, and kept in
+    // registers, up to KR; or read on every pass, with the marks set, cleared and set again.
+    int ri[KR > 0 ? KR : 1];
+    float rt[KR > 0 ? KR : 1], rz[KR > 0 ? KR : 1];
+    auto entries = [&](int pass, auto f) {
+        if constexpr (KR > 0) {
+            if (pass == 0) {
+#pragma unroll
+                for (int e = 0; e < KR; ++e) {
+                    ri[e] = -1;
+                    if (e < a.k) {
+                        ri[e] = distill_index(a, rec + (size_t)e * a.inner);
+                        rt[e] = distill_value(a, rec + (size_t)e * a.inner);
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < KR; ++e) rz[e] = ri[e] >= 0 ? (float)z[(size_t)ri[e] * a.inner] : NEG_INF;
+#pragma unroll
+                for (int e = 0; e < KR; ++e)
+                    if (ri[e] >= 0) {
+                        uint32_t& word = mine[64 * (ri[e] >> 5)];
+                        const uint32_t b = 1u << (ri[e] & 31);
+                        if (word & b) ri[e] = -1;
+                        else word |= b;
+                    }
+            }
+#pragma unroll
+            for (int e = 0; e < KR; ++e)
+                if (ri[e] >= 0) f(ri[e], rt[e], rz[e]);
+            return;
         }
-        RunSum acc;
-        for (int i0 = 0; i0 < a.V; i0 += 32) {
-            const uint32_t b = mine[256 * (i0 >> 5)];
-            const int top = a.V - i0 < 32 ? a.V - i0 : 32;
-            for (int e = 0; e < top; ++e) {
-                const float v = (float)z[(size_t)(i0 + e) * a.inner];
-                if (!(b >> e & 1)) acc.add1(v, a.c);
+        for (int j0 = 0; j0 < a.k; j0 += 4) {
+            int i[4];
+            float t[4], zi[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const size_t q = rec + (size_t)(j0 + e < a.k ? j0 + e : a.k - 1) * a.inner;
+                i[e] = j0 + e < a.k ? distill_index(a, q) : -1;
+                t[e] = distill_value(a, q);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) zi[e] = i[e] >= 0 ? (float)z[(size_t)i[e] * a.inner] : NEG_INF;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (i[e] < 0) continue;
+                uint32_t& word = mine[64 * (i[e] >> 5)];
+                const uint32_t b = 1u << (i[e] & 31);
+                if (((word & b) != 0) == (pass != 1)) continue;
+                word ^= b;
+                f(i[e], t[e], zi[e]);
             }
         }
-        const MaxSum rs = acc.done(a.c);
+    };
+    const float w = a.weight ? a.weight[r] : 1.f;
+    const float rest = a.rest ? a.rest[r] : NEG_INF;
+    float M = rest, m = NEG_INF;
+    if (sl == 0)
+        entries(0, [&](int, float t, float zi) {
+            M = fmaxf(M, t);
+            m = fmaxf(m, zi);
+        });
+    __syncthreads();
+    // classes in eights, so that a group's marks lie in one word
+    const int per = (a.V + 31) / 32 * 8, v0 = sl * per < a.V ? sl * per : a.V, v1 = v0 + per < a.V ? v0 + per : a.V;
+    auto each = [&](auto f) {
+        for (int i0 = v0; i0 < v1; i0 += 8) {
+            const uint32_t b = mine[64 * (i0 >> 5)] >> (i0 & 31);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = (float)z[(size_t)(i0 + e < v1 ? i0 + e : v1 - 1) * a.inner];
+            f(i0, b, x);
+        }
+    };
+    RunSum acc;
+    each([&](int i0, uint32_t b, float (&x)[8]) {
+        float mx = NEG_INF;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (b >> e & 1 || i0 + e >= v1) x[e] = NEG_INF;
+            mx = fmaxf(mx, x[e]);
+        }
+        acc.add(x, 8, mx, c);
+    });
+    MaxSum rs = acc.done(c);
+    sm[tid] = rs.m;
+    ss[tid] = rs.s;
+    __syncthreads();
+    double l = 0;
+    if (sl == 0) {
+        for (int q = px + 64; q < 256; q += 64) rs.merge(sm[q], ss[q], c);
         const bool has = rs.m != NEG_INF;
         m = fmaxf(m, rs.m);
-        // the k + 1 terms; the marks are cleared as entries are met, so a second pass over the
-        // entries again takes each index once
-        auto entries = [&](bool set, auto f) {
-            for (int j = 0; j < a.k; ++j) {
-                const size_t at = rec + (size_t)j * a.inner;
-                const int i = distill_index(a, at);
-                if (i < 0) continue;
-                const uint32_t b = 1u << (i & 31);
-                uint32_t& word = mine[256 * (i >> 5)];
-                if (((word & b) != 0) == set) continue;
-                word ^= b;
-                f(i, distill_value(a, at), (float)z[(size_t)i * a.inner]);
-            }
-        };
-        double sq = 0, ss = 0;
-        entries(false, [&](int, float t, float zi) {
-            sq += exp2_raw((t - M) * a.c);
-            ss += exp2_raw((zi - m) * a.c);
+        double sq = 0, sp = 0;
+        entries(1, [&](int, float t, float zi) {
+            sq += exp2_raw((t - M) * c);
+            sp += exp2_raw((zi - m) * c);
         });
-        const float er = rest == NEG_INF ? 0.f : exp2_raw((rest - M) * a.c);
-        const double iTd = (double)a.c * LN2;  // (see RowTerms)
-        const double logr = has ? ((double)rs.m - (double)m) * iTd + log((double)rs.s) : (double)NEG_INF;
-        const float er_s = has ? rs.s * exp2_raw((rs.m - m) * a.c) : rs.s;
+        const float er = rest == NEG_INF ? 0.f : exp2_raw((rest - M) * c);
+        const double iT = (double)c * LN2;  // (see RowTerms)
+        const double logr = has ? ((double)rs.m - (double)m) * iT + log((double)rs.s) : (double)NEG_INF;
+        const float sr = has ? rs.s * exp2_raw((rs.m - m) * c) : rs.s;
         sq += er;
-        ss += er_s;
-        const double lq = log(sq), ls = log(ss), rsq = 1.0 / sq, rss = 1.0 / ss;
+        sp += sr;
+        const double lq = log(sq), ls = log(sp), rsq = 1.0 / sq, rsp = 1.0 / sp;
         const bool none = M == NEG_INF || w == 0.f;
         const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
         const double g = none ? 0.0 : a.coef * a.T * (double)w * go;
         T* d = static_cast<T*>(a.dz) + (a.dz ? (size_t)n * a.V * a.inner + p : 0);
         double kl = 0;
-        entries(true, [&](int i, float t, float zi) {
-            const double q = (double)exp2_raw((t - M) * a.c) * rsq;
+        entries(2, [&](int i, float t, float zi) {
+            const double q = (double)exp2_raw((t - M) * c) * rsq;
             if (!(q == 0.0))
-                kl += q * ((((double)t - (double)M) * iTd - lq) - (((double)zi - (double)m) * iTd - ls));
-            if (a.dz) d[(size_t)i * a.inner] = (T)(none ? 0.f : (float)(g * ((double)exp2_raw((zi - m) * a.c) * rss - q)));
+                kl += q * ((((double)t - (double)M) * iT - lq) - (((double)zi - (double)m) * iT - ls));
+            if (a.dz && on)
+                d[(size_t)i * a.inner] = (T)(none ? 0.f : (float)(g * ((double)exp2_raw((zi - m) * c) * rsp - q)));
         });
         const double qr = (double)er * rsq;
-        if (!(qr == 0.0)) kl += qr * ((((double)rest - (double)M) * iTd - lq) - (logr - ls));
-        l = none ? 0.0 : a.coef * a.T * a.T * (double)w * kl;
-        if (a.row_out) a.row_out[r] = (float)l;
-        if (a.dz) {
-            const float f = none || !has ? 0.f : (float)(g * (((double)er_s * rss - qr) / (double)rs.s));
-            for (int i0 = 0; i0 < a.V; i0 += 32) {
-                const uint32_t b = mine[256 * (i0 >> 5)];
-                const int top = a.V - i0 < 32 ? a.V - i0 : 32;
-                for (int e = 0; e < top; ++e) {
-                    const float v = (float)z[(size_t)(i0 + e) * a.inner];
-                    if (!(b >> e & 1))
-                        d[(size_t)(i0 + e) * a.inner] = (T)(f == 0.f ? 0.f : f * exp2_raw((v - rs.m) * a.c));
-                }
-            }
-        }
+        if (!(qr == 0.0)) kl += qr * ((((double)rest - (double)M) * iT - lq) - (logr - ls));
+        l = none || !on ? 0.0 : a.coef * a.T * a.T * (double)w * kl;
+        if (a.row_out && on) a.row_out[r] = (float)l;
+        sm[px] = rs.m;
+        ss[px] = none || !has ? 0.f : (float)(g * (((double)sr * rsp - qr) / (double)rs.s));
+    }
+    if (a.dz) {
+        __syncthreads();
+        const float mr = sm[px], f = ss[px];
+        T* d = static_cast<T*>(a.dz) + (size_t)n * a.V * a.inner + p;
+        each([&](int i0, uint32_t b, float (&x)[8]) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (on && !(b >> e & 1) && i0 + e < v1)
+                    d[(size_t)(i0 + e) * a.inner] = (T)(f == 0.f ? 0.f : f * exp2_raw((x[e] - mr) * c));
+        });
     }
     block_loss(a, wave_sum_d(l));
 }
@@ -1201,45 +1263,147 @@ template <typename T> __global__ void __launch_bounds__(256) top_wave_kernel(Top
     if (lane == 0) a.rest[r] = rest_logit(rest, a.T);
 }
 
-// class maps: a thread a pixel, k rounds of "the next in order"; VR > 0: the pixel's classes
-// stay in registers
-template <typename T, int VR> __global__ void __launch_bounds__(256) top_map_kernel(TopArgs a) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r >= a.rows) return;
+// Signed keys in order_key's order, and back; a place not taken is -inf.
+constexpr int MAP_NINF = (int)0x807fffffu, MAP_EMPTY = MAP_NINF - 1, MAP_TOP = 0x7fffffff;
+__device__ __forceinline__ int map_key(float v) {
+    const int b = __float_as_int(v + 0.f);  // (-0 is 0)
+    return v != v ? MAP_TOP : b ^ (b >> 31 & 0x7fffffff);
+}
+__device__ __forceinline__ float map_value(int k) {
+    k = k > MAP_NINF ? k : MAP_NINF;
+    return __int_as_float(k ^ (k >> 31 & 0x7fffffff));
+}
+// KR places in order; a class that enters pushes the last one out.  Classes come by their
+// index, so one that equals a place stays behind it.
+template <int KR> struct MapTop {
+    int key[KR], id[KR];
+    // `used` places, the last ones
+    __device__ __forceinline__ void clear(int used) {
+#pragma unroll
+        for (int e = 0; e < KR; ++e) {
+            key[e] = e < KR - used ? MAP_TOP : MAP_EMPTY;
+            id[e] = -1;
+        }
+    }
+    // x: the key that is left over
+    __device__ __forceinline__ void put(int& x, int i) {
+        const int over = x < key[KR - 1] ? x : key[KR - 1];
+#pragma unroll
+        for (int e = KR - 1; e > 0; --e) {
+            const bool here = x > key[e], before = x > key[e - 1];
+            id[e] = before ? id[e - 1] : here ? i : id[e];
+            const int up = x > key[e] ? x : key[e];
+            key[e] = up < key[e - 1] ? up : key[e - 1];
+        }
+        id[0] = x > key[0] ? i : id[0];
+        key[0] = x > key[0] ? x : key[0];
+        x = over;
+    }
+};
+
+// Class maps: a thread a pixel, or S threads of different waves a pixel, each a part of the
+// classes, whose lists are joined.  One reading gives KR entries and the sums of what is
+// pushed out; more than KR take a reading for each KR.  A round of "the next in order"
+// for every entry took 62 us where 4 maps of 32 x 256^2 keep 8 classes, this
+// MEASURED32; with 64 classes 166 against MEASURED64.
+template <typename T, int KR, int S> __global__ void __launch_bounds__(256) top_map_kernel(TopArgs a) {
+    constexpr int PX = 256 / S;
+    __shared__ int sk[S > 1 ? 256 * KR : 1], si[S > 1 ? 256 * KR : 1];
+    __shared__ float sm[S > 1 ? 256 : 1], ss[S > 1 ? 256 : 1];
+    const int tid = threadIdx.x, px = tid % PX, sl = tid / PX;
+    const int64_t at = (int64_t)blockIdx.x * PX + px;
+    const bool on = at < a.rows;
+    const int64_t r = on ? at : a.rows - 1;  // (a thread beyond the last pixel reads that one)
     const int64_t n = r / a.inner, p = r % a.inner;
     const T* z = static_cast<const T*>(a.logits) + (size_t)n * a.V * a.inner + p;
-    T* val = static_cast<T*>(a.values) + (size_t)n * a.k * a.inner + p;
-    int64_t* idx = a.indices + (size_t)n * a.k * a.inner + p;
-    uint32_t key[VR > 0 ? VR : 1];
-    if constexpr (VR > 0) {
+    const int per = (a.V + S - 1) / S, v0 = sl * per < a.V ? sl * per : a.V, v1 = v0 + per < a.V ? v0 + per : a.V;
+    int lastk = MAP_TOP, lasti = -1;
+    for (int j0 = 0;; j0 += KR) {
+        const int used = a.k - j0 < KR ? a.k - j0 : KR;
+        const bool fin = j0 + KR >= a.k;
+        MapTop<KR> top;
+        top.clear(used);
+        RunSum acc;
+        for (int i0 = v0; i0 < v1; i0 += 8) {
+            float y[8];
 #pragma unroll
-        for (int i = 0; i < VR; ++i) key[i] = i < a.V ? order_key((float)z[(size_t)i * a.inner]) : 0u;
-    }
-    uint64_t last = ~0ull;
-    RunSum rest;
-    for (int j = 0; j <= a.k; ++j) {
-        uint64_t best = 0;
-        auto see = [&](uint32_t kv, int i) {
-            const uint64_t o = order_pair(kv, i);
-            if (j == 0 || o < last) {
-                if (j < a.k) best = o > best ? o : best;
-                else rest.add1(key_value(kv), a.c);
+            for (int e = 0; e < 8; ++e) y[e] = (float)z[(size_t)(i0 + e < v1 ? i0 + e : v1 - 1) * a.inner];
+            int x[8], mx = MAP_EMPTY;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                x[e] = i0 + e < v1 ? map_key(y[e]) : MAP_EMPTY;
+                if (j0 > 0 && !(x[e] < lastk || (x[e] == lastk && i0 + e > lasti))) x[e] = MAP_EMPTY;
+                mx = mx > x[e] ? mx : x[e];
             }
-        };
-        if constexpr (VR > 0) {
+            if (mx > top.key[KR - 1]) {
 #pragma unroll
-            for (int i = 0; i < VR; ++i)
-                if (i < a.V) see(key[i], i);
-        } else {
-            for (int i = 0; i < a.V; ++i) see(order_key((float)z[(size_t)i * a.inner]), i);
+                for (int e = 0; e < 8; ++e) top.put(x[e], i0 + e);
+            }
+            if (fin) {
+                float m = NEG_INF;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    y[e] = map_value(x[e]);
+                    m = fmaxf(m, y[e]);
+                }
+                acc.add(y, 8, m, a.c);
+            }
         }
-        if (j < a.k) {
-            last = best;
-            val[(size_t)j * a.inner] = (T)key_value((uint32_t)(best >> 32));
-            idx[(size_t)j * a.inner] = (int64_t)(uint32_t)~(uint32_t)best;
+        if constexpr (S > 1) {
+            __syncthreads();  // (the last round's entries have been read)
+            if (sl > 0) {
+                const MaxSum o = acc.done(a.c);
+                sm[tid] = o.m;
+                ss[tid] = o.s;
+#pragma unroll
+                for (int e = 0; e < KR; ++e) {
+                    sk[e * 256 + tid] = top.key[e];
+                    si[e * 256 + tid] = top.id[e];
+                }
+            }
+            __syncthreads();
+            if (sl == 0)
+                for (int q = px + PX; q < 256; q += PX)
+#pragma unroll
+                    for (int e = 0; e < KR; ++e)
+                        if (e >= KR - used) {
+                            int x = sk[e * 256 + q];
+                            top.put(x, si[e * 256 + q]);
+                            if (fin) acc.add1(map_value(x), a.c);
+                        }
+        }
+        if (sl == 0 && on) {
+            T* val = static_cast<T*>(a.values) + (size_t)n * a.k * a.inner + p;
+            int64_t* idx = a.indices + (size_t)n * a.k * a.inner + p;
+#pragma unroll
+            for (int e = 0; e < KR; ++e)
+                if (e >= KR - used) {
+                    const size_t j = (size_t)(j0 + e - (KR - used)) * a.inner;
+                    val[j] = (T)map_value(top.key[e]);
+                    idx[j] = top.id[e];
+                }
+        }
+        if (fin) {
+            if (sl == 0) {
+                MaxSum rest = acc.done(a.c);
+                if constexpr (S > 1)
+                    for (int q = px + PX; q < 256; q += PX) rest.merge(sm[q], ss[q], a.c);
+                if (on) a.rest[r] = rest_logit(rest, a.T);
+            }
+            break;
+        }
+        lastk = top.key[KR - 1];
+        lasti = top.id[KR - 1];
+        if constexpr (S > 1) {
+            if (sl == 0) {
+                sk[px] = lastk;  // (places 0 .. PX - 1 hold no list)
+                si[px] = lasti;
+            }
+            __syncthreads();
+            lastk = sk[px];
+            lasti = si[px];
         }
     }
-    a.rest[r] = rest_logit(rest.done(a.c), a.T);
 }
 
 // ---------------------------------------------------------------- host side
@@ -1261,8 +1425,8 @@ static int rows_check(const char* what, const void* logits, int dtype, int64_t N
                   (long long)inner);
         return UGPG_ERR_INVALID;
     }
-    // (grids of at most 2^32 threads; V leaves room for a span's padding in 32 bits)
-    if (V > (1 << 30) || (inner == 1 ? N > (1 << 22) : N > (int64_t)0x7fffffff / inner)) {
+    // (grids below 2^32 threads, up to four a pixel; V leaves room for a span's padding in 32 bits)
+    if (V > (1 << 30) || (inner == 1 ? N > (1 << 22) : N > (int64_t)0x3fffffff / inner)) {
         set_error("%s: N=%lld V=%d inner=%lld is too large", what, (long long)N, V, (long long)inner);
         return UGPG_ERR_INVALID;
     }
@@ -1313,11 +1477,18 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
         else hipLaunchKernelGGL(KH, dim3((unsigned)(grid)), dim3(nt), 0, s, a);     \
     } while (0)
     if (inner > 1) {
-        const int64_t g = cdiv(a.rows, 256);
-        if (V <= 8) TOP_GO((top_map_kernel<float, 8>), (top_map_kernel<__bf16, 8>), g, 256);
-        else if (V <= 16) TOP_GO((top_map_kernel<float, 16>), (top_map_kernel<__bf16, 16>), g, 256);
-        else if (V <= 32) TOP_GO((top_map_kernel<float, 32>), (top_map_kernel<__bf16, 32>), g, 256);
-        else TOP_GO((top_map_kernel<float, 0>), (top_map_kernel<__bf16, 0>), g, 256);
+        // the classes of a pixel in four parts where there are many, or few pixels
+        const bool four = V > 32 || (V > 16 && a.rows < (1 << 17));
+        const int64_t g = cdiv(a.rows, four ? 64 : 256);
+#define TOP_MAP(KR)                                                                                       \
+    do {                                                                                                  \
+        if (four) TOP_GO((top_map_kernel<float, KR, 4>), (top_map_kernel<__bf16, KR, 4>), g, 256);        \
+        else TOP_GO((top_map_kernel<float, KR, 1>), (top_map_kernel<__bf16, KR, 1>), g, 256);             \
+    } while (0)
+        if (k <= 2) TOP_MAP(2);
+        else if (k <= 4) TOP_MAP(4);
+        else TOP_MAP(8);
+#undef TOP_MAP
     } else if (V <= 64) {
         TOP_GO((top_wave_kernel<float>), (top_wave_kernel<__bf16>), cdiv(N, 4), 256);
     } else {
@@ -1330,6 +1501,9 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
 #undef TOP_GO
     return check_launch("top_logits");
 }
+
+// pixels of a block: a thread a pixel in registers, or four threads a pixel
+static int map_pixels(int V, int k) { return V <= 32 && k <= 8 ? 256 : 64; }
 
 // blocks of four waves for short rows: up to 16 rounds of the card's 2048
 static int64_t wave_blocks(int64_t rows) {
@@ -1363,7 +1537,7 @@ static int distill_check(const char* what, const ugpg_distill_t* p) {
 
 extern "C" size_t ugpg_distill_workspace(const ugpg_distill_t* p, int backward) {
     if (distill_check("distill_workspace", p)) return 0;
-    if (p->inner > 1) return backward ? 0 : (size_t)cdiv(p->N * p->inner, 256) * 8;
+    if (p->inner > 1) return backward ? 0 : (size_t)cdiv(p->N * p->inner, map_pixels(p->V, p->k)) * 8;
     size_t n = backward ? 0 : (size_t)p->N * 8;  // the rows' losses, then the parts of split rows
     if (p->V > DW_MAX) {
         const Split sp = row_split(p->N, p->V);
@@ -1380,16 +1554,19 @@ static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, bool
     int64_t nsum = rows;
     a.row_loss = loss ? static_cast<double*>(ws) : nullptr;
     if (p->inner > 1) {
-        nsum = cdiv(rows, 256);
+        nsum = cdiv(rows, map_pixels(a.V, a.k));
         const dim3 grid((unsigned)nsum);
-        if (a.V <= 8 && a.k <= 4)
+        const unsigned marks = (unsigned)(cdiv(a.V, 32) * 256);
+        if (map_pixels(a.V, a.k) == 64) {
+            if (a.k <= 8) hipLaunchKernelGGL((distill_map_kernel<T, 8>), grid, dim3(256), marks, s, a);
+            else if (a.k <= 32) hipLaunchKernelGGL((distill_map_kernel<T, 32>), grid, dim3(256), marks, s, a);
+            else hipLaunchKernelGGL((distill_map_kernel<T, 0>), grid, dim3(256), marks, s, a);
+        } else if (a.V <= 8 && a.k <= 4)
             hipLaunchKernelGGL((distill_map_small_kernel<T, 8, 4>), grid, dim3(256), 0, s, a);
         else if (a.V <= 16 && a.k <= 8)
             hipLaunchKernelGGL((distill_map_small_kernel<T, 16, 8>), grid, dim3(256), 0, s, a);
-        else if (a.V <= 32 && a.k <= 8)
-            hipLaunchKernelGGL((distill_map_small_kernel<T, 32, 8>), grid, dim3(256), 0, s, a);
         else
-            hipLaunchKernelGGL((distill_map_kernel<T>), grid, dim3(256), (unsigned)(cdiv(a.V, 32) * 1024), s, a);
+            hipLaunchKernelGGL((distill_map_small_kernel<T, 32, 8>), grid, dim3(256), 0, s, a);
     } else if (a.V <= DW_MAX) {
         // up to 64 rows: one block of 16 waves, which also sums them
         const bool one = rows <= 64;
