@@ -216,6 +216,44 @@ __device__ __forceinline__ float distill_value(const DistillArgs& a, size_t at) 
                  : static_cast<const float*>(a.values)[at];
 }
 
+// Entries 0 .. K - 1 of a pixel's record at `at` (absent beyond the k it has).  All loads go out
+// before the first value is looked at: a choice of type per entry made the loads wait for one
+// another (8 maps of 16 x 256^2 with 12 entries: 202 us against 153; of 8 classes with 3
+// entries and the gradient 37 against 32).
+template <int K>
+__device__ __forceinline__ void map_entries(const DistillArgs& a, size_t at, int k, int* idx, float* t) {
+    int lo[K], hi[K];
+    uint32_t v[K];
+    if (a.i64) {
+#pragma unroll
+        for (int e = 0; e < K; ++e) {
+            const int2 q = static_cast<const int2*>(a.indices)[at + (size_t)(e < k ? e : k - 1) * a.inner];
+            lo[e] = q.x;
+            hi[e] = q.y;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < K; ++e) {
+            lo[e] = static_cast<const int*>(a.indices)[at + (size_t)(e < k ? e : k - 1) * a.inner];
+            hi[e] = 0;
+        }
+    }
+    if (a.v16) {
+#pragma unroll
+        for (int e = 0; e < K; ++e)
+            v[e] = static_cast<const uint16_t*>(a.values)[at + (size_t)(e < k ? e : k - 1) * a.inner];
+    } else {
+#pragma unroll
+        for (int e = 0; e < K; ++e)
+            v[e] = static_cast<const uint32_t*>(a.values)[at + (size_t)(e < k ? e : k - 1) * a.inner];
+    }
+#pragma unroll
+    for (int e = 0; e < K; ++e) {
+        idx[e] = e < k && hi[e] == 0 && (uint32_t)lo[e] < (uint32_t)a.V ? lo[e] : -1;
+        t[e] = __uint_as_float(a.v16 ? v[e] << 16 : v[e]);
+    }
+}
+
 // What a row's k + 1 classes give (computed by one wave over entries in LDS), in fp64: a loss is
 // the difference of logarithms of nearly equal probabilities, and fp32 exponentials alone
 // put a single row's KL 2e-7 off.  1 / T is c * ln 2 with the rounded c that the rest's fp32
@@ -629,15 +667,7 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
         int idx[KR];
 #pragma unroll
         for (int i = 0; i < VR; ++i) x[i] = i < a.V ? (float)z[(size_t)i * a.inner] : NEG_INF;
-#pragma unroll
-        for (int j = 0; j < KR; ++j) {
-            idx[j] = -1;
-            t[j] = NEG_INF;
-            if (j < a.k) {
-                idx[j] = distill_index(a, rec + (size_t)j * a.inner);
-                t[j] = distill_value(a, rec + (size_t)j * a.inner);
-            }
-        }
+        map_entries<KR>(a, rec, a.k, idx, t);
         const float w = a.weight ? a.weight[r] : 1.f;
         const float rest = a.rest ? a.rest[r] : NEG_INF;
         uint32_t mask = 0;
@@ -742,12 +772,9 @@ template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map
         if constexpr (KR > 0) {
             if (pass == 0) {
 #pragma unroll
-                for (int e = 0; e < KR; ++e) {
-                    ri[e] = -1;
-                    if (e < a.k) {
-                        ri[e] = distill_index(a, rec + (size_t)e * a.inner);
-                        rt[e] = distill_value(a, rec + (size_t)e * a.inner);
-                    }
+                for (int e = 0; e < KR; e += 8) {
+                    for (int i = e; i < e + 8; ++i) ri[i] = -1;
+                    if (e < a.k) map_entries<8>(a, rec + (size_t)e * a.inner, a.k - e, ri + e, rt + e);
                 }
 #pragma unroll
                 for (int e = 0; e < KR; ++e) rz[e] = ri[e] >= 0 ? (float)z[(size_t)ri[e] * a.inner] : NEG_INF;
@@ -768,12 +795,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map
         for (int j0 = 0; j0 < a.k; j0 += 4) {
             int i[4];
             float t[4], zi[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const size_t q = rec + (size_t)(j0 + e < a.k ? j0 + e : a.k - 1) * a.inner;
-                i[e] = j0 + e < a.k ? distill_index(a, q) : -1;
-                t[e] = distill_value(a, q);
-            }
+            map_entries<4>(a, rec + (size_t)j0 * a.inner, a.k - j0, i, t);
 #pragma unroll
             for (int e = 0; e < 4; ++e) zi[e] = i[e] >= 0 ? (float)z[(size_t)i[e] * a.inner] : NEG_INF;
 #pragma unroll
@@ -1305,7 +1327,7 @@ template <int KR> struct MapTop {
 // classes, whose lists are joined.  One reading gives KR entries and the sums of what is
 // pushed out; more than KR take a reading for each KR.  A round of "the next in order"
 // for every entry took 62 us where 4 maps of 32 x 256^2 keep 8 classes, this
-// MEASURED32; with 64 classes 166 against MEASURED64.
+// 21; 2 maps of 64 classes 166 against 30, one of 1000 at 128^2 with 5 entries 2012 against 70.
 template <typename T, int KR, int S> __global__ void __launch_bounds__(256) top_map_kernel(TopArgs a) {
     constexpr int PX = 256 / S;
     __shared__ int sk[S > 1 ? 256 * KR : 1], si[S > 1 ? 256 * KR : 1];
