@@ -557,7 +557,8 @@ int ugpg_group_norm_bwd(const ugpg_group_norm_t* p, const void* dy, int dy_dtype
  * of its output, and the loss of the current stage against that record.
  * Rows: N rows of V logits (inner == 1; row r at logits + r*stride, stride >= V), or the
  * pixels of N class maps [V][inner] (inner > 1, stride == V*inner).  dtype UGPG_DT_F32 or
- * UGPG_DT_BF16.  1 <= k <= min(V, 256).  With t a row's logits at temperature T:
+ * UGPG_DT_BF16.  1 <= k <= min(V, 256), T in 1e-30..1e30, at most 2^22 rows or 2^30 pixels.
+ * With t a row's logits at temperature T:
  *   values, indices [N][k][inner]: the k largest, the larger first, equal ones by the lower
  *     index (a NaN counts as the largest); values have the logits' type
  *   rest [N][inner]: T * logsumexp(t_v / T) over the others (-inf: none) */

@@ -651,8 +651,8 @@ __global__ void __launch_bounds__(256) distill_wave_kernel(DistillArgs a) {
 // ---------------------------------------------------------------- class maps, a thread each
 // At most VR classes and KR entries: a pixel's logits and record stay in registers, read once.
 // Exponentials are fp32 here (a map's loss is a mean over its pixels), sums and differences
-// fp64.  16 maps of 8 x 256^2 fp32 at 3 entries, with the gradient: 34 us against 55 for the form
-// below; its floor, 113 MB at a copy's 4.8 TB/s, is 24.
+// fp64.  16 maps of 8 x 256^2 fp32 at 3 entries, with the gradient: 30 us (55 with marks in LDS
+// and the classes read twice); its floor, 113 MB at a copy's 4.8 TB/s, is 24.
 template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) distill_map_small_kernel(DistillArgs a) {
     if (distill_skip(a)) return;
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
