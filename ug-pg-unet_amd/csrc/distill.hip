@@ -218,8 +218,7 @@ __device__ __forceinline__ float distill_value(const DistillArgs& a, size_t at) 
 
 // Entries 0 .. K - 1 of a pixel's record at `at` (absent beyond the k it has).  All loads go out
 // before the first value is looked at: a choice of type per entry made the loads wait for one
-// another (8 maps of 16 x 256^2 with 12 entries: 202 us against 153; of 8 classes with 3
-// entries and the gradient 37 against 32).
+// another (16 maps of 8 x 256^2 with 3 entries and the gradient: 37 us against 32).
 template <int K>
 __device__ __forceinline__ void map_entries(const DistillArgs& a, size_t at, int k, int* idx, float* t) {
     int lo[K], hi[K];
@@ -746,15 +745,20 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
     block_loss(a, wave_sum_d(l));
 }
 
-// More classes or entries: 64 pixels a block, the classes in four parts, a wave each; the first
-// wave reads the record and joins the parts.  Marks of the kept classes lie in LDS.
+// More classes or entries: a thread a pixel, or (S = 4, more than 32 classes: the pixels alone may
+// not fill the card) four threads of different waves, each a part of the classes; the first
+// reads the record and joins the parts.  Marks of the kept classes lie in LDS.  2 maps of 64 x
+// 256^2 fp32, 8 entries, with the gradient: 35 us (a thread a pixel, entries read three times:
+// 87); one of 1000 x 128^2: 67 (690); 8 maps of 16 x 256^2 with 12 entries, the loss: 36, with
+// S = 4 153.  Bound by the record's steps and the classes' second reading.
 constexpr int DM_MAX = 1024;  // classes
-template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map_kernel(DistillArgs a) {
-    extern __shared__ uint32_t bits[];  // [ceil(V / 32)][64]
+template <typename T, int KR, int S> __global__ void __launch_bounds__(256) distill_map_kernel(DistillArgs a) {
+    constexpr int PX = 256 / S;
+    extern __shared__ uint32_t bits[];  // [ceil(V / 32)][PX]
     __shared__ float sm[256], ss[256];
     if (distill_skip(a)) return;
-    const int tid = threadIdx.x, px = tid & 63, sl = tid / 64;
-    const int64_t at = (int64_t)blockIdx.x * 64 + px;
+    const int tid = threadIdx.x, px = tid % PX, sl = tid / PX;
+    const int64_t at = (int64_t)blockIdx.x * PX + px;
     const bool on = at < a.rows;
     const int64_t r = on ? at : a.rows - 1;  // (a thread beyond the last pixel reads that one)
     const int64_t n = r / a.inner, p = r % a.inner;
@@ -762,7 +766,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map
     const size_t rec = (size_t)n * a.k * a.inner + p;
     uint32_t* mine = bits + px;
     const float c = a.c;
-    for (int i = sl; i < (a.V + 31) / 32; i += 4) mine[64 * i] = 0;
+    for (int i = sl; i < (a.V + 31) / 32; i += S) mine[PX * i] = 0;
     __syncthreads();
     // The record's entries, each index once: read on pass 0, which marks them, and kept in
     // registers, up to KR; or read on every pass, with the marks set, cleared and set again.
@@ -781,7 +785,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map
 #pragma unroll
                 for (int e = 0; e < KR; ++e)
                     if (ri[e] >= 0) {
-                        uint32_t& word = mine[64 * (ri[e] >> 5)];
+                        uint32_t& word = mine[PX * (ri[e] >> 5)];
                         const uint32_t b = 1u << (ri[e] & 31);
                         if (word & b) ri[e] = -1;
                         else word |= b;
@@ -801,7 +805,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 if (i[e] < 0) continue;
-                uint32_t& word = mine[64 * (i[e] >> 5)];
+                uint32_t& word = mine[PX * (i[e] >> 5)];
                 const uint32_t b = 1u << (i[e] & 31);
                 if (((word & b) != 0) == (pass != 1)) continue;
                 word ^= b;
@@ -819,10 +823,10 @@ template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map
         });
     __syncthreads();
     // classes in eights, so that a group's marks lie in one word
-    const int per = (a.V + 31) / 32 * 8, v0 = sl * per < a.V ? sl * per : a.V, v1 = v0 + per < a.V ? v0 + per : a.V;
+    const int per = (a.V + 8 * S - 1) / (8 * S) * 8, v0 = sl * per < a.V ? sl * per : a.V, v1 = v0 + per < a.V ? v0 + per : a.V;
     auto each = [&](auto f) {
         for (int i0 = v0; i0 < v1; i0 += 8) {
-            const uint32_t b = mine[64 * (i0 >> 5)] >> (i0 & 31);
+            const uint32_t b = mine[PX * (i0 >> 5)] >> (i0 & 31);
             float x[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = (float)z[(size_t)(i0 + e < v1 ? i0 + e : v1 - 1) * a.inner];
@@ -845,7 +849,7 @@ template <typename T, int KR> __global__ void __launch_bounds__(256) distill_map
     __syncthreads();
     double l = 0;
     if (sl == 0) {
-        for (int q = px + 64; q < 256; q += 64) rs.merge(sm[q], ss[q], c);
+        for (int q = px + PX; q < 256; q += PX) rs.merge(sm[q], ss[q], c);
         const bool has = rs.m != NEG_INF;
         m = fmaxf(m, rs.m);
         double sq = 0, sp = 0;
@@ -1524,8 +1528,8 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
     return check_launch("top_logits");
 }
 
-// pixels of a block: a thread a pixel in registers, or four threads a pixel
-static int map_pixels(int V, int k) { return V <= 32 && k <= 8 ? 256 : 64; }
+// pixels of a block: a thread a pixel, or four
+static int map_pixels(int V) { return V <= 32 ? 256 : 64; }
 
 // blocks of four waves for short rows: up to 16 rounds of the card's 2048
 static int64_t wave_blocks(int64_t rows) {
@@ -1559,7 +1563,7 @@ static int distill_check(const char* what, const ugpg_distill_t* p) {
 
 extern "C" size_t ugpg_distill_workspace(const ugpg_distill_t* p, int backward) {
     if (distill_check("distill_workspace", p)) return 0;
-    if (p->inner > 1) return backward ? 0 : (size_t)cdiv(p->N * p->inner, map_pixels(p->V, p->k)) * 8;
+    if (p->inner > 1) return backward ? 0 : (size_t)cdiv(p->N * p->inner, map_pixels(p->V)) * 8;
     size_t n = backward ? 0 : (size_t)p->N * 8;  // the rows' losses, then the parts of split rows
     if (p->V > DW_MAX) {
         const Split sp = row_split(p->N, p->V);
@@ -1576,13 +1580,16 @@ static int distill_run(const ugpg_distill_t* p, DistillArgs a, float* loss, bool
     int64_t nsum = rows;
     a.row_loss = loss ? static_cast<double*>(ws) : nullptr;
     if (p->inner > 1) {
-        nsum = cdiv(rows, map_pixels(a.V, a.k));
+        nsum = cdiv(rows, map_pixels(a.V));
         const dim3 grid((unsigned)nsum);
-        const unsigned marks = (unsigned)(cdiv(a.V, 32) * 256);
-        if (map_pixels(a.V, a.k) == 64) {
-            if (a.k <= 8) hipLaunchKernelGGL((distill_map_kernel<T, 8>), grid, dim3(256), marks, s, a);
-            else if (a.k <= 32) hipLaunchKernelGGL((distill_map_kernel<T, 32>), grid, dim3(256), marks, s, a);
-            else hipLaunchKernelGGL((distill_map_kernel<T, 0>), grid, dim3(256), marks, s, a);
+        const unsigned marks = (unsigned)(cdiv(a.V, 32) * 4 * map_pixels(a.V));
+        if (a.V > 32) {
+            if (a.k <= 8) hipLaunchKernelGGL((distill_map_kernel<T, 8, 4>), grid, dim3(256), marks, s, a);
+            else if (a.k <= 16) hipLaunchKernelGGL((distill_map_kernel<T, 16, 4>), grid, dim3(256), marks, s, a);
+            else hipLaunchKernelGGL((distill_map_kernel<T, 0, 4>), grid, dim3(256), marks, s, a);
+        } else if (a.k > 8) {
+            if (a.k <= 16) hipLaunchKernelGGL((distill_map_kernel<T, 16, 1>), grid, dim3(256), marks, s, a);
+            else hipLaunchKernelGGL((distill_map_kernel<T, 0, 1>), grid, dim3(256), marks, s, a);
         } else if (a.V <= 8 && a.k <= 4)
             hipLaunchKernelGGL((distill_map_small_kernel<T, 8, 4>), grid, dim3(256), 0, s, a);
         else if (a.V <= 16 && a.k <= 8)
