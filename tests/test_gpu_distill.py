@@ -163,6 +163,25 @@ def test_top_logits(dev, dtype, kind):
             assert ok.all(), (shape, k, top.rest[~ok][:3], r[~ok][:3])
 
 
+@pytest.mark.parametrize("V", [66, 127, 255, 257, 511, 513, 769, 1000, 1023, 1025, 1100, 2000, 2047, 3001])
+def test_top_logits_of_middling_rows(dev, V):
+    """A wave a row up to 1024 classes, then a block whose vectors may be fewer than the entries;
+    rows that begin and end anywhere."""
+    import ugpg
+    for kind in ("random", "ties", "equal", "masked", "nan", "one_nan", "nothing", "zeros"):
+        for dtype in (F32, BF16):
+            z = fill(kind, (9, V + 3), dev, dtype, seed=V)[:, 1:V + 1]
+            for k in sorted({1, 2, 63, 64, 65, 250, 256} | {V if V <= 256 else 200}):
+                if k > V:
+                    continue
+                top = ugpg.teacher_top_logits(z, k, 1.5)
+                v, i, r = ref_top(z, k, 1.5)
+                assert torch.equal(top.indices, i), (kind, k)
+                assert torch.equal(top.values.double().nan_to_num(7e7), v.nan_to_num(7e7)), (kind, k)
+                same = (top.rest.double() == r) | (top.rest.isnan() & r.isnan())
+                assert (same | ((top.rest.double() - r).abs() <= 1.5 * REL + 2.0 ** -23 * r.abs())).all(), (kind, k)
+
+
 @pytest.mark.parametrize("shape,k", [((2, 20, 300, 240), 6), ((2, 24, 270, 250), 20), ((1, 100, 37, 41), 2),
                                      ((3, 70, 8, 9), 4), ((1, 1000, 5, 13), 5), ((1, 5000, 3, 5), 9),
                                      ((1, 35, 1, 2), 35)])

@@ -1182,28 +1182,31 @@ template <typename T, int NT, int CAP> __global__ void __launch_bounds__(NT, 8) 
         end = 2 * end < tiles ? 2 * end : tiles;
     }
     MaxSum rest = block_maxsum(acc.done(c), c, s.ms);
-    // the values of the vectors set aside: value e of vector i is f(pair)
+    // the values of the vectors set aside: the key of value e of vector i, f(pair) for each
+    auto key_of = [&](int i, int e) {
+        const uint32_t w = reinterpret_cast<const uint32_t*>(&s.raw[i])[e * (int)sizeof(T) / 4];
+        return order_key(sizeof(T) == 4 ? __uint_as_float(w) : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16));
+    };
     auto each = [&](auto f) {
-        for (int j = tid; j < n * N; j += nt) {
-            const int i = j / N, e = j % N;
-            if (e < (int)s.cnt[i]) {
-                const uint32_t w = reinterpret_cast<const uint32_t*>(&s.raw[i])[e * (int)sizeof(T) / 4];
-                const float v = sizeof(T) == 4 ? __uint_as_float(w)
-                                               : __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
-                f(order_pair(order_key(v), (int)s.idx[i] + e));
-            }
-        }
+        for (int j = tid; j < n * N; j += nt)
+            if (j % N < (int)s.cnt[j / N]) f(order_pair(key_of(j / N, j % N), (int)s.idx[j / N] + j % N));
     };
     bool exact = n > CAP || rest.s != rest.s;  // too much near the top, or a NaN below it
     if (!exact) {
-        uint32_t low = 0;
-        if (n > 64) {
+        // bounds of the k-th: the last tau and the vectors' k-th maximum, or, where that leaves most
+        // of a short row, the k-th value's own prefix (8192 x 2000 bf16, k = 250: 260 us, 512
+        // without, mostly in exact selections; of 3000 it would take 275 instead of 205)
+        uint32_t low = order_key(tau);
+        const bool few = n * 4 > 3 * sp.nv && n * N <= 2048;  // (so wherever n < k <= 256: all are set aside)
+        if (n > 64 || few) {
             if (tid < 64) {
-                const uint32_t p = kth_prefix(n, a.k, [&](int i) { return s.key[i]; });
+                const uint32_t p =
+                    few ? kth_prefix(n * N, a.k, [&](int j) { return j % N < (int)s.cnt[j / N] ? key_of(j / N, j % N) : 0u; })
+                        : kth_prefix(n, a.k, [&](int i) { return s.key[i]; });
                 if (lane == 0) s.tau = p;
             }
             __syncthreads();
-            low = n >= a.k ? s.tau << 16 : 0u;
+            low = s.tau << 16 > low ? s.tau << 16 : low;
         }
         each([&](uint64_t p) {
             if ((uint32_t)(p >> 32) >= low) {
@@ -1285,6 +1288,88 @@ template <typename T> __global__ void __launch_bounds__(256) top_wave_kernel(Top
     if (kept) {
         static_cast<T*>(a.values)[(size_t)r * a.k + rank] = (T)key_value(key);
         a.indices[(size_t)r * a.k + rank] = lane;
+    }
+    if (lane == 0) a.rest[r] = rest_logit(rest, a.T);
+}
+
+// At most 64 * R classes: a wave a row, R classes a lane in registers.  The k-th key is found two
+// bits a step by counting with ballots, until exactly k keys reach the prefix; the entries go
+// to LDS by their index and are ranked there.  No barrier and no second reading: a block a row
+// took 233 us for 7804 x 539 bf16, k = 104, this 50; 8192 x 512, k = 50: 26.
+template <typename T, int R> __global__ void __launch_bounds__(256) top_wide_wave_kernel(TopArgs a) {
+    __shared__ uint32_t skey[4][DK_MAX + 4];
+    __shared__ int sidx[4][DK_MAX];
+    const int lane = threadIdx.x & 63, w = threadIdx.x / 64;
+    const int64_t r = (int64_t)blockIdx.x * 4 + w;
+    if (r >= a.rows) return;
+    const T* z = static_cast<const T*>(a.logits) + r * a.stride;
+    uint32_t key[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) key[i] = lane + 64 * i < a.V ? order_key((float)z[lane + 64 * i]) : 0u;
+    uint32_t t = 0;
+    int reach = 64 * R;  // keys that reach t
+    for (int b = 30; b >= 0 && reach != a.k; b -= 2) {
+        const uint32_t u1 = t | 1u << b, u2 = t | 2u << b, u3 = t | 3u << b;
+        int c1 = 0, c2 = 0, c3 = 0;
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            c1 += __popcll(__ballot(key[i] >= u1));
+            c2 += __popcll(__ballot(key[i] >= u2));
+            c3 += __popcll(__ballot(key[i] >= u3));
+        }
+        t = c3 >= a.k ? u3 : c2 >= a.k ? u2 : c1 >= a.k ? u1 : t;
+        reach = c3 >= a.k ? c3 : c2 >= a.k ? c2 : c1 >= a.k ? c1 : reach;
+    }
+    // more than k: t is the k-th key itself, and of those equal to it the first belong to the record
+    const bool all = reach == a.k;
+    int spare = a.k, base = 0;
+    if (!all) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) spare -= __popcll(__ballot(key[i] > t));
+    }
+    const uint64_t below = (1ull << lane) - 1;
+    RunSum acc;
+    float y[R < 8 ? R : 8], mx = NEG_INF;
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int x = lane + 64 * i;
+        bool take = x < a.V && key[i] >= t;
+        if (!all) {
+            const uint64_t eq = __ballot(take && key[i] == t);
+            take = take && (key[i] > t || __popcll(eq & below) < spare);
+            spare -= __popcll(eq) < spare ? __popcll(eq) : spare;
+        }
+        const uint64_t m = __ballot(take);
+        if (take) {
+            const int at = base + __popcll(m & below);
+            skey[w][at] = key[i];
+            sidx[w][at] = x;
+        }
+        base += __popcll(m);
+        y[i % 8] = take || x >= a.V ? NEG_INF : key_value(key[i]);
+        mx = fmaxf(mx, y[i % 8]);
+        if (i % 8 == 7 || i == R - 1) {
+            acc.add(y, R < 8 ? R : 8, mx, a.c);
+            mx = NEG_INF;
+        }
+    }
+    if (lane < 4) skey[w][a.k + lane] = 0;  // (the ranking reads four at a time)
+    MaxSum rest = acc.done(a.c);
+    rest.wave(a.c);
+    wave_sync();
+    T* val = static_cast<T*>(a.values) + (size_t)r * a.k;
+    int64_t* idx = a.indices + (size_t)r * a.k;
+    for (int j = lane; j < a.k; j += 64) {
+        const uint32_t kj = skey[w][j];
+        int rank = 0;
+        for (int l = 0; l < a.k; l += 4)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t kl = skey[w][l + e];
+                rank += kl > kj || (kl == kj && l + e < j);
+            }
+        val[rank] = (T)key_value(kj);
+        idx[rank] = sidx[w][j];
     }
     if (lane == 0) a.rest[r] = rest_logit(rest, a.T);
 }
@@ -1483,6 +1568,8 @@ static Split row_split(int64_t rows, int V) {
 
 using namespace ugpg;
 
+constexpr int TOPW_MAX = 1024;  // classes of a row that one wave holds
+
 extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, int64_t inner,
                                int64_t stride, int k, float temperature, void* values,
                                int64_t* indices, float* rest, void* stream) {
@@ -1517,6 +1604,12 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
 #undef TOP_MAP
     } else if (V <= 64) {
         TOP_GO((top_wave_kernel<float>), (top_wave_kernel<__bf16>), cdiv(N, 4), 256);
+    } else if (V <= 256) {
+        TOP_GO((top_wide_wave_kernel<float, 4>), (top_wide_wave_kernel<__bf16, 4>), cdiv(N, 4), 256);
+    } else if (V <= 512) {
+        TOP_GO((top_wide_wave_kernel<float, 8>), (top_wide_wave_kernel<__bf16, 8>), cdiv(N, 4), 256);
+    } else if (V <= TOPW_MAX) {
+        TOP_GO((top_wide_wave_kernel<float, 16>), (top_wide_wave_kernel<__bf16, 16>), cdiv(N, 4), 256);
     } else {
         // twice as many maxima as entries keep the first bound near the k-th; about 3.2 k vectors
         // are set aside (all, up to 512 classes)
