@@ -1112,35 +1112,32 @@ template <typename T, int NT, int CAP> __global__ void __launch_bounds__(NT, 8) 
     };
     // tiles of nt vectors; the row's ends belong to the first segment
     const int tiles = (sp.nv + nt - 1) / nt;
-    int end = tiles;
-    if (a.V > TK_NEAR) {
-        end = (tiles + a.first - 1) / a.first;
-        float mx = NEG_INF;
-        const int last = end * nt < sp.nv ? end * nt : sp.nv;
-        int i = tid;
-        for (; i + (U - 1) * nt < last; i += U * nt) {
-            Pack<T, N> v[U];
+    int end = (tiles + a.first - 1) / a.first;
+    float mx = NEG_INF;
+    const int last = end * nt < sp.nv ? end * nt : sp.nv;
+    int i = tid;
+    for (; i + (U - 1) * nt < last; i += U * nt) {
+        Pack<T, N> v[U];
 #pragma unroll
-            for (int u = 0; u < U; ++u) v[u].load(body + (size_t)(i + u * nt) * N);
+        for (int u = 0; u < U; ++u) v[u].load(body + (size_t)(i + u * nt) * N);
 #pragma unroll
-            for (int u = 0; u < U; ++u) mx = fmaxf(mx, top_of(v[u]));
-        }
-        for (; i < last; i += nt) {
-            Pack<T, N> v;
-            v.load(body + (size_t)i * N);
-            mx = fmaxf(mx, top_of(v));
-        }
-        sp.ends(tid, nt, [&](int, int, const Pack<T, N>& v, int) { mx = fmaxf(mx, top_of(v)); });
-        s.mx[tid] = mx;
-        __syncthreads();
-        if (tid < 64) {
-            const uint32_t t = kth_prefix(nt, a.k, [&](int i) { return order_key(s.mx[i]); });
-            if (lane == 0) s.tau = t;
-        }
+        for (int u = 0; u < U; ++u) mx = fmaxf(mx, top_of(v[u]));
+    }
+    for (; i < last; i += nt) {
+        Pack<T, N> v;
+        v.load(body + (size_t)i * N);
+        mx = fmaxf(mx, top_of(v));
+    }
+    sp.ends(tid, nt, [&](int, int, const Pack<T, N>& v, int) { mx = fmaxf(mx, top_of(v)); });
+    s.mx[tid] = mx;
+    __syncthreads();
+    if (tid < 64) {
+        const uint32_t t = kth_prefix(nt, a.k, [&](int i) { return order_key(s.mx[i]); });
+        if (lane == 0) s.tau = t;
     }
     if (tid == 0) s.n = s.nn = 0;
     __syncthreads();
-    if (a.V > TK_NEAR) tau = prefix_value(s.tau);
+    tau = prefix_value(s.tau);
     sp.ends(tid, nt, [&](int, int i0, const Pack<T, N>& v, int cnt) { eat(i0, v, cnt); });
     int n = 0;
     for (int t = 0;;) {
@@ -1612,7 +1609,7 @@ extern "C" int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, 
         TOP_GO((top_wide_wave_kernel<float, 16>), (top_wide_wave_kernel<__bf16, 16>), cdiv(N, 4), 256);
     } else {
         // twice as many maxima as entries keep the first bound near the k-th; about 3.2 k vectors
-        // are set aside (all, up to 512 classes)
+        // are set aside
         if (k <= 64 && V <= 4096) TOP_GO((top_row_kernel<float, 128, 256>), (top_row_kernel<__bf16, 128, 256>), N, 128);
         else if (k <= 128 && V <= 16384) TOP_GO((top_row_kernel<float, 256, 512>), (top_row_kernel<__bf16, 256, 512>), N, 256);
         else TOP_GO((top_row_kernel<float, 512, 1024>), (top_row_kernel<__bf16, 512, 1024>), N, 512);
