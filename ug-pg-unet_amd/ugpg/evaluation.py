@@ -23,7 +23,7 @@ import torch
 import torch.nn as nn
 
 from . import ops
-from .unet import PGUNet1, PGUNet2, PGUNet3, PGUNet4
+from .unet import PGUNet1, PGUNet2, PGUNet3, PGUNet4, checkpoint_groups
 
 METRIC_KEYS = ("iou", "dice", "accuracy", "precision", "recall", "specificity")
 _STAGE_MODELS = {1: PGUNet1, 2: PGUNet2, 3: PGUNet3, 4: PGUNet4}
@@ -91,14 +91,12 @@ class MoNuSegTester:
             stage, state = 4, ckpt
         else:
             raise RuntimeError(f"Unrecognized checkpoint format for: {model_path}")
-        # a model without running statistics was trained with norm="group"
-        norm, groups = "batch", 32
-        if not any(k.endswith("running_mean") for k in state):
-            norm, groups = "group", ckpt.get("norm_groups", self.norm_groups)
-            if groups is None or (self.norm_groups or groups) != groups:
-                raise RuntimeError(f"{model_path} holds a group-norm model of {groups or 'unknown'} groups: "
-                                   f"give norm_groups (given: {self.norm_groups})")
-        model = _STAGE_MODELS.get(stage, PGUNet4)(in_channels=3, num_classes=1, norm=norm, groups=int(groups))
+        try:
+            groups = checkpoint_groups(ckpt, state, self.norm_groups, model_path)
+        except ValueError as e:
+            raise RuntimeError(str(e)) from None
+        norm = {} if groups is None else {"norm": "group", "groups": groups}
+        model = _STAGE_MODELS.get(stage, PGUNet4)(in_channels=3, num_classes=1, **norm)
         model.load_state_dict(state)
         self.stage = stage
         return model.to(self.device)

@@ -37,7 +37,8 @@ from .dist import (allreduce_gradients, allreduce_metrics, broadcast_buffers,
                    broadcast_parameters, overlapped_allreduce, shard_batch,
                    sync_batchnorm_from_env, world)
 from .optim import Adam
-from .unet import STAGE_CLASSES, STAGE_RESOLUTIONS, _LAYOUT
+from .unet import (NORM_GROUPS, STAGE_CLASSES, STAGE_RESOLUTIONS, _LAYOUT, check_model_groups,
+                   norm_record)
 
 FEATURE_DIM = 512  # output width of inc (stage 1) / down3 (stages 2-4)
 
@@ -103,17 +104,20 @@ def _dropout(x, p, training):
 
 class HerlevClassificationModel(nn.Module):
     def __init__(self, stage: int, num_classes: int, pretrained_unet_path: str = None,
-                 norm: str = "batch", norm_groups: int = 32):
+                 norm: str = "batch", norm_groups: int = None):
+        """norm_groups: the group count of norm="group" (32); a pretrained checkpoint that does
+        not name its own needs it given."""
         super().__init__()
         self.stage = stage
         self.num_classes = num_classes
-        self.unet = STAGE_CLASSES[stage](in_channels=3, num_classes=1, norm=norm, groups=norm_groups)
+        self.unet = STAGE_CLASSES[stage](in_channels=3, num_classes=1, norm=norm,
+                                         groups=NORM_GROUPS if norm_groups is None else norm_groups)
         if pretrained_unet_path and os.path.exists(pretrained_unet_path):
             print(f"Loading pretrained U-Net weights from: {pretrained_unet_path}")
             sd = torch.load(pretrained_unet_path, map_location="cpu", weights_only=True)
-            if "model_state_dict" in sd:
-                sd = sd["model_state_dict"]
-            self.unet.load_state_dict(sd)
+            state = sd["model_state_dict"] if "model_state_dict" in sd else sd
+            check_model_groups(sd, state, self.unet, norm_groups, pretrained_unet_path)
+            self.unet.load_state_dict(state)
         # the reference's feature-width probe: same RNG draw, same point (train_herlev.py:59-63)
         res = STAGE_RESOLUTIONS[stage]
         self._probe = torch.randn(1, 3, res, res)
@@ -217,7 +221,7 @@ class HerlevTrainer:
                 stage, config["num_classes"],
                 config.get("pretrained_unet_paths", {}).get(stage),
                 norm=config.get("norm", "batch"),
-                norm_groups=config.get("norm_groups", 32)).to(self.device)
+                norm_groups=config.get("norm_groups")).to(self.device)
         self.setup_loss_function()
         self.uncertainty_loss = UncertaintyGuidedLoss(self.device)
         self.uncertainty_alpha = config.get("uncertainty_alpha", 1.0)
@@ -401,7 +405,7 @@ class HerlevTrainer:
                                     "stage": stage, "epoch": epoch + 1,
                                     "train_loss": tr_loss, "val_loss": va_loss,
                                     "train_acc": tr_acc, "val_acc": va_acc,
-                                    "config": self.config},
+                                    "config": self.config, **norm_record(self.models[stage])},
                                    os.path.join(save_dir, f"herlev_stage{stage}_best.pth"))
                     print(f"New best model saved! Val Acc: {va_acc:.2f}%")
                 else:

@@ -27,7 +27,8 @@ from .dist import (allreduce_gradients, allreduce_metrics, broadcast_buffers,
 from .graphs import StepGraph
 from .loss import UncertaintyGuidedLoss, weighted_loss_tensors
 from .optim import RMSprop
-from .unet import PGUNet1, PGUNet2, PGUNet3, PGUNet4, ProgressiveUNet
+from .unet import (NORM_GROUPS, PGUNet1, PGUNet2, PGUNet3, PGUNet4, ProgressiveUNet,
+                   check_model_groups, norm_record)
 
 try:  # plotting is optional, as in the reference
     import matplotlib
@@ -61,10 +62,12 @@ class MetricsReadback:
 
 class UncertaintyGuidedProgressiveTrainer:
     def __init__(self, in_channels=3, num_classes=1, device="cuda", uncertainty_alpha=1.0,
-                 norm="batch", norm_groups=32):
-        """norm, norm_groups: the models' normalisation (PGUNet1-4's `norm`, `groups`)."""
+                 norm="batch", norm_groups=None):
+        """norm, norm_groups (32): the models' normalisation (PGUNet1-4's `norm`, `groups`); a
+        checkpoint that does not name its group count loads only where norm_groups is given."""
         self.device = device
-        self.norm, self.norm_groups = norm, norm_groups
+        self.norm, self.groups_given = norm, norm_groups
+        self.norm_groups = NORM_GROUPS if norm_groups is None else norm_groups
         self.in_channels = in_channels
         self.num_classes = num_classes
         self.uncertainty_alpha = uncertainty_alpha
@@ -74,7 +77,7 @@ class UncertaintyGuidedProgressiveTrainer:
             3: {"resolution": 128, "epochs_per_stage": 40, "lr": 1e-4},
             4: {"resolution": 256, "epochs_per_stage": 40, "lr": 1e-4},
         }
-        self.models = {s: cls(in_channels, num_classes, norm, norm_groups).to(device)
+        self.models = {s: cls(in_channels, num_classes, norm, self.norm_groups).to(device)
                        for s, cls in ((1, PGUNet1), (2, PGUNet2), (3, PGUNet3), (4, PGUNet4))}
         self.current_stage = 1
         self.current_model = self.models[1]
@@ -400,8 +403,7 @@ class UncertaintyGuidedProgressiveTrainer:
                                     "val_dice": va[2], "train_dice": tr[2],
                                     "uncertainty_alpha": self.uncertainty_alpha,
                                     "history": self.history,
-                                    **({"norm_groups": self.norm_groups}
-                                       if getattr(self, "norm", "batch") == "group" else {})},
+                                    **norm_record(self.current_model)},
                                    save_path / f"ug_pgunet_stage{stage}_best.pth")
                 print("-" * 60)
             # the finished stage becomes the next stage's U-map producer: one BN state
@@ -440,11 +442,9 @@ class UncertaintyGuidedProgressiveTrainer:
         models[stage] (uncertainty_guided_trainer.py:469-473).  COLLECTIVE under data
         parallelism: every rank calls it, then rank 0's weights are broadcast."""
         ck = torch.load(checkpoint_path, map_location=self.device, weights_only=True)
-        groups = ck.get("norm_groups")
-        if groups is not None and groups != self.norm_groups:
-            raise ValueError(f"{checkpoint_path} was trained with {groups} norm groups, this trainer "
-                             f"has {self.norm_groups}")
-        self.models[stage].load_state_dict(ck["model_state_dict"] if "model_state_dict" in ck else ck)
+        state = ck["model_state_dict"] if "model_state_dict" in ck else ck
+        check_model_groups(ck, state, self.models[stage], self.groups_given, checkpoint_path)
+        self.models[stage].load_state_dict(state)
         self.sync_replicas([stage])
         print(f"Loaded weights for stage {stage} from {checkpoint_path}")
 

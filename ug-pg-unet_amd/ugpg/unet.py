@@ -138,6 +138,38 @@ def resize_input(x, res):
     return ops.resize_nchw(x.detach().float(), res, res, ops.RESIZE_BILINEAR)
 
 
+NORM_GROUPS = 32  # groups of norm="group" where nobody says
+
+
+def checkpoint_groups(ckpt, state, given, path):
+    """The group count of a checkpoint's group norms, or None where it holds BatchNorm's running
+    statistics.  The count is no part of a state_dict and no shape depends on it, so a wrong one
+    would load and compute another function: it is recorded beside the state as "norm_groups",
+    or `given` by the caller, else the checkpoint is refused."""
+    if any(k.endswith("running_mean") for k in state):
+        return None
+    said = ckpt.get("norm_groups")
+    if said is None and given is None:
+        raise ValueError(f"{path} holds a group-norm model and does not say its group count: give norm_groups")
+    if said is not None and given is not None and int(said) != int(given):
+        raise ValueError(f"{path} was trained with {said} norm groups, norm_groups is {given}")
+    return int(given if said is None else said)
+
+
+def norm_record(model):
+    """What a checkpoint of `model` records of its normalisation."""
+    groups = next((m.num_groups for m in model.modules() if isinstance(m, nn.GroupNorm)), None)
+    return {} if groups is None else {"norm_groups": groups}
+
+
+def check_model_groups(ckpt, state, model, given, path):
+    """Refuse a checkpoint for a group-norm model that it is not known to fit."""
+    groups = norm_record(model).get("norm_groups")
+    found = None if groups is None else checkpoint_groups(ckpt, state, given, path)
+    if found is not None and found != groups:
+        raise ValueError(f"{path} was trained with {found} norm groups, this model has {groups}: give norm_groups")
+
+
 def transfer_state(prev_stage_dict, current_stage_dict):
     """Name-matched (partial) copy of a previous stage's tensors (UG_unet.py:345-411).
 
