@@ -73,6 +73,14 @@ void check_capture(const char* what, std::initializer_list<const Tensor*> inputs
     }
 }
 
+// A tangent of forward-mode differentiation would be left out of the result: refused, for
+// constants of a loss too.  (Undefined wherever forward mode is off.)
+void check_tangents(const char* what, std::initializer_list<const Tensor*> inputs) {
+    for (const Tensor* t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what,
+                                    ": forward-mode derivatives are not implemented");
+}
+
 // The gradients of a backward that runs with create_graph: differentiating through one of them
 // raises, whether or not the upstream gradient required one.
 void once(const char* what, variable_list& grads) {
@@ -158,8 +166,9 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
 bool wants(const Maybe& t) { return t.has_value() && t->defined() && t->requires_grad(); }
 
 Tensor group_norm_act(const Tensor& x, const Maybe& w, const Maybe& b, int64_t groups, double eps, int64_t act) {
+    const Tensor none;
+    check_tangents("group_norm_act", {&x, w ? &*w : &none, b ? &*b : &none});
     if (c10::GradMode::is_enabled() && (wants(x) || wants(w) || wants(b))) {
-        const Tensor none;
         check_capture("group_norm_act", {&x, w ? &*w : &none, b ? &*b : &none});
         return GroupNormAct::apply(x, w, b, groups, eps, act);
     }
@@ -265,6 +274,8 @@ struct Distill : torch::autograd::Function<Distill> {
 
 Tensor distill(const Tensor& logits, const Tensor& values, const Tensor& indices, const Maybe& rest,
                const Maybe& weight, double T, double scale, bool per_row) {
+    const Tensor none;
+    check_tangents("distillation_loss", {&logits, &values, rest ? &*rest : &none, weight ? &*weight : &none});
     if (c10::GradMode::is_enabled() && logits.requires_grad()) {
         check_capture("distillation_loss", {&logits});
         return Distill::apply(logits, values, indices, rest, weight, T, scale, per_row);
