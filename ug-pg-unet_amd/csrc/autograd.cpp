@@ -10,10 +10,12 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include <optional>
 #include <string>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/ugpg.h"
@@ -70,6 +72,33 @@ void check_capture(const char* what, std::initializer_list<const Tensor*> inputs
         const auto s = node ? node->stream() : std::nullopt;
         TORCH_CHECK(!s || s->id() != 0, what, ": captured while a graph of the same input lives on the "
                     "default stream; drop that graph first, or run it on another stream");
+    }
+}
+
+// The same for what lies behind this node: a captured backward that is about to run into a node of
+// the default stream (a view or a cast of a leaf whose eager graph lives, say) ends here, with
+// an error, while that stream is untouched.  Only nodes that this pass executes count.
+void check_captured_backward(const char* what) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+    const auto self = torch::autograd::get_current_node();
+    const auto* info = torch::autograd::get_current_graph_task_exec_info();  // empty: all execute
+    std::unordered_set<torch::autograd::Node*> seen;
+    std::vector<torch::autograd::Node*> todo{self.get()};
+    while (!todo.empty()) {
+        torch::autograd::Node* const node = todo.back();
+        todo.pop_back();
+        for (const auto& edge : node->next_edges()) {
+            torch::autograd::Node* const next = edge.function.get();
+            if (!next || !seen.insert(next).second) continue;
+            if (info && !info->empty()) {
+                const auto it = info->find(next);
+                if (it == info->end() || !it->second.should_execute()) continue;
+            }
+            const auto s = next->stream();
+            TORCH_CHECK(!s || s->id() != 0, what, ": its backward is captured while a graph of the same "
+                        "input lives on the default stream; drop that graph first, or run it on another stream");
+            todo.push_back(next);
+        }
     }
 }
 
@@ -143,6 +172,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
         const variable_list s = ctx->get_saved_variables();  // (raises if one was written in place since)
         const Tensor &x = s[0], &w = s[1], &b = s[2];
         c10::OptionalDeviceGuard guard(x.device());
+        check_captured_backward("group_norm_act");
         const Tensor dy = up[0].detach().to(x.scalar_type()).contiguous();
         const ugpg_group_norm_t d = gn_desc(x, ctx->saved_data["groups"].toInt(), some(w), some(b), 0.0,
                                             ctx->saved_data["act"].toInt(), s[3]);
@@ -248,6 +278,7 @@ struct Distill : torch::autograd::Function<Distill> {
         const variable_list s = ctx->get_saved_variables();  // (raises if one was written in place since)
         const Tensor& logits = s[0];
         c10::OptionalDeviceGuard guard(logits.device());
+        check_captured_backward("distillation_loss");
         const Tensor z = class_rows(logits.detach());
         const ugpg_distill_t d = ds_desc(logits, z, s[1], s[2], some(s[3]), some(s[4]),
                                          ctx->saved_data["T"].toDouble(), ctx->saved_data["scale"].toDouble());
