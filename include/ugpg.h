@@ -522,7 +522,8 @@ int ugpg_mul(const float* x, const float* m, float* y, int64_t n, void* stream);
  *   y = act(xh * gamma + beta)
  * mean, rstd [B][G] fp32 are written (the backward reads them).  Statistics are centred
  * (no sum of squares), sums have a fixed order.  The normalisation of a DoubleConv whose
- * batch is too small for BatchNorm; the reference has BatchNorm only. */
+ * batch is too small for BatchNorm; the reference has BatchNorm only.  B * G < 2^22,
+ * C <= 2^20, B * ceil(C / 256) <= 2^22. */
 #define UGPG_ACT_NONE 0
 #define UGPG_ACT_RELU 1
 #define UGPG_ACT_SILU 2
@@ -557,7 +558,8 @@ int ugpg_group_norm_bwd(const ugpg_group_norm_t* p, const void* dy, int dy_dtype
  * of its output, and the loss of the current stage against that record.
  * Rows: N rows of V logits (inner == 1; row r at logits + r*stride, stride >= V), or the
  * pixels of N class maps [V][inner] (inner > 1, stride == V*inner).  dtype UGPG_DT_F32 or
- * UGPG_DT_BF16.  1 <= k <= min(V, 256), T in 1e-30..1e30, at most 2^22 rows or 2^30 pixels.
+ * UGPG_DT_BF16.  1 <= k <= min(V, 256), T in 1e-30..1e30, V <= 2^30, at most 2^22 rows or
+ * 2^30 - 64 pixels.
  * With t a row's logits at temperature T:
  *   values, indices [N][k][inner]: the k largest, the larger first, equal ones by the lower
  *     index (a NaN counts as the largest); values have the logits' type

@@ -1533,8 +1533,9 @@ static int rows_check(const char* what, const void* logits, int dtype, int64_t N
                   (long long)inner);
         return UGPG_ERR_INVALID;
     }
-    // (grids below 2^32 threads, up to four a pixel; V leaves room for a span's padding in 32 bits)
-    if (V > (1 << 30) || (inner == 1 ? N > (1 << 22) : N > (int64_t)0x3fffffff / inner)) {
+    // (grids below 2^32 threads, up to four a pixel in blocks of 64 pixels; V leaves room for a
+    // span's padding in 32 bits)
+    if (V > (1 << 30) || (inner == 1 ? N > (1 << 22) : N > (int64_t)((1 << 30) - 64) / inner)) {
         set_error("%s: N=%lld V=%d inner=%lld is too large", what, (long long)N, V, (long long)inner);
         return UGPG_ERR_INVALID;
     }

@@ -952,8 +952,9 @@ static int gn_check(const char* what, const ugpg_group_norm_t* p, bool tensors) 
         set_error("%s: x, mean and rstd must be given, x aligned to its type", what);
         return UGPG_ERR_INVALID;
     }
-    // (grids: B*G blocks, B * column blocks; offsets are 64-bit)
-    if (p->C > (1 << 20) || (int64_t)p->B * p->G > (1 << 22) ||
+    // (grids: B*G blocks of up to 1024 threads, below 2^32 in all; B * column blocks; offsets
+    // are 64-bit)
+    if (p->C > (1 << 20) || (int64_t)p->B * p->G >= (1 << 22) ||
         (int64_t)p->B * cdiv(p->C, 256) > (1 << 22) || p->HW > ((int64_t)1 << 40) ||
         (double)p->B * (double)p->HW * (double)p->C > 1e15) {
         set_error("%s: B=%d HW=%lld C=%d is too large", what, p->B, (long long)p->HW, p->C);

@@ -35,6 +35,11 @@ def _check_logits(what, logits):
         raise ValueError(f"{what}: empty logits {tuple(logits.shape)}")
     if logits.shape[1] > 1 << 30:
         raise ValueError(f"{what}: {logits.shape[1]} classes are too many")
+    rows = logits.numel() // logits.shape[1]
+    if rows > ops.ROWS_MAX and rows == logits.shape[0]:
+        raise ValueError(f"{what}: {rows} rows, at most {ops.ROWS_MAX} rows a call")
+    if rows > ops.PIXELS_MAX:
+        raise ValueError(f"{what}: {rows} pixels, at most {ops.PIXELS_MAX} pixels a call")
 
 
 def _check_temperature(what, t):
@@ -50,7 +55,8 @@ def _check_device(what, logits):
 def teacher_top_logits(logits, k, temperature=1.0):
     """The ``k`` largest logits of every row of (N, V) -- or of every pixel of (N, V, *spatial)
     -- the larger first and equal ones by the lower index, and the rest's logit at
-    ``temperature``.  float32 or bfloat16; 1 <= k <= min(V, 256).  A constant: no gradient."""
+    ``temperature``.  float32 or bfloat16; 1 <= k <= min(V, 256); at most 2^22 rows, or 2^30 - 64
+    pixels.  A constant: no gradient."""
     what = "teacher_top_logits"
     _check_logits(what, logits)
     _check_temperature(what, temperature)
@@ -68,7 +74,8 @@ def distillation_loss(logits, top, temperature=1.0, weight=None, reduction="mean
     distributions live on its classes and, where it has a ``rest``, all the others as one.
     ``weight``: one float32 factor a row (N, *spatial); a row of weight 0 gives neither loss
     nor gradient, whatever it holds.  ``reduction``: "mean" (over all rows, as the
-    uncertainty-weighted loss), "sum" or "none".  Class maps have at most 1024 classes.
+    uncertainty-weighted loss), "sum" or "none".  Class maps have at most 1024 classes;
+    rows and pixels as for teacher_top_logits.
     The gradient goes to ``logits`` alone (once); record and weight are constants."""
     what = "distillation_loss"
     _check_logits(what, logits)

@@ -19,7 +19,8 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
 
     Statistics run over a sample's middle dimensions and its C/num_groups consecutive
     channels, in float32.  weight, bias: (C,) float32 or None.  activation: "relu", "silu"
-    or "none".  Differentiable in x, weight and bias (once)."""
+    or "none".  Differentiable in x, weight and bias (once).  Less than 2^22 groups over the whole
+    batch, at most 2^20 channels."""
     if x.dim() < 2:
         raise ValueError(f"group_norm_act: expected (B, ..., C), got shape {tuple(x.shape)}")
     c = x.shape[-1]
@@ -41,12 +42,14 @@ def group_norm_act(x, num_groups, weight=None, bias=None, eps=1e-5, activation="
             raise TypeError(f"group_norm_act: {name} must be float32, got {p.dtype}")
         if p.device != x.device:
             raise RuntimeError(f"group_norm_act: {name} is on {p.device}, x on {x.device}")
-    if not x.is_cuda:
-        raise RuntimeError("ugpg: tensor is not on a ROCm/HIP device (no CPU fallback)")
     if x.numel() == 0:
         raise ValueError(f"group_norm_act: empty input {tuple(x.shape)}")
-    if x.shape[0] > 1 << 30 or c > 1 << 20:
+    if x.shape[0] * num_groups >= 1 << 22:
+        raise ValueError(f"group_norm_act: {x.shape[0]} samples of {num_groups} groups are {1 << 22} or more")
+    if c > 1 << 20 or x.shape[0] * -(-c // 256) > 1 << 22:
         raise ValueError(f"group_norm_act: {x.shape[0]} samples of {c} channels are too many")
+    if not x.is_cuda:
+        raise RuntimeError("ugpg: tensor is not on a ROCm/HIP device (no CPU fallback)")
     if not x.is_contiguous():
         x = x.contiguous()
     if weight is not None and not weight.is_contiguous():

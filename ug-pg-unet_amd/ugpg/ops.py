@@ -862,6 +862,8 @@ def ce_ug_bwd(x, y, wts, class_weights, gout):
 # limits of teacher_top_logits and distillation_loss (csrc/distill.hip)
 TOP_MAX = 256        # entries of a teacher's record
 MAP_CLASSES = 1024   # classes of the maps distillation reads
+ROWS_MAX = 1 << 22
+PIXELS_MAX = (1 << 30) - 64
 
 
 def adam_step(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, grad_scale=1.0):
