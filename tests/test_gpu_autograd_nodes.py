@@ -68,3 +68,78 @@ def test_captured_backward_into_a_living_eager_graph_is_refused(dev):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_recomputed_and_from_two_threads(dev):
+    """Under activation checkpointing, and in two host threads on streams of their own, the
+    gradients are the plain call's bits."""
+    import threading
+
+    import ugpg
+    from torch.utils.checkpoint import checkpoint
+    torch.manual_seed(7)
+    top = ugpg.teacher_top_logits(torch.randn(2, 24, 16, 12, device=dev), 3, 2.0)
+    x0 = torch.randn(2, 16, 12, 24, device=dev)
+    w0, b0 = torch.rand(24, device=dev) + 0.5, torch.randn(24, device=dev)
+
+    def both(x, w, b):
+        y = ugpg.group_norm_act(x, 4, w, b, 1e-5, "silu")
+        return ugpg.distillation_loss(y.movedim(-1, 1), top, 2.0)
+
+    def grads(run, scale):
+        leaf = [t.clone().requires_grad_(True) for t in (x0, w0, b0)]
+        loss = run(*leaf)
+        return (loss.detach(), *torch.autograd.grad(scale * loss, leaf))
+    want = {s: grads(both, s) for s in (1.0, 3.0)}
+    for s in want:
+        got = grads(lambda *a: checkpoint(both, *a, use_reentrant=False), s)
+        assert all(torch.equal(p, q) for p, q in zip(got, want[s]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(s):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = grads(both, s)
+                stream.synchronize()
+                if not all(torch.equal(p, q) for p, q in zip(got, want[s])):
+                    wrong.append(s)
+    threads = [threading.Thread(target=work, args=(s,)) for s in want]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_graphed_callables(dev):
+    """Forward and backward captured apart (torch.cuda.make_graphed_callables), replayed with new
+    inputs and upstream factors."""
+    import ugpg
+    torch.manual_seed(8)
+    top = ugpg.teacher_top_logits(torch.randn(40, 24, device=dev), 3, 2.0)
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.norm = ugpg.GroupNormAct(4, 24, activation="silu")
+
+        def forward(self, x):
+            return ugpg.distillation_loss(self.norm(x), top, 2.0)
+    eager = Net().to(dev)
+    graphed = Net().to(dev)
+    graphed.load_state_dict(eager.state_dict())
+    graphed = torch.cuda.make_graphed_callables(graphed, (torch.randn(40, 24, device=dev, requires_grad=True),))
+    for k in range(4):
+        x = torch.randn(40, 24, device=dev)
+        out = []
+        for net in (eager, graphed):
+            leaf = x.clone().requires_grad_(True)
+            loss = net(leaf) * (1.0 if k % 2 else 2.5)
+            loss.backward()
+            out.append([loss.detach().clone(), leaf.grad.clone(),
+                        *(p.grad.clone() for p in net.parameters())])
+            net.zero_grad(set_to_none=True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(*out)), k
