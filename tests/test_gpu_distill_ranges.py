@@ -1,0 +1,64 @@
+"""Logits on both sides of a power of two, far from zero: a thread's running maximum rises many times
+while its product with log2(e) / T carries few digits after the point.
+
+The rest's logit is T log S + m with S off by REL = 2^-15 of itself (128 additions at most in these
+rows, exponents of at most 126); a loss by REL of a unit of KL, a gradient by REL (p + q), as in
+tests/test_gpu_distill.py; and half a step of what is stored."""
+import math
+
+import pytest
+import torch
+
+from tests.test_gpu_distill import check_grad, check_loss, ref_loss, ref_top
+
+pytestmark = pytest.mark.gpu
+REL = 2.0 ** -15
+# a wave a row (64, 512, 1024 classes), a block a row, class maps of one and four threads a pixel
+FORMS = [((70, 50), 5), ((9, 300), 20), ((9, 900), 20), ((3, 5000), 64), ((2, 40001), 100),
+         ((2, 12, 5, 7), 3), ((1, 80, 6, 5), 4)]
+# the loss: a wave a row, a block a row, a row over several blocks, maps
+LOSSES = [((16, 50), 5), ((70, 500), 20), ((300, 1500), 20), ((3, 9001), 20), ((2, 8, 5, 7), 3), ((1, 24, 5, 7), 12),
+          ((1, 80, 6, 5), 4)]
+
+
+def check_rest(top, z, k, T, what):
+    v, i, r = ref_top(z, k, T)
+    assert torch.equal(top.indices, i) and torch.equal(top.values.double(), v), what
+    lim = T * REL + 2.0 ** -23 * r.abs()
+    bad = ~((top.rest.double() == r) | ((top.rest.double() - r).abs() <= lim))
+    assert not bad.any(), (what, top.rest[bad][:3].tolist(), r[bad][:3].tolist())
+
+
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+@pytest.mark.parametrize("bits", [10, 16, 19, 20, 21, 24, 30])
+def test_rows_across_a_magnitude(dev, bits, sign):
+    """Values within a few units of sign * T 2^bits ln 2 (an exponent of 2^bits), rising and falling,
+    so that a thread's maximum crosses it in either direction."""
+    import ugpg
+    for shape, k in FORMS:
+        for T in (1.0, 3.0):
+            mid = sign * T * 2.0 ** bits * math.log(2.0)
+            ramp = torch.linspace(-6.0 * T, 6.0 * T, shape[1], device=dev).view(1, -1, *[1] * (len(shape) - 2))
+            for way in (1.0, -1.0):
+                z = (mid + way * ramp).expand(shape).contiguous()
+                check_rest(ugpg.teacher_top_logits(z, k, T), z, k, T, (shape, T, way))
+
+
+@pytest.mark.parametrize("bits", [10, 16, 19, 20, 21, 24])
+def test_loss_across_a_magnitude(dev, bits):
+    import ugpg
+    for shape, k in LOSSES:
+        g = torch.Generator(device=dev).manual_seed(bits)
+        for sign in (1.0, -1.0):
+            T = 2.0
+            mid = sign * T * 2.0 ** bits * math.log(2.0)
+            ramp = torch.linspace(-4.0 * T, 4.0 * T, shape[1], device=dev).view(1, -1, *[1] * (len(shape) - 2))
+            z = mid + ramp + torch.randn(shape, generator=g, device=dev)
+            v, i, r = ref_top(z - sign + torch.randn(shape, generator=g, device=dev), k, T)
+            v, i, r = v.float().contiguous(), i.contiguous(), r.float()
+            rows, dz, size, unit = ref_loss(z, v, i, r, None, T, 1.0)
+            zr = z.clone().requires_grad_(True)
+            loss = ugpg.distillation_loss(zr, (v, i, r), T, reduction="sum")
+            check_loss(loss, rows, unit)
+            loss.backward()
+            check_grad(zr.grad, dz, size)

@@ -130,6 +130,8 @@ struct RunSum {
     float m = NEG_INF, mc = NEG_INF, s = 0.f;
     __device__ __forceinline__ void raise(float v, float c) {
         if (v > m) {
+// (s is relative to mc as stored: mc - vc with the rounded vc, never one fma of v * c)
+#pragma clang fp contract(off)
             const float vc = v * c;
             const bool safe = fabsf(mc) < EXP_SAFE && fabsf(vc) < EXP_SAFE;
             s *= exp2_raw(safe ? mc - vc : (m - v) * c);
