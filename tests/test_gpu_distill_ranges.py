@@ -1,5 +1,6 @@
-"""Logits on both sides of a power of two, far from zero: a thread's running maximum rises many times
-while its product with log2(e) / T carries few digits after the point.
+"""Logits and temperatures of every size: masks of -1e9 to the type's lowest value, large positive
+logits, temperatures over the whole documented range, and values on both sides of every
+magnitude at which the kernels change how they take an exponent.
 
 The rest's logit is T log S + m with S off by REL = 2^-15 of itself (128 additions at most in these
 rows, exponents of at most 126); a loss by REL of a unit of KL, a gradient by REL (p + q), as in
@@ -12,6 +13,7 @@ import torch
 from tests.test_gpu_distill import check_grad, check_loss, ref_loss, ref_top
 
 pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
 REL = 2.0 ** -15
 # a wave a row (64, 512, 1024 classes), a block a row, class maps of one and four threads a pixel
 FORMS = [((70, 50), 5), ((9, 300), 20), ((9, 900), 20), ((3, 5000), 64), ((2, 40001), 100),
@@ -29,6 +31,37 @@ def check_rest(top, z, k, T, what):
     assert not bad.any(), (what, top.rest[bad][:3].tolist(), r[bad][:3].tolist())
 
 
+def masked(shape, k, dev, dtype, level, seed=1):
+    """k confident classes a row, all others within a few units of `level`."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    z = level + torch.randn(shape, generator=g, device=dev)
+    pos = torch.arange(shape[1], device=dev).view(1, -1, *[1] * (len(shape) - 2))
+    z = torch.where(pos % (shape[1] // k) == 0, level + abs(level) + 5.0 + pos / shape[1], z)
+    return z.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max).to(dtype)
+
+
+LEVELS = [-1e6, -1e9, -1e10, -1e12, -1e20, -1e30, -3.3e38, 1e6, 1e10, 1e15, 1e30]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("level", LEVELS)
+def test_rest_of_masked_rows(dev, dtype, level):
+    import ugpg
+    for shape, k in FORMS:
+        z = masked(shape, k, dev, dtype, level)
+        for T in (0.25, 1.0, 8.0, 100.0):
+            check_rest(ugpg.teacher_top_logits(z, k, T), z, k, T, (shape, T))
+
+
+@pytest.mark.parametrize("T", [1e-30, 1e-20, 1e-12, 1e-9, 1e-6, 1e-3, 1e3, 1e6, 1e12, 1e30])
+def test_rest_at_every_temperature(dev, T):
+    import ugpg
+    for shape, k in FORMS:
+        g = torch.Generator(device=dev).manual_seed(3)
+        z = 5.0 * torch.randn(shape, generator=g, device=dev) - 3.0
+        check_rest(ugpg.teacher_top_logits(z, k, T), z, k, T, shape)
+
+
 @pytest.mark.parametrize("sign", [1.0, -1.0])
 @pytest.mark.parametrize("bits", [10, 16, 19, 20, 21, 24, 30])
 def test_rows_across_a_magnitude(dev, bits, sign):
@@ -42,6 +75,23 @@ def test_rows_across_a_magnitude(dev, bits, sign):
             for way in (1.0, -1.0):
                 z = (mid + way * ramp).expand(shape).contiguous()
                 check_rest(ugpg.teacher_top_logits(z, k, T), z, k, T, (shape, T, way))
+
+
+@pytest.mark.parametrize("level", LEVELS)
+def test_loss_of_masked_students(dev, level):
+    """All classes outside the record at one far level, in the student and in the teacher."""
+    import ugpg
+    for shape, k in LOSSES:
+        for T in (1.0, 8.0):
+            z = masked(shape, k, dev, F32, level, seed=2)
+            v, i, r = ref_top(masked(shape, k, dev, F32, level, seed=4), k, T)
+            v, i, r = v.float().contiguous(), i.contiguous(), r.float()
+            rows, dz, size, unit = ref_loss(z, v, i, r, None, T, 1.0)
+            zr = z.clone().requires_grad_(True)
+            loss = ugpg.distillation_loss(zr, (v, i, r), T, reduction="sum")
+            check_loss(loss, rows, unit)
+            loss.backward()
+            check_grad(zr.grad, dz, size)
 
 
 @pytest.mark.parametrize("bits", [10, 16, 19, 20, 21, 24])
@@ -62,3 +112,21 @@ def test_loss_across_a_magnitude(dev, bits):
             check_loss(loss, rows, unit)
             loss.backward()
             check_grad(zr.grad, dz, size)
+
+
+@pytest.mark.parametrize("T", [1e-20, 1e-12, 1e-9, 1e-6, 1e-3])
+def test_loss_at_small_temperatures(dev, T):
+    """Here a row's KL is a difference of logits over T: the loss is T^2 of it, whose error beside
+    REL of a unit is a rounding of itself."""
+    import ugpg
+    for shape, k in LOSSES:
+        g = torch.Generator(device=dev).manual_seed(9)
+        z = torch.randn(shape, generator=g, device=dev)
+        v, i, r = ref_top(z + 0.5 * torch.randn(shape, generator=g, device=dev), k, T)
+        v, i, r = v.float().contiguous(), i.contiguous(), r.float()
+        rows, dz, size, unit = ref_loss(z, v, i, r, None, T, 1.0)
+        zr = z.clone().requires_grad_(True)
+        loss = ugpg.distillation_loss(zr, (v, i, r), T, reduction="sum")
+        check_loss(loss, rows, unit)
+        loss.backward()
+        check_grad(zr.grad, dz, size)

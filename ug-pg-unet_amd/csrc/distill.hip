@@ -121,11 +121,16 @@ struct MaxSum {
         m = mm;
     }
 };
-// A product v * c below this is far from overflow, and exp2(v * c - mc) is one fma and one
-// exp2; values near the type's ends take the difference first.
-constexpr float EXP_SAFE = 1e38f;
-// A thread's running form: s = the sum of exp2(v * c - mc), mc = fl(m * c).  The rounding of
-// mc is a factor common to all terms; done() takes it out again.
+// Where |m * c| is below this, exp2(v * c - mc) is one fma and one exp2: the rounding of mc =
+// fl(m * c), at most 2^-5, is a factor common to all terms, which done() takes out again.  Beyond
+// (logits masked with -1e10, say, or a temperature near 0) that factor would leave float32
+// itself: the difference is taken first, exp2((v - m) * c).
+constexpr float EXP_SAFE = 0x1p20f;
+// what mc leaves of m * c
+__device__ __forceinline__ float exp_off(float m, float mc, float c) {
+    return fabsf(mc) < EXP_SAFE ? fmaf(m, c, -mc) : 0.f;
+}
+// A thread's running form: s = the sum of exp2(v * c - mc), or of exp2((v - m) * c).
 struct RunSum {
     float m = NEG_INF, mc = NEG_INF, s = 0.f;
     __device__ __forceinline__ void raise(float v, float c) {
@@ -133,8 +138,9 @@ struct RunSum {
 // (s is relative to mc as stored: mc - vc with the rounded vc, never one fma of v * c)
 #pragma clang fp contract(off)
             const float vc = v * c;
-            const bool safe = fabsf(mc) < EXP_SAFE && fabsf(vc) < EXP_SAFE;
-            s *= exp2_raw(safe ? mc - vc : (m - v) * c);
+            float d = mc - vc;
+            if (!(fmaxf(fabsf(mc), fabsf(vc)) < EXP_SAFE)) d = (m - v) * c + (exp_off(v, vc, c) - exp_off(m, mc, c));
+            s *= exp2_raw(d);
             m = v;
             mc = vc;
         }
@@ -156,7 +162,7 @@ struct RunSum {
     }
     __device__ __forceinline__ void add1(float v, float c) { add(&v, 1, v, c); }
     __device__ __forceinline__ MaxSum done(float c) const {
-        return MaxSum{m, fabsf(mc) < EXP_SAFE ? s * exp2_raw(-fmaf(m, c, -mc)) : s};
+        return MaxSum{m, s * exp2_raw(-exp_off(m, mc, c))};
     }
 };
 
