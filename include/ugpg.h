@@ -563,7 +563,8 @@ int ugpg_group_norm_bwd(const ugpg_group_norm_t* p, const void* dy, int dy_dtype
  * With t a row's logits at temperature T:
  *   values, indices [N][k][inner]: the k largest, the larger first, equal ones by the lower
  *     index (a NaN counts as the largest); values have the logits' type
- *   rest [N][inner]: T * logsumexp(t_v / T) over the others (-inf: none) */
+ *   rest [N][inner]: T * logsumexp(t_v / T) over the others (-inf: none); their sum of
+ *     exponentials is fp32, off by (V / 512 + 64) 2^-24 of itself at most */
 int ugpg_top_logits(const void* logits, int dtype, int64_t N, int V, int64_t inner,
                     int64_t stride, int k, float temperature, void* values, int64_t* indices,
                     float* rest, void* stream);

@@ -657,8 +657,9 @@ __global__ void __launch_bounds__(256) distill_wave_kernel(DistillArgs a) {
 
 // ---------------------------------------------------------------- class maps, a thread each
 // At most VR classes and KR entries: a pixel's logits and record stay in registers, read once.
-// Exponentials are fp32 here (a map's loss is a mean over its pixels), sums and differences
-// fp64.  16 maps of 8 x 256^2 fp32 at 3 entries, with the gradient: 30 us (55 with marks in LDS
+// Exponentials are fp32 here, sums and differences fp64: a pixel's KL is off by 2^-19 of a unit
+// at most (1e-7 in the mean over a map; fp64 exponentials, as a row's terms have, would be k + 1
+// for every pixel).  16 maps of 8 x 256^2 fp32 at 3 entries, with the gradient: 30 us (55 with marks in LDS
 // and the classes read twice); its floor, 113 MB at a copy's 4.8 TB/s, is 24.
 template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) distill_map_small_kernel(DistillArgs a) {
     if (distill_skip(a)) return;
@@ -1080,7 +1081,9 @@ __device__ __forceinline__ float prefix_value(uint32_t t) {
 // quarter (which is read a second time, from the caches) and rises to the k-th maximum of
 // what is set aside before each further segment, which so adds about k vectors.  At the end
 // the values of the vectors set aside are told apart: those near the k-th are ranked by
-// counting, the others join the rest.  What bounds it is the instructions: setting single
+// counting, the others join the rest.  A thread's sum is V / (NT * N) additions deep, V / NT in
+// the exact selection: V / 512 for wide rows.  A row has one block whatever its length: 65537 fp32
+// values take 19 us, 2^20 131, 2^22 628.  What bounds many rows is the instructions: setting single
 // values aside took 196 us for 2048 x 131072 bf16 (22 vector instructions a value), and so did
 // two readings of whole rows; rows held in registers 299 (a block a CU).
 template <typename T, int NT, int CAP> __global__ void __launch_bounds__(NT, 8) top_row_kernel(TopArgs a) {
