@@ -83,7 +83,8 @@ void check_captured_backward(const char* what) {
     const auto self = torch::autograd::get_current_node();
     const auto* info = torch::autograd::get_current_graph_task_exec_info();  // empty: all execute
     std::unordered_set<torch::autograd::Node*> seen;
-    std::vector<torch::autograd::Node*> todo{self.get()};
+    std::vector<torch::autograd::Node*> todo;
+    if (self) todo.push_back(self.get());
     while (!todo.empty()) {
         torch::autograd::Node* const node = todo.back();
         todo.pop_back();
