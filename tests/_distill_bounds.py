@@ -10,10 +10,11 @@ logarithmic derivative, at most 32 KL for exponents up to 16).  The gradient's p
     others (p_rest - q_rest) r_v:  REL r_v (p_rest (1 - p_rest) + |p_rest - q_rest|)
 and half a step of the stored type.
 
-Class maps take the k + 1 exponentials in float32 too: an exponent x below 24 is off by |x| / 2
-steps, its exponential by as much and 2 steps of its own, and |x| p <= 0.37 for p = e^-x, so that
-up to 16 entries on both sides, the rest's sum of at most 64 terms and the common factor make
-less than 32 steps of a unit of KL: MAP = 2^-19."""
+Class maps take the k + 1 exponentials in float32 too: an exponent x = (t - M) c carries three
+roundings, so a probability p = 2^-x is off by 3 ln 2 |x| half steps and 2 of its own; the sum of
+p |x| over a row is its entropy, at most log2(17) = 4.1 with 16 entries: 9 + 2 half steps a side,
+and 8 for the rest's sum of at most 64 terms and the common factor, make less than 32 of 2^-24 of a
+unit of KL: MAP = 2^-19."""
 import math
 
 import torch

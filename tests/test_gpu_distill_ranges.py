@@ -130,3 +130,38 @@ def test_loss_at_small_temperatures(dev, T):
         check_loss(loss, rows, unit)
         loss.backward()
         check_grad(zr.grad, dz, size)
+
+
+@pytest.mark.parametrize("shape,k", [((2, 8, 5, 7), 3), ((1, 16, 5, 7), 8), ((1, 30, 4, 6), 8), ((1, 24, 5, 7), 12),
+                                     ((1, 30, 3, 5), 24), ((1, 80, 6, 5), 4), ((1, 80, 4, 5), 40), ((70, 50), 5),
+                                     ((3, 9001), 20)])
+@pytest.mark.parametrize("bits", [90, 120, 128, 135, 145])
+def test_lowest_logit_against_a_small_probability(dev, shape, k, bits):
+    """A class the teacher keeps at 2^-bits, or its rest at 2^-bits, and the student at the type's lowest
+    value: T^2 times 2^-bits times 3.4e38 / T is most of the loss or a visible part of it.  The exponent
+    (t - M) c, of size `bits`, carries three roundings (the difference, c, the product), 2^-24 of it each,
+    so its exponential is off by 3 bits ln 2 half steps of 2^-24, and 8 more for the exponential itself
+    and the sums; the other terms by REL (rows) or 2^-19 (maps) of the unit."""
+    import ugpg
+    g = torch.Generator(device=dev).manual_seed(bits)
+    low = torch.finfo(F32).min
+    for T in (1.0, 3.0):
+        t = 0.5 * torch.randn(shape, generator=g, device=dev)
+        t[:, :k - 1] += 20.0 * T * math.log(2.0)
+        t[:, k - 1] = t[:, 0] - bits * T * math.log(2.0)
+        for far_rest in (False, True):
+            z = t + 0.1 * torch.randn(shape, generator=g, device=dev)
+            v, i = t[:, :k].clone(), torch.arange(k, device=dev).view(1, k, *[1] * (t.dim() - 2)).expand_as(t[:, :k])
+            r = torch.full_like(t[:, 0], -math.inf)
+            if far_rest:
+                v[:, k - 1] = t[:, 0] - 1.0
+                z[:, k:] = low
+                r = t[:, 0] - bits * T * math.log(2.0)
+            else:
+                z[:, k - 1] = low
+            i = i.contiguous()
+            rows, _, _, unit = ref_loss(z, v, i, r, None, T, 1.0)
+            out = ugpg.distillation_loss(z, (v, i, r), T, reduction="none")
+            lim = (3 * bits * math.log(2.0) + 8) * 2.0 ** -24 * rows.abs() + (REL if z.dim() == 2 else 2.0 ** -19) * unit + 1e-30
+            ok = ((out.double() - rows).abs() <= lim) | ((rows > 3.4e38) & (out == math.inf))
+            assert ok.all(), (T, far_rest, out[~ok][:3].tolist(), rows[~ok][:3].tolist())

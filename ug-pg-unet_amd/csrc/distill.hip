@@ -656,6 +656,17 @@ __global__ void __launch_bounds__(256) distill_wave_kernel(DistillArgs a) {
 }
 
 // ---------------------------------------------------------------- class maps, a thread each
+// The teacher's exp2(x).  Below float32's range it still counts: against a student's logit of the
+// type's lowest value, 3e38, a probability of 2^-130 is a loss of 0.2.
+__device__ __forceinline__ double teacher_exp2(float x) {
+    double e = exp2_raw(x);
+    if (__builtin_expect(x < -100.f, 0)) {
+        const float n = fmaxf(rintf(x), -2000.f);
+        e = x < -2000.f ? 0.0 : ldexp((double)exp2_raw(x - n), (int)n);
+    }
+    return e;
+}
+
 // At most VR classes and KR entries: a pixel's logits and record stay in registers, read once.
 // Exponentials are fp32 here, sums and differences fp64: a pixel's KL is off by 2^-19 of a unit
 // at most (1e-7 in the mean over a map; fp64 exponentials, as a row's terms have, would be k + 1
@@ -714,18 +725,19 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
         for (int j = 0; j < KR; ++j) {
             eq[j] = ep[j] = 0.f;
             if (idx[j] >= 0) {
-                eq[j] = exp2_raw((t[j] - M) * c);
+                const double e = teacher_exp2((t[j] - M) * c);
+                eq[j] = (float)e;
                 ep[j] = exp2_raw((zj[j] - m) * c);
-                sq += eq[j];
+                sq += e;
                 ss += ep[j];
-                if (!(eq[j] == 0.f)) kl += (double)eq[j] * (((double)t[j] - M) - ((double)zj[j] - m));
+                if (!(e == 0.0)) kl += e * (((double)t[j] - M) - ((double)zj[j] - m));
             }
         }
         kl *= iT;
-        const float er = rest == NEG_INF ? 0.f : exp2_raw((rest - M) * c);
+        const double er = rest == NEG_INF ? 0.0 : teacher_exp2((rest - M) * c);
         const float sr = has ? rs.s * exp2_raw((rs.m - m) * c) : rs.s;
-        if (!(er == 0.f))
-            kl += has ? (double)er * ((((double)rest - M) - ((double)rs.m - m)) * iT - log((double)rs.s))
+        if (!(er == 0.0))
+            kl += has ? er * ((((double)rest - M) - ((double)rs.m - m)) * iT - log((double)rs.s))
                       : (double)__builtin_inff();
         sq += er;
         ss += sr;
@@ -737,7 +749,7 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
             T* d = static_cast<T*>(a.dz) + (size_t)n * a.V * a.inner + p;
             const double go = a.gout ? (double)a.gout[a.gout_rows ? r : 0] : 1.0;
             const double g = none ? 0.0 : a.coef * a.T * (double)w * go;
-            const float f = none || !has ? 0.f : (float)(g * ((double)sr * rss - (double)er * rsq) / (double)rs.s);
+            const float f = none || !has ? 0.f : (float)(g * ((double)sr * rss - er * rsq) / (double)rs.s);
             float dk[KR];
 #pragma unroll
             for (int j = 0; j < KR; ++j) dk[j] = none ? 0.f : (float)(g * ((double)ep[j] * rss - (double)eq[j] * rsq));
@@ -758,7 +770,7 @@ template <typename T, int VR, int KR> __global__ void __launch_bounds__(256) dis
 // not fill the card) four threads of different waves, each a part of the classes; the first
 // reads the record and joins the parts.  Marks of the kept classes lie in LDS.  2 maps of 64 x
 // 256^2 fp32, 8 entries, with the gradient: 35 us (a thread a pixel, entries read three times:
-// 87); one of 1000 x 128^2: 67 (690); 8 maps of 16 x 256^2 with 12 entries, the loss: 36, with
+// 87); one of 1000 x 128^2: 67 (690); 8 maps of 16 x 256^2 with 12 entries, the loss: 37, with
 // S = 4 153.  Bound by the record's steps and the classes' second reading.
 constexpr int DM_MAX = 1024;  // classes
 template <typename T, int KR, int S> __global__ void __launch_bounds__(256) distill_map_kernel(DistillArgs a) {
@@ -863,10 +875,10 @@ template <typename T, int KR, int S> __global__ void __launch_bounds__(256) dist
         m = fmaxf(m, rs.m);
         double sq = 0, sp = 0;
         entries(1, [&](int, float t, float zi) {
-            sq += exp2_raw((t - M) * c);
+            sq += teacher_exp2((t - M) * c);
             sp += exp2_raw((zi - m) * c);
         });
-        const float er = rest == NEG_INF ? 0.f : exp2_raw((rest - M) * c);
+        const double er = rest == NEG_INF ? 0.0 : teacher_exp2((rest - M) * c);
         const double iT = (double)c * LN2;  // (see RowTerms)
         const double logr = has ? ((double)rs.m - (double)m) * iT + log((double)rs.s) : (double)NEG_INF;
         const float sr = has ? rs.s * exp2_raw((rs.m - m) * c) : rs.s;
@@ -879,13 +891,13 @@ template <typename T, int KR, int S> __global__ void __launch_bounds__(256) dist
         T* d = static_cast<T*>(a.dz) + (a.dz ? (size_t)n * a.V * a.inner + p : 0);
         double kl = 0;
         entries(2, [&](int i, float t, float zi) {
-            const double q = (double)exp2_raw((t - M) * c) * rsq;
+            const double q = teacher_exp2((t - M) * c) * rsq;
             if (!(q == 0.0))
                 kl += q * ((((double)t - (double)M) * iT - lq) - (((double)zi - (double)m) * iT - ls));
             if (a.dz && on)
                 d[(size_t)i * a.inner] = (T)(none ? 0.f : (float)(g * ((double)exp2_raw((zi - m) * c) * rsp - q)));
         });
-        const double qr = (double)er * rsq;
+        const double qr = er * rsq;
         if (!(qr == 0.0)) kl += qr * ((((double)rest - (double)M) * iT - lq) - (logr - ls));
         l = none || !on ? 0.0 : a.coef * a.T * a.T * (double)w * kl;
         if (a.row_out && on) a.row_out[r] = (float)l;
